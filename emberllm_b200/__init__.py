@@ -13,8 +13,10 @@ import ctypes
 
 from . import _lib as _libmod
 from ._lib import EmberHeader, cuda_available, load
+from .kv4 import Kv4Cache, sample_rows
 
-__all__ = ["Ember", "EmberBatch", "Sampler", "EmberHeader", "cuda_available", "load"]
+__all__ = ["Ember", "EmberBatch", "Sampler", "EmberHeader", "Kv4Cache", "cuda_available", "load",
+           "sample_rows"]
 
 
 class Ember:

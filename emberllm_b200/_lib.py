@@ -1,5 +1,5 @@
 """ctypes binding of libember_b200.so (the C-ABI declared in include/ember.h,
-include/ember_ops.h and include/ember_cuda.h).
+include/ember_ops.h, include/ember_cuda.h and include/ember_kv4.h).
 
 The prototypes for the public API are the ones emberllm's own Python bindings
 declare (bindings/python/emberllm.py:89-109); the rest cover the op-level
@@ -77,6 +77,11 @@ CUDA_SYMBOLS = [
     "ember_cuda_batch_new", "ember_cuda_batch_free", "ember_cuda_batch_prefill", "ember_cuda_batch_greedy",
     "ember_cuda_batch_stream", "ember_batch_new", "ember_batch_cuda", "ember_batch_free", "ember_batch_prefill",
     "ember_batch_greedy",
+]
+
+KV4_SYMBOLS = [
+    "ember_cuda_kv4_bytes", "ember_cuda_kv4_store", "ember_cuda_kv4_read", "ember_cuda_kv4_attention_workspace",
+    "ember_cuda_kv4_attention", "ember_cuda_sample_rows",
 ]
 
 _lib = None
@@ -160,6 +165,13 @@ def load(path=None):
     lib.ember_cuda_available.restype = ctypes.c_int
     lib.ember_cuda_model_bytes.restype = ctypes.c_uint64
     lib.ember_cuda_model_bytes.argtypes = [_P]
+    lib.ember_cuda_kv4_bytes.restype = ctypes.c_size_t
+    lib.ember_cuda_kv4_bytes.argtypes = [ctypes.c_int32] * 4
+    for name in ("store", "read", "attention"):
+        getattr(lib, "ember_cuda_kv4_" + name).argtypes = [_P, _P, _P, _P]
+    lib.ember_cuda_kv4_attention_workspace.restype = ctypes.c_size_t
+    lib.ember_cuda_kv4_attention_workspace.argtypes = [_P] + [ctypes.c_int32] * 4
+    lib.ember_cuda_sample_rows.argtypes = [_P, _P]
     lib.ember_host_rope_table.argtypes = [_P, ctypes.c_int, ctypes.c_int, ctypes.c_float]
     _lib = lib
     return lib

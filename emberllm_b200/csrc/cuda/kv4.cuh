@@ -1,0 +1,65 @@
+// kv4.cuh — layout of the paged 4-bit KV cache and the batch's index arithmetic,
+// shared by the kernels that write it (kv4.cu) and read it (kv4.cu, kv4_attn.cuh).
+//
+// One page of one kv head is one contiguous chunk:
+//
+//     [page_size][hd/2] key codes | [page_size][hd/2] value codes
+//     | [page_size][hd/32] fp16 key scales | [page_size][hd/32] fp16 value scales
+//
+// The order inside a row of codes serves the matrix fragments that the attention
+// builds from it in registers (nb = hd/32 blocks):
+//   keys    word (t, b), t = 0..3, at byte t*(4*nb) + 4*b holds dims b*32 + 8*t + n
+//           in nibble n: lane t of a fragment loads its words of every block at once
+//   values  byte (g, b, j), g = 0..7, j = 0..1, at g*(2*nb) + 2*b + j holds dims
+//           b*32 + 4*g + 2*j (low nibble) and + 1 (high nibble)
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+#include "ember_kv4.h"
+
+namespace emb {
+
+struct Kv4View {
+    uint8_t *data;
+    int n_pages, page_shift, n_kv;
+    uint32_t chunk;               // bytes of one page of one kv head
+};
+
+struct Kv4Rows {                  // EmberKv4Batch on the device side
+    const int32_t *q_start, *kv_len, *table;
+    int n_seqs, table_stride, n_tokens;
+    int cap;                      // table_stride * page_size, within int
+};
+
+__host__ __device__ inline uint32_t kv4_chunk(int page_size, int hd) { return (uint32_t)page_size * (hd + hd / 8); }
+
+// one sequence's rows and length, every number within the bounds the host knows
+struct Kv4Seq {
+    int row0, rows, len;          // first row, number of rows, positions in the cache
+};
+EMB_DEV Kv4Seq kv4_seq(const Kv4Rows &b, int i) {
+    Kv4Seq s;
+    int r0 = i, r1 = i + 1;
+    if (b.q_start) { r0 = b.q_start[i]; r1 = b.q_start[i + 1]; }
+    r0 = max(0, min(r0, b.n_tokens));
+    r1 = max(r0, min(r1, b.n_tokens));
+    s.row0 = r0;
+    s.rows = r1 - r0;
+    s.len = max(0, b.kv_len[i]);
+    return s;
+}
+
+// the page of position pos (0 <= pos < cap), or -1
+EMB_DEV int kv4_page(const Kv4View &c, const Kv4Rows &b, int i, int pos) {
+    const int p = b.table[(size_t)i * b.table_stride + (pos >> c.page_shift)];
+    return (unsigned)p < (unsigned)c.n_pages ? p : -1;
+}
+EMB_DEV uint8_t *kv4_chunk_ptr(const Kv4View &c, int page, int head) {
+    return c.data + ((size_t)page * c.n_kv + head) * c.chunk;
+}
+
+}  // namespace emb

@@ -1,0 +1,178 @@
+"""The many-stream operators of include/ember_kv4.h on device arrays: the paged
+4-bit KV cache (``Kv4Cache``: store, read, attention) and one draw per row of a
+batch of logits (``sample_rows``).
+
+Arrays are CUDA tensors as torch makes them (anything with ``data_ptr``,
+``shape``, ``stride()``, ``dtype`` and ``device`` works; this module does not
+import torch). The caller owns every buffer; a call allocates nothing and enqueues
+its work on ``stream`` (a cudaStream_t as an integer; 0 is the default stream).
+Arguments that do not fit raise ValueError; what the library refuses raises
+RuntimeError with its message.
+"""
+import ctypes
+
+from . import _lib as _libmod
+
+_DTYPES = {"torch.float32": 0, "torch.float16": 3}
+
+
+class _Cache(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("n_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("n_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
+class _Batch(ctypes.Structure):
+    _fields_ = [("q_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p), ("block_table", ctypes.c_void_p),
+                ("n_seqs", ctypes.c_int32), ("table_stride", ctypes.c_int32), ("n_tokens", ctypes.c_int32),
+                ("max_q", ctypes.c_int32)]
+
+
+class _Rows(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("dtype", ctypes.c_int32),
+                ("k_tok", ctypes.c_int64), ("k_head", ctypes.c_int64), ("v_tok", ctypes.c_int64),
+                ("v_head", ctypes.c_int64)]
+
+
+class _Attention(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("dtype", ctypes.c_int32),
+                ("n_heads", ctypes.c_int32), ("q_tok", ctypes.c_int64), ("q_head", ctypes.c_int64),
+                ("out_tok", ctypes.c_int64), ("out_head", ctypes.c_int64), ("scale", ctypes.c_float),
+                ("max_kv", ctypes.c_int32), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class _SampleRows(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("n_rows", ctypes.c_int32),
+                ("vocab", ctypes.c_int32), ("stride", ctypes.c_int64), ("temperature", ctypes.c_void_p),
+                ("top_p", ctypes.c_void_p), ("min_p", ctypes.c_void_p), ("u", ctypes.c_void_p),
+                ("top_k", ctypes.c_void_p), ("out", ctypes.c_void_p)]
+
+
+def _fail():
+    raise RuntimeError(_libmod.load().ember_cuda_error().decode())
+
+
+def _dtype(t, name):
+    d = _DTYPES.get(str(t.dtype))
+    if d is None:
+        raise ValueError(f"{name} must be float32 or float16, not {t.dtype}")
+    return d
+
+
+def _array(t, name, dtype, n):
+    """pointer of a contiguous array of n elements of `dtype`"""
+    if str(t.dtype) != dtype or t.ndim != 1 or t.shape[0] != n or (n > 1 and t.stride()[0] != 1):
+        raise ValueError(f"{name} must be a contiguous {dtype} array of {n}")
+    return t.data_ptr()
+
+
+def _rows(t, name, heads, head_dim):
+    """strides (row, head) of a [rows][heads][head_dim] tensor"""
+    s = t.shape
+    if len(s) != 3 or s[1] != heads or s[2] != head_dim:
+        raise ValueError(f"{name} must be [rows][{heads}][{head_dim}], not {list(s)}")
+    st = t.stride()
+    if st[2] != 1:
+        raise ValueError(f"{name}: a head's elements must be consecutive")
+    return st[0], st[1]
+
+
+class Kv4Cache:
+    """One layer's paged cache in 4 bits over the caller's device buffer."""
+
+    @staticmethod
+    def nbytes(n_pages, page_size, n_kv_heads, head_dim):
+        """bytes of the buffer such a cache needs"""
+        n = _libmod.load().ember_cuda_kv4_bytes(int(n_pages), int(page_size), int(n_kv_heads), int(head_dim))
+        if not n:
+            raise ValueError(f"a cache of {n_pages} pages of {page_size} positions, {n_kv_heads} kv heads of {head_dim} "
+                             "is not supported")
+        return n
+
+    def __init__(self, buffer, n_pages, page_size, n_kv_heads, head_dim):
+        need = Kv4Cache.nbytes(n_pages, page_size, n_kv_heads, head_dim)
+        if not buffer.is_contiguous() or buffer.numel() * buffer.element_size() < need:
+            raise ValueError(f"the cache needs a contiguous buffer of {need} bytes")
+        self.lib = _libmod.load()
+        self.buffer = buffer            # kept alive
+        self.page_size, self.n_kv_heads, self.head_dim = int(page_size), int(n_kv_heads), int(head_dim)
+        self._c = _Cache(buffer.data_ptr(), n_pages, page_size, n_kv_heads, head_dim)
+        self._p = ctypes.byref(self._c)
+
+    def _batch(self, tokens, q_start, kv_len, block_table, max_q):
+        n = kv_len.shape[0]
+        if block_table.ndim != 2 or block_table.shape[0] != n or str(block_table.dtype) != "torch.int32" or \
+                (n and block_table.stride()[1] != 1 and block_table.shape[1] > 1):
+            raise ValueError(f"block_table must be an int32 [{n}][pages] array with consecutive pages")
+        stride = block_table.stride()[0] if n > 1 else block_table.shape[1]
+        if stride != block_table.shape[1]:
+            raise ValueError("block_table must be contiguous")
+        return _Batch(None if q_start is None else _array(q_start, "q_start", "torch.int32", n + 1),
+                      _array(kv_len, "kv_len", "torch.int32", n), block_table.data_ptr(), n, stride, tokens, int(max_q))
+
+    def _io(self, fn, k, v, q_start, kv_len, block_table, max_q, stream):
+        k_tok, k_head = _rows(k, "k", self.n_kv_heads, self.head_dim)
+        v_tok, v_head = _rows(v, "v", self.n_kv_heads, self.head_dim)
+        if k.shape[0] != v.shape[0] or k.dtype != v.dtype:
+            raise ValueError("k and v must have the same rows and type")
+        b = self._batch(k.shape[0], q_start, kv_len, block_table, max_q)
+        r = _Rows(k.data_ptr(), v.data_ptr(), _dtype(k, "k"), k_tok, k_head, v_tok, v_head)
+        if fn(self._p, ctypes.byref(b), ctypes.byref(r), stream):
+            _fail()
+
+    def store(self, k, v, q_start, kv_len, block_table, max_q=1, stream=0):
+        """Quantize the rows' keys and values ([rows][kv heads][head_dim]) into the
+        cache: rows q_start[i]..q_start[i+1]-1 are the last positions of sequence i's
+        kv_len[i]. ``q_start`` None: one row per sequence. ``max_q``: the most rows
+        any sequence has."""
+        self._io(self.lib.ember_cuda_kv4_store, k, v, q_start, kv_len, block_table, max_q, stream)
+
+    def read(self, k, v, q_start, kv_len, block_table, max_q=1, stream=0):
+        """The inverse of ``store``: the cached values of the rows' positions into k
+        and v."""
+        self._io(self.lib.ember_cuda_kv4_read, k, v, q_start, kv_len, block_table, max_q, stream)
+
+    def attention_workspace(self, n_heads, n_seqs, max_q, max_kv):
+        """bytes of workspace an attention call of these sizes needs (may be 0)"""
+        return self.lib.ember_cuda_kv4_attention_workspace(self._p, n_heads, n_seqs, max_q, max_kv)
+
+    def attention(self, q, out, q_start, kv_len, block_table, max_q=1, max_kv=None, scale=None, window=0, sinks=0,
+                  workspace=None, stream=0):
+        """Causal attention of the rows' queries ([rows][heads][head_dim]) over the
+        cache into ``out``; ``window`` > 0 limits it to the last ``window`` positions
+        and the first ``sinks``. ``max_kv`` bounds kv_len (default: all the block table
+        can hold), ``scale`` defaults to head_dim ** -0.5."""
+        heads = q.shape[1]
+        q_tok, q_head = _rows(q, "q", heads, self.head_dim)
+        out_tok, out_head = _rows(out, "out", heads, self.head_dim)
+        if q.shape[0] != out.shape[0] or q.dtype != out.dtype:
+            raise ValueError("q and out must have the same rows and type")
+        b = self._batch(q.shape[0], q_start, kv_len, block_table, max_q)
+        if max_kv is None:
+            max_kv = min(block_table.shape[1] * self.page_size, 2 ** 31 - 1)
+        ws, nws = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None \
+            else (None, 0)
+        a = _Attention(q.data_ptr(), out.data_ptr(), _dtype(q, "q"), heads, q_tok, q_head, out_tok, out_head,
+                       self.head_dim ** -0.5 if scale is None else scale, max_kv, window, sinks, ws, nws)
+        if self.lib.ember_cuda_kv4_attention(self._p, ctypes.byref(b), ctypes.byref(a), stream):
+            _fail()
+
+
+def sample_rows(logits, out, u, temperature=None, top_k=None, top_p=None, min_p=None, stream=0):
+    """Draw one token per row of ``logits`` [rows][vocab] into ``out`` (int32), with
+    each row's own random number ``u`` in [0, 1) and settings (float32 arrays,
+    ``top_k`` int32; None: temperature 1, no truncation). See
+    ember_cuda_sample_rows for the exact definition."""
+    lib = _libmod.load()
+    if logits.ndim != 2 or (logits.shape[1] > 1 and logits.stride()[1] != 1):
+        raise ValueError("logits must be [rows][vocab] with consecutive elements")
+    n = logits.shape[0]
+
+    def opt(t, name, dtype="torch.float32"):
+        return None if t is None else _array(t, name, dtype, n)
+    a = _SampleRows(logits.data_ptr(), _dtype(logits, "logits"), n, logits.shape[1], logits.stride()[0],
+                    opt(temperature, "temperature"), opt(top_p, "top_p"), opt(min_p, "min_p"),
+                    _array(u, "u", "torch.float32", n), opt(top_k, "top_k", "torch.int32"),
+                    _array(out, "out", "torch.int32", n))
+    if lib.ember_cuda_sample_rows(ctypes.byref(a), stream):
+        _fail()

@@ -1,0 +1,156 @@
+/* ember_kv4.h — operators for decoding many streams: a paged KV cache held in 4
+ * bits, attention over it, and one draw per row of a batch of logits.
+ *
+ * No counterpart in emberllm (one sequence per state, fp32 / fp16 cache, sampling
+ * on the host). The operators work on device memory that the caller owns, allocate
+ * nothing, run on the caller's stream and may be captured into a graph. They
+ * return 0, or 1 with a message in ember_cuda_error(); nothing has been enqueued
+ * then. The work runs on the device that owns the buffers; the caller's current
+ * device is unchanged on return. Host arguments are checked on the host. Lengths
+ * and page numbers live on the device: the kernels bound every index they form
+ * from them (see each operator), so wrong ones give wrong results but touch no
+ * memory outside the buffers.
+ *
+ * Only plain C types cross this boundary.
+ */
+#ifndef EMBER_B200_KV4_H
+#define EMBER_B200_KV4_H
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include "ember.h"
+#include "ember_cuda.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* ---- the cache ----
+ * n_pages pages of page_size positions, each with the keys and values of every kv
+ * head of one layer, in blocks of 32 consecutive elements with the values of
+ * Q4_0: (code - 8) * d, codes 0..15, d an fp16 number. d is the block's first
+ * value of largest magnitude divided by -8, rounded to 8 significant bits (as
+ * bf16 does, to nearest even) and then to fp16, at most 8160 in magnitude; the
+ * code of x is floor(x / d + 8.5) in exact arithmetic, clamped to 0..15 (8 where
+ * d is 0). With so short a d every cached value is exactly an fp16 number. A NaN
+ * is stored as 0 and an infinity as the largest value the block can hold: the
+ * cache never holds either.
+ *
+ * The order of the bytes inside a page is the kernels' own: only the functions
+ * below read or write it. Bytes never written may have any content: positions
+ * behind a sequence's length are not looked at. */
+typedef struct {
+    void   *data;         /* device memory of this layer's cache, 16-byte aligned     */
+    int32_t n_pages;      /* n_pages * page_size at most 2^31 - 1                     */
+    int32_t page_size;    /* 16, 32, 64 or 128                                        */
+    int32_t n_kv_heads;
+    int32_t head_dim;     /* 32, 64 or 128                                            */
+} EmberKv4Cache;
+
+/* bytes of `data` for such a cache; 0 when a number is not allowed */
+size_t ember_cuda_kv4_bytes(int32_t n_pages, int32_t page_size, int32_t n_kv_heads, int32_t head_dim);
+
+/* Which rows of a batch belong to which sequence and where its pages are. Sequence
+ * i has kv_len[i] positions in the cache (the rows of this call included), and its
+ * rows q_start[i] .. q_start[i+1]-1 are the last ones: row q_start[i+1]-1 is position
+ * kv_len[i]-1. Position p lies in page block_table[i][p / page_size].
+ * All three arrays are device memory. */
+typedef struct {
+    const int32_t *q_start;      /* [n_seqs + 1]; NULL: one row per sequence, row i          */
+    const int32_t *kv_len;       /* [n_seqs]                                                 */
+    const int32_t *block_table;  /* [n_seqs][table_stride]                                   */
+    int32_t n_seqs;              /* at most 65535                                            */
+    int32_t table_stride;
+    int32_t n_tokens;            /* rows of the batch's tensors                              */
+    int32_t max_q;               /* no sequence has more rows than this (1 when q_start NULL)*/
+} EmberKv4Batch;
+
+/* Quantize the rows' keys and values into the cache. k and v are [n_tokens]
+ * [n_kv_heads][head_dim] of dtype EMBER_DT_F32 or EMBER_DT_F16, a head's elements
+ * consecutive, *_tok and *_head the other strides in elements. Rows whose position
+ * is negative or behind the table, or whose table entry is no page, are not stored.
+ * One call must not store the same position of the same page twice. */
+typedef struct {
+    const void *k, *v;
+    int32_t dtype;
+    int64_t k_tok, k_head, v_tok, v_head;
+} EmberKv4Rows;
+int ember_cuda_kv4_store(const EmberKv4Cache *cache, const EmberKv4Batch *batch, const EmberKv4Rows *rows,
+                         void *stream);
+
+/* The inverse: the cached values of the rows' positions into k and v (which must
+ * be writable). Rows that store would not have stored are left as they are. */
+int ember_cuda_kv4_read(const EmberKv4Cache *cache, const EmberKv4Batch *batch, const EmberKv4Rows *rows,
+                        void *stream);
+
+/* Attention of the rows' queries over the cache: per row at position pos and per
+ * query head, softmax over the visible positions p of scale * (q . k_p), times v_p.
+ * Query head h reads kv head h / (n_heads / n_kv_heads). Visible are p <= pos with
+ * a valid page and, when window > 0, only those with pos - p < window or
+ * p < sinks (the first tokens that stay visible). A row that sees nothing gets
+ * zeros. q and out are [n_tokens][n_heads][head_dim] of dtype F32 or F16; rows
+ * that belong to no sequence are left as they are. A NaN or an infinity in a query
+ * makes that (row, head)'s output NaN and no other.
+ *
+ * Arithmetic: the queries enter the products in 22 significant bits relative to
+ * the row's largest element, the softmax weights in 22 bits (fp16 outputs of
+ * many-row calls: 11 bits); scores, maxima, sums and outputs accumulate in fp32.
+ * The result of a sequence does not depend on its neighbours in the batch, but it
+ * depends in the last bits on the split of the cache, which follows from n_seqs,
+ * max_q and max_kv. The same call gives the same bits.
+ *
+ * max_kv bounds kv_len (positions behind it are not looked at). workspace: device
+ * memory of at least ember_cuda_kv4_attention_workspace() bytes, 16-byte aligned,
+ * contents irrelevant before and after; calls that overlap on the GPU (other
+ * streams, graphs replayed at once) need one each. */
+typedef struct {
+    const void *q;
+    void *out;
+    int32_t dtype;
+    int32_t n_heads;             /* a multiple of n_kv_heads                         */
+    int64_t q_tok, q_head, out_tok, out_head;
+    float scale;                 /* finite                                           */
+    int32_t max_kv;
+    int32_t window, sinks;       /* window 0: every position up to the row's own     */
+    void *workspace;
+    size_t workspace_bytes;
+} EmberKv4Attention;
+size_t ember_cuda_kv4_attention_workspace(const EmberKv4Cache *cache, int32_t n_heads, int32_t n_seqs, int32_t max_q,
+                                          int32_t max_kv);
+int ember_cuda_kv4_attention(const EmberKv4Cache *cache, const EmberKv4Batch *batch, const EmberKv4Attention *att,
+                             void *stream);
+
+/* ---- one draw per row ----
+ * out[r] = a token drawn from row r of logits [n_rows][vocab] (dtype F32 or F16, row
+ * stride in elements, a row's elements consecutive), with that row's settings and
+ * its own random number u[r] in [0, 1). The steps of ember_sample_device without the
+ * penalties, in exact order instead of the reference's rounded one:
+ *   order       logits descending, equal ones by index ascending; a NaN counts as -inf
+ *   weight      w = exp((logit - max) / temperature)
+ *   kept        the first top_k of the order (0 or less: all), of those the ones with
+ *               w >= min_p (outside (0, 1): all), of those the shortest prefix whose
+ *               weights reach top_p of the whole row's (outside (0, 1): all)
+ *   draw        the first kept token whose running weight exceeds u * (kept weight);
+ *               u outside [0, 1) counts as its nearest end, a NaN as 0
+ * A temperature of 0 or less (or NaN) gives the first index of the maximum; so does a
+ * row whose logits are all -inf or NaN (index 0). Weights are exp in double precision,
+ * held as multiples of 2^-44 and added as integers: neither the order of the additions
+ * nor the other rows can change a token. temperature, top_k, top_p, min_p and u are
+ * device arrays of n_rows; NULL means 1, all, all, all (u is required). */
+#define EMBER_SAMPLE_MAX_VOCAB 393216
+typedef struct {
+    const void *logits;
+    int32_t dtype, n_rows, vocab;        /* vocab in [1, EMBER_SAMPLE_MAX_VOCAB] */
+    int64_t stride;
+    const float *temperature, *top_p, *min_p, *u;
+    const int32_t *top_k;
+    int32_t *out;
+} EmberSampleRows;
+int ember_cuda_sample_rows(const EmberSampleRows *args, void *stream);
+
+#ifdef __cplusplus
+}  /* extern "C" */
+#endif
+
+#endif /* EMBER_B200_KV4_H */
