@@ -288,7 +288,7 @@ extern "C" size_t ember_cuda_kv4_attention_workspace(const EmberKv4Cache *cache,
     if (!cache || n_heads < 1 || n_seqs < 1 || max_q < 1 || max_kv < 1 || cache->n_kv_heads < 1 ||
         n_heads % cache->n_kv_heads)
         return 0;
-    return kv4_attention_workspace(n_heads, cache->n_kv_heads, cache->head_dim, n_seqs, max_q, max_kv);
+    return kv4_attention_workspace(cache->head_dim, max_kv);
 }
 
 extern "C" int ember_cuda_kv4_attention(const EmberKv4Cache *cache, const EmberKv4Batch *batch,
@@ -317,7 +317,7 @@ extern "C" int ember_cuda_kv4_attention(const EmberKv4Cache *cache, const EmberK
         return set_err("%s: negative strides are not supported", who);
     const int hd = cache->head_dim;
     int max_kv = att->max_kv < b.cap ? att->max_kv : b.cap;
-    const size_t need = max_kv > 0 ? kv4_attention_workspace(att->n_heads, c.n_kv, hd, b.n_seqs, max_q, max_kv) : 0;
+    const size_t need = kv4_attention_workspace(hd, max_kv);
     if (need) {
         if (att->workspace_bytes < need)
             return set_err("%s: workspace of %zu bytes, %zu needed", who, att->workspace_bytes, need);
