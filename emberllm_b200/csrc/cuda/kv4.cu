@@ -80,16 +80,18 @@ __global__ void __launch_bounds__(KV4_IO_THREADS) kv4_io_kernel(Kv4View c, Kv4Ro
     live = live && pos >= 0 && pos < b.cap;
     const int page = live ? kv4_page(c, b, blockIdx.y, (int)pos) : -1;
     live = page >= 0;
-    const int slot = (int)(pos & ((1 << c.page_shift) - 1)), ps = 1 << c.page_shift;
+    const int slot = (int)(pos & ((1 << c.page_shift) - 1)), in = slot & 15;
     uint8_t *chunk = live ? kv4_chunk_ptr(c, page, head) : nullptr;
     const int blk = lane >> 3, g = lane & 7;
     uint16_t *code = nullptr;
     __half *scale = nullptr;
     if (live) {
-        uint8_t *r = chunk + (size_t)slot * (HD / 2) + (is_v ? (size_t)ps * (HD / 2) : 0);
-        code = reinterpret_cast<uint16_t *>(is_v ? r + g * (2 * NB) + 2 * blk
-                                                 : r + (g >> 1) * (4 * NB) + 4 * blk + 2 * (g & 1));
-        scale = reinterpret_cast<__half *>(chunk + (size_t)ps * HD) + (is_v ? ps * NB : 0) + slot * NB + blk;
+        uint8_t *group = chunk + (slot >> 4) * kv4_group(HD);
+        const int pair = in >> 1, odd = in & 1;
+        code = reinterpret_cast<uint16_t *>(
+            group + (is_v ? 8 * HD + pair * HD + g * (4 * NB) + 4 * blk + 2 * odd
+                          : in * (HD / 2) + (g >> 1) * (4 * NB) + 4 * blk + 2 * (g & 1)));
+        scale = reinterpret_cast<__half *>(group + 16 * HD) + (is_v ? 16 * NB + (pair * NB + blk) * 2 + odd : in * NB + blk);
     }
     const long long tok = s.row0 + row;
     T *mem = nullptr;

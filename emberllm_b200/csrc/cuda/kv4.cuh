@@ -1,17 +1,22 @@
 // kv4.cuh — layout of the paged 4-bit KV cache and the batch's index arithmetic,
 // shared by the kernels that write it (kv4.cu) and read it (kv4.cu, kv4_attn.cuh).
 //
-// One page of one kv head is one contiguous chunk:
+// One page of one kv head is one contiguous chunk of page_size / 16 groups; a group
+// holds 16 positions, whole, so that one contiguous copy brings what a warp works on
+// (hd = head_dim, nb = hd/32 blocks, p = position inside the group):
 //
-//     [page_size][hd/2] key codes | [page_size][hd/2] value codes
-//     | [page_size][hd/32] fp16 key scales | [page_size][hd/32] fp16 value scales
+//     [16][hd/2] key codes | [8][hd] value codes | [16][nb] fp16 key scales
+//     | [8][nb][2] fp16 value scales                       (18 * hd bytes)
 //
-// The order inside a row of codes serves the matrix fragments that the attention
-// builds from it in registers (nb = hd/32 blocks):
-//   keys    word (t, b), t = 0..3, at byte t*(4*nb) + 4*b holds dims b*32 + 8*t + n
-//           in nibble n: lane t of a fragment loads its words of every block at once
-//   values  byte (g, b, j), g = 0..7, j = 0..1, at g*(2*nb) + 2*b + j holds dims
-//           b*32 + 4*g + 2*j (low nibble) and + 1 (high nibble)
+// The order of the codes serves the matrix fragments that the attention builds
+// from them in registers:
+//   keys    row p of hd/2 bytes: word (t, b), t = 0..3, at byte t*(4*nb) + 4*b holds
+//           dims b*32 + 8*t + n in nibble n: lane t of a fragment loads its words of
+//           every block at once
+//   values  pairs of positions share rows of hd bytes: word (g, b), g = 0..7, at
+//           byte g*(4*nb) + 4*b holds dims b*32 + 4*g + n in nibble n of its lower
+//           half for the even position and of its upper half for the odd one, so
+//           that a masked word is a pair of operands; their scales likewise
 #pragma once
 
 #include <cuda_fp16.h>
@@ -35,7 +40,8 @@ struct Kv4Rows {                  // EmberKv4Batch on the device side
     int cap;                      // table_stride * page_size, within int
 };
 
-__host__ __device__ inline uint32_t kv4_chunk(int page_size, int hd) { return (uint32_t)page_size * (hd + hd / 8); }
+__host__ __device__ constexpr uint32_t kv4_group(int hd) { return 18u * hd; }   // bytes of 16 positions
+__host__ __device__ inline uint32_t kv4_chunk(int page_size, int hd) { return page_size / 16 * kv4_group(hd); }
 
 // one sequence's rows and length, every number within the bounds the host knows
 struct Kv4Seq {

@@ -7,22 +7,25 @@
 //
 // Bound by memory (144 bytes a position and kv head of 128) once the codes are
 // turned into matrix operands cheaply enough: at 44 bytes per ns and SM there are
-// about 3 lane instructions per element. So the codes go from global memory to
-// registers in the order of the fragments of mma m16n8k16 and are made operands
-// there: shared memory would be written and read 4x the packed bytes. tcgen05
-// takes its operands from shared memory and at least 64 rows of one side; with a
-// handful of query rows per kv head it has nothing to gain here (prompts use it).
+// about 3 lane instructions per element. So the codes stay packed until they are in
+// registers, in the order of the fragments of mma m16n8k16, and become operands
+// there; in shared memory, as tcgen05 wants them, they would be 4x the bytes, and
+// with a handful of query rows per kv head its 64 rows and more have nothing to do
+// (prompts use it). Asynchronous copies keep a unit ahead in flight per warp without
+// holding registers for it.
 //   scores   A = keys (16 positions x 16 dims): a nibble of a word, masked in
 //            place, IS an fp16 subnormal (code * 2^-24, or code * 2^-20 for the
 //            upper nibbles, whose query elements carry 1/16), so 5 instructions
 //            make 8 operands; B = queries. Sums per 32-block, to which the block's
 //            scale and -8 * (sum of the queries) are applied in fp32.
 //   outputs  A = values (16 dims x 16 positions), made exact fp16 numbers
-//            (code - 8) * d; B = the weights, times 2^14.
+//            (code - 8) * d; B = the weights.
 // Queries and weights take two columns of B each, the fp16 rounding and the
 // rounded rest: 22 bits for the price of idle columns. A query row is first scaled
 // by a power of two so that its largest element is below 2^14.
 #pragma once
+
+#include <atomic>
 
 #include "kv4.cuh"
 #include "runtime_internal.cuh"
@@ -38,13 +41,13 @@ struct Kv4AttnArgs {
     int n_heads, group;
     float scale;
     int max_kv, max_q, window, sinks;
-    int splits, chunks;           // cache splits per sequence; row chunks per kv head
+    int span, parts, chunks;      // units of a CTA; CTAs of the longest sequence; row chunks per kv head
     float *ws;
 };
 
 constexpr int KD_WARPS = 4;
 constexpr int KD_THREADS = 32 * KD_WARPS;
-constexpr int KD_UNIT = 16;        // positions a warp takes at a time (within one page)
+constexpr int KD_UNIT = 32;        // positions a warp takes at a time, in two groups of 16
 constexpr float KV4_LOG2E = 1.44269504088896341f;
 
 EMB_DEV bool kv4_visible(int pos, int p, int window, int sinks) {
@@ -57,61 +60,37 @@ EMB_DEV float kv4_exp2(float x) {
     return y;
 }
 
-// C += A (16x16) * B (16x8), fp16 operands, fp32 sums
-EMB_DEV void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+// D = A (16x16) * B (16x8) + C, fp16 operands, fp32 sums
+EMB_DEV void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                     float c0, float c1, float c2, float c3) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
 EMB_DEV uint32_t h2bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 EMB_DEV __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
 EMB_DEV uint32_t pack_half2(float lo, float hi) { return h2bits(__floats2half2_rn(lo, hi)); }
-// {v & mask, or magic}: one lop3
-EMB_DEV uint32_t and_or(uint32_t v, uint32_t mask, uint32_t magic) { return (v & mask) | magic; }
-
-// W consecutive 32-bit words (or one 16-bit piece, W = 0) without polluting L1
-template <int W>
-EMB_DEV void ldg_words(uint32_t (&r)[W < 1 ? 1 : W], const void *p) {
-    if (W == 0) r[0] = __ldg(reinterpret_cast<const unsigned short *>(p));
-    else if (W == 1) r[0] = __ldg(reinterpret_cast<const uint32_t *>(p));
-    else if (W == 2) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
-        r[0] = v.x; r[W - 1] = v.y;
-    } else {
-        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
-        r[0] = v.x; r[1 % W] = v.y; r[2 % W] = v.z; r[W - 1] = v.w;
-    }
+// (v & mask) | magic as the one instruction it can be: written in C++ it became two,
+// a tenth of the kernel's instructions
+EMB_DEV uint32_t and_or(uint32_t v, uint32_t mask, uint32_t magic) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(magic));
+    return r;
 }
 
-// what a lane loads of one unit of 16 positions: key words of positions g and g+8,
-// value bytes of positions 2t, 2t+1, 2t+8, 2t+9, and those positions' scales
-template <int HD>
-struct KdUnit {
-    static constexpr int NB = HD / 32;
-    static constexpr int VW = NB / 2;                 // words of a lane's value bytes (0: 16 bits)
-    static constexpr int VR = VW < 1 ? 1 : VW;
-    uint32_t k[2][NB], ks[2][VR], v[4][VR], vs[4][VR];
-};
-
-template <int HD>
-EMB_DEV void kd_load(KdUnit<HD> &u, const uint8_t *chunk, int slot0, int ps, int lane) {
-    constexpr int NB = HD / 32;
-    const int g = lane >> 2, t = lane & 3;
-    const uint8_t *k = chunk + (size_t)(slot0 + g) * (HD / 2) + t * (4 * NB);
-    const uint8_t *ks = chunk + (size_t)ps * HD + (slot0 + g) * (2 * NB);
-    ldg_words<NB>(u.k[0], k);
-    ldg_words<NB>(u.k[1], k + 8 * (HD / 2));
-    ldg_words<KdUnit<HD>::VW>(u.ks[0], ks);
-    ldg_words<KdUnit<HD>::VW>(u.ks[1], ks + 8 * (2 * NB));
-    const uint8_t *v = chunk + (size_t)ps * (HD / 2) + (size_t)(slot0 + 2 * t) * (HD / 2) + g * (2 * NB);
-    const uint8_t *vs = chunk + (size_t)ps * HD + ps * (2 * NB) + (slot0 + 2 * t) * (2 * NB);
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int o = (j & 1) + (j >> 1) * 8;
-        ldg_words<KdUnit<HD>::VW>(u.v[j], v + o * (HD / 2));
-        ldg_words<KdUnit<HD>::VW>(u.vs[j], vs + o * (2 * NB));
+// W consecutive 32-bit words of shared memory (W = 0: one 16-bit piece)
+template <int W>
+EMB_DEV void lds_words(uint32_t (&r)[W < 1 ? 1 : W], const uint8_t *p) {
+    if (W == 0) r[0] = *reinterpret_cast<const uint16_t *>(p);
+    else if (W == 1) r[0] = *reinterpret_cast<const uint32_t *>(p);
+    else if (W == 2) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        r[0] = v.x; r[W - 1] = v.y;
+    } else {
+        const uint4 v = *reinterpret_cast<const uint4 *>(p);
+        r[0] = v.x; r[1 % W] = v.y; r[2 % W] = v.z; r[W - 1] = v.w;
     }
 }
 
@@ -119,7 +98,8 @@ EMB_DEV void kd_load(KdUnit<HD> &u, const uint8_t *chunk, int slot0, int ps, int
 // those from the first row's window on
 struct KdRange {
     int sink_units, lo, total;
-    __device__ __forceinline__ int unit(int i) const { return i < sink_units ? i : lo + (i - sink_units); }
+    // first position of unit i
+    __device__ __forceinline__ int pos(int i) const { return (i < sink_units ? i : i + (lo - sink_units)) * KD_UNIT; }
 };
 EMB_DEV KdRange kd_range(int first_pos, int last_pos, int len, int window, int sinks) {
     KdRange r;
@@ -133,12 +113,25 @@ EMB_DEV KdRange kd_range(int first_pos, int last_pos, int len, int window, int s
 
 // NT column tiles of 4 query rows each. Grid: (split, kv head * row chunk, sequence).
 // A row's partial result: max (log2 units), sum, HD outputs, in units of 2^14.
+template <int HD, int NT>
+struct KdLayout {
+    static constexpr int STAGES = 2;
+    static constexpr int UNIT = 2 * kv4_group(HD);                      // bytes of a unit
+    static constexpr int RING = KD_WARPS * STAGES * UNIT;
+    static constexpr int PS = HD + 4;                                   // row stride of partials, in floats
+    static constexpr int PART = KD_WARPS * 4 * NT * PS * 4;             // takes the ring's place at the end
+    static constexpr int SMEM = RING > PART ? RING : PART;
+    static constexpr int CTAS = NT == 1 ? (HD == 128 ? 4 : 5) : (HD == 128 ? 2 : 4);   // per SM, by registers
+};
+
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(KD_THREADS) kv4_decode_kernel(const Kv4AttnArgs a) {
-    constexpr int NB = HD / 32, R = 4 * NT, PS = HD + 4;   // PS: row stride of partials, in floats
+__global__ void __launch_bounds__(KD_THREADS, KdLayout<HD, NT>::CTAS) kv4_decode_kernel(const Kv4AttnArgs a) {
+    using L = KdLayout<HD, NT>;
+    constexpr int NB = HD / 32, R = 4 * NT, PS = L::PS, GB = kv4_group(HD);
+    extern __shared__ __align__(128) uint8_t ring[];                    // [warp][stage][unit]
+    float(*part)[R][PS] = reinterpret_cast<float(*)[R][PS]>(ring);      // [warp][row][PS]
     __shared__ __align__(16) uint4 qf[NT][NB][32];
-    __shared__ float xs8[R][NB], rscale[R];
-    __shared__ __align__(16) float part[KD_WARPS][R][PS];
+    __shared__ float xs8[R][NB], rscale[R];   // -8 * sum of a block's queries and the scores' factor, both in 2^-24
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int kv = blockIdx.y / a.chunks, chunk_row = (blockIdx.y - kv * a.chunks) * R;
     const Kv4Seq s = kv4_seq(a.b, blockIdx.z);
@@ -148,8 +141,11 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_kernel(const Kv4AttnArg
     const int len = min(min(s.len, a.max_kv), a.b.cap);
     const KdRange range = kd_range(pos0 + chunk_row / a.group, pos0 + (chunk_row + min(rows, R) - 1) / a.group, len,
                                    a.window, a.sinks);
-    const int u0 = (int)((long long)range.total * blockIdx.x / a.splits),
-              u1 = (int)((long long)range.total * (blockIdx.x + 1) / a.splits);
+    // CTA x works on units [x * span, x * span + span); a sequence that fits one CTA
+    // is finished by it, the others' partial results are joined by kv4_join_kernel
+    const int parts = max(1, (range.total + a.span - 1) / a.span);
+    if ((int)blockIdx.x >= parts) return;
+    const int u0 = blockIdx.x * a.span, u1 = min(range.total, u0 + a.span);
 
     // ---- queries into B fragments ----
     {
@@ -182,9 +178,9 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_kernel(const Kv4AttnArg
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                 x[r * HD + b * 32 + lane] = y;
-                if (lane == 0) xs8[r][b] = 8.0f * sum;
+                if (lane == 0) xs8[r][b] = sum * (-8.0f / 16777216.0f);
             }
-            if (lane == 0) rscale[r] = a.scale * KV4_LOG2E / f1 / f2;
+            if (lane == 0) rscale[r] = a.scale * (16777216.0f * KV4_LOG2E) / f1 / f2;
         }
         __syncthreads();
         for (int f = warp; f < NT * NB; f += KD_WARPS) {
@@ -214,63 +210,129 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_kernel(const Kv4AttnArg
             for (int j = 0; j < 4; j++) o[nt][i][j] = 0.0f;
     }
     const int ps = 1 << a.c.page_shift;
-    auto page_of = [&](int i) { return i < u1 ? kv4_page(a.c, a.b, blockIdx.z, range.unit(i) * KD_UNIT) : -1; };
+    const float rest = (g & 1) ? -1.0f : 0.0f;             // odd columns hold what fp16 rounded away
+    int row_pos[NT];
+    float row_scale[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        row_pos[nt] = pos0 + (chunk_row + nt * 4 + t) / a.group;
+        row_scale[nt] = rscale[nt * 4 + t];
+    }
+    // positions that every row sees: up to the first row's, from the last row's window on
+    const int all_to = min(len, pos0 + chunk_row / a.group + 1);
+    const long long all_from = a.window > 0 ? (long long)pos0 + (chunk_row + min(rows, R) - 1) / a.group - a.window + 1 : 0;
 
-    KdUnit<HD> nxt;
-    int i = u0 + warp;
-    int page = page_of(i), page_next = page_of(i + KD_WARPS);
-    if (page >= 0) kd_load<HD>(nxt, kv4_chunk_ptr(a.c, page, kv), (range.unit(i) * KD_UNIT) & (ps - 1), ps, lane);
+    // The warp's units are u0 + warp, + KD_WARPS, ...: the next one is copied while
+    // this one is worked on, and the page numbers of the one after are loaded a unit
+    // ahead and looked at when needed. A group whose page is no page is not copied;
+    // its positions are hidden like those behind the length.
+    const int32_t *table = a.b.table + (size_t)blockIdx.z * a.b.table_stride;
+    const uint8_t *base = a.c.data + (size_t)kv * a.c.chunk;
+    const uint32_t stride = (uint32_t)a.c.n_kv * a.c.chunk;
+    const bool small = ps == 16;                   // the groups lie in two pages
+    const int last = max(0, len - 1) >> a.c.page_shift;
+    struct Pages { int p[2]; };
+    auto pages_of = [&](int i, int pos) {
+        Pages r = {{-1, -1}};
+        if (i < u1) {
+            const int p = pos >> a.c.page_shift;
+            r.p[0] = __ldg(table + p);
+            r.p[1] = small ? __ldg(table + min(p + 1, last)) : r.p[0];
+        }
+        return r;
+    };
+    auto valid = [&](int page) { return (unsigned)page < (unsigned)a.c.n_pages; };
+    uint8_t *const mine = ring + warp * (L::STAGES * L::UNIT);
+    const uint32_t mine32 = smem_u32(mine) + lane * 16;
+    auto copy = [&](const Pages &pg, int pos, int stage) {
+        const bool ok0 = valid(pg.p[0]), ok1 = valid(pg.p[1]);
+        const uint8_t *c0 = base + (uint64_t)(uint32_t)pg.p[0] * stride + (pos & (ps - 1)) / 16 * GB + lane * 16;
+        const uint8_t *c1 = small ? base + (uint64_t)(uint32_t)pg.p[1] * stride + lane * 16 - GB : c0;
+        const uint32_t dst = mine32 + stage * L::UNIT;
+#pragma unroll
+        for (int k = 0; k * 512 < L::UNIT; k++) {
+            const int at = k * 512 + lane * 16;            // byte of the unit
+            const bool second = at >= GB;
+            if (at < L::UNIT && (second ? ok1 : ok0))
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + k * 512),
+                             "l"((second ? c1 : c0) + k * 512)
+                             : "memory");
+        }
+    };
+
+    int i = u0 + warp, p0 = range.pos(i), pn = range.pos(i + KD_WARPS), stage = 0;
+    Pages pg = pages_of(i, p0);
+    if (i < u1) copy(pg, p0, 0);
+    cp_async_commit();
+    bool ok0 = valid(pg.p[0]), ok1 = valid(pg.p[1]);
+    pg = pages_of(i + KD_WARPS, pn);
     for (; i < u1; i += KD_WARPS) {
-        const KdUnit<HD> cur = nxt;
-        const bool have = page >= 0;
-        page = page_next;
-        page_next = page_of(i + 2 * KD_WARPS);
-        if (page >= 0)
-            kd_load<HD>(nxt, kv4_chunk_ptr(a.c, page, kv), (range.unit(i + KD_WARPS) * KD_UNIT) & (ps - 1), ps, lane);
-        if (!have) continue;
-        const int p0 = range.unit(i) * KD_UNIT;
+        if (i + KD_WARPS < u1) copy(pg, pn, stage ^ 1);
+        cp_async_commit();
+        const bool n0 = valid(pg.p[0]), n1 = valid(pg.p[1]);
+        const int p2 = range.pos(i + 2 * KD_WARPS);
+        pg = pages_of(i + 2 * KD_WARPS, p2);
+        cp_async_wait_1();
+        __syncwarp();
+        const uint8_t *unit = mine + stage * L::UNIT;
 
-        // scores of positions p0 + g and p0 + g + 8 for row nt*4 + t
-        float sc[NT][2];
+        // scores of positions p0 + 16 h + g (and + 8) for row nt*4 + t
+        float sc[NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) sc[nt][0] = sc[nt][1] = 0.0f;
+        for (int h = 0; h < 2; h++) {
+            const uint8_t *kp = unit + h * GB + g * (HD / 2) + t * (4 * NB), *sp = unit + h * GB + 16 * HD + g * (2 * NB);
+            uint32_t k[2][NB], ks[2][NB < 2 ? 1 : NB / 2];
+            lds_words<NB>(k[0], kp);
+            lds_words<NB>(k[1], kp + 8 * (HD / 2));
+            lds_words<NB / 2>(ks[0], sp);
+            lds_words<NB / 2>(ks[1], sp + 8 * (2 * NB));
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            const uint32_t w0 = cur.k[0][b], w1 = cur.k[1][b];
-            const uint32_t h0 = w0 >> 8, h1 = w1 >> 8;
-            const float d0 = __half2float((b & 1) ? __high2half(bits_h2(cur.ks[0][b / 2])) : __low2half(bits_h2(cur.ks[0][b / 2])));
-            const float d1 = __half2float((b & 1) ? __high2half(bits_h2(cur.ks[1][b / 2])) : __low2half(bits_h2(cur.ks[1][b / 2])));
+            for (int nt = 0; nt < NT; nt++) sc[nt][2 * h] = sc[nt][2 * h + 1] = 0.0f;
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                const uint4 f = qf[nt][b][lane];
-                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                mma_f16(c, w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, f.x, f.y);
-                mma_f16(c, h0 & 0x000F000Fu, h1 & 0x000F000Fu, h0 & 0x00F000F0u, h1 & 0x00F000F0u, f.z, f.w);
-                const float e8 = xs8[nt * 4 + t][b];
-                sc[nt][0] = fmaf(d0, fmaf(c[0] + c[1], 16777216.0f, -e8), sc[nt][0]);
-                sc[nt][1] = fmaf(d1, fmaf(c[2] + c[3], 16777216.0f, -e8), sc[nt][1]);
+            for (int b = 0; b < NB; b++) {
+                const uint32_t w0 = k[0][b], w1 = k[1][b];
+                const uint32_t h0 = w0 >> 8, h1 = w1 >> 8;
+                const float d0 = (b & 1) ? __high2float(bits_h2(ks[0][b / 2])) : __low2float(bits_h2(ks[0][b / 2]));
+                const float d1 = (b & 1) ? __high2float(bits_h2(ks[1][b / 2])) : __low2float(bits_h2(ks[1][b / 2]));
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    const uint4 f = qf[nt][b][lane];
+                    const float e8 = xs8[nt * 4 + t][b];
+                    float c[4];
+                    mma_f16(c, w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, f.x, f.y, e8,
+                            0.0f, e8, 0.0f);
+                    mma_f16(c, h0 & 0x000F000Fu, h1 & 0x000F000Fu, h0 & 0x00F000F0u, h1 & 0x00F000F0u, f.z, f.w, c[0],
+                            c[1], c[2], c[3]);
+                    sc[nt][2 * h] = fmaf(d0, c[0] + c[1], sc[nt][2 * h]);
+                    sc[nt][2 * h + 1] = fmaf(d1, c[2] + c[3], sc[nt][2 * h + 1]);
+                }
             }
         }
+        const bool whole = p0 >= all_from && p0 + KD_UNIT <= all_to && ok0 && ok1;
 
         // softmax: the row's lanes are those of equal t
-        uint32_t pb[NT][2];
+        uint32_t pb[NT][2][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const int r = nt * 4 + t;
-            const int pos = pos0 + (chunk_row + r) / a.group;
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int p = p0 + g + 8 * j;
-                const bool see = p < len && kv4_visible(pos, p, a.window, a.sinks);
-                sc[nt][j] = see ? sc[nt][j] * rscale[r] : -INFINITY;
+            for (int j = 0; j < 4; j++) sc[nt][j] *= row_scale[nt];
+            if (!whole) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int p = p0 + g + 8 * j;
+                    if (!((j < 2 ? ok0 : ok1) && p < len && kv4_visible(row_pos[nt], p, a.window, a.sinks)))
+                        sc[nt][j] = -INFINITY;
+                }
             }
-            float mx = fmaxf(sc[nt][0], sc[nt][1]);
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            if (__any_sync(0xffffffffu, mx > m[nt])) {
+            // the row's maximum is only raised when a score passes it by 2^8: until then
+            // the weights, 2^(score - m + 6), stay below fp16's 2^14
+            float mx = fmaxf(fmaxf(sc[nt][0], sc[nt][1]), fmaxf(sc[nt][2], sc[nt][3]));
+            if (__any_sync(0xffffffffu, mx > m[nt] + 8.0f)) {
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                 const float mn = fmaxf(m[nt], mx);
-                const float f = m[nt] == -INFINITY ? 0.0f : kv4_exp2(m[nt] - mn);
+                const float f = mn == m[nt] ? 1.0f : kv4_exp2(m[nt] - mn);
                 m[nt] = mn;
                 l[nt] *= f;
 #pragma unroll
@@ -278,58 +340,73 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_kernel(const Kv4AttnArg
 #pragma unroll
                     for (int j = 0; j < 4; j++) o[nt][k][j] *= f;
             }
-            const float base = m[nt] == -INFINITY ? 0.0f : m[nt] - 14.0f;
-            const float e0 = kv4_exp2(sc[nt][0] - base), e1 = kv4_exp2(sc[nt][1] - base);
-            l[nt] += e0 + e1;
+            const float base = m[nt] == -INFINITY ? 0.0f : m[nt] - 6.0f;
+            float e[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) e[j] = kv4_exp2(sc[nt][j] - base);
+            l[nt] += (e[0] + e[1]) + (e[2] + e[3]);
             // the weights into B: column g is row g/2 of this tile, positions 2t, 2t+1, 2t+8, 2t+9
             const int src = 8 * t + (g >> 1);
-            float y[4];
-            y[0] = __shfl_sync(0xffffffffu, e0, src);
-            y[1] = __shfl_sync(0xffffffffu, e0, src + 4);
-            y[2] = __shfl_sync(0xffffffffu, e1, src);
-            y[3] = __shfl_sync(0xffffffffu, e1, src + 4);
-            pb[nt][0] = pack_half2(y[0], y[1]);
-            pb[nt][1] = pack_half2(y[2], y[3]);
-            if (g & 1) {
-                const float2 h0 = __half22float2(bits_h2(pb[nt][0])), h1 = __half22float2(bits_h2(pb[nt][1]));
-                pb[nt][0] = pack_half2(y[0] - h0.x, y[1] - h0.y);
-                pb[nt][1] = pack_half2(y[2] - h1.x, y[3] - h1.y);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float y0 = __shfl_sync(0xffffffffu, e[j], src), y1 = __shfl_sync(0xffffffffu, e[j], src + 4);
+                const float2 hi = __half22float2(__floats2half2_rn(y0, y1));
+                pb[nt][j >> 1][j & 1] = pack_half2(fmaf(hi.x, rest, y0), fmaf(hi.y, rest, y1));
             }
         }
 
-        // outputs. Positions behind the length may hold any bytes: their scales count as 0
-        uint32_t vs[4][KdUnit<HD>::VR];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const bool in = p0 + 2 * t + (j & 1) + (j >> 1) * 8 < len;
-#pragma unroll
-            for (int k = 0; k < KdUnit<HD>::VR; k++) vs[j][k] = in ? cur.vs[j][k] : 0u;
-        }
-        const __half2 bias_lo = bits_h2(0x64086408u);                        // 1032
+        // outputs
+        const bool cut = p0 + KD_UNIT > len || !ok0 || !ok1;
+        const __half2 bias_lo = bits_h2(0x64086408u);                                     // 1032
         const __half2 sixteenth = bits_h2(0x2C002C00u), bias_hi = bits_h2(0xD480D480u);   // 1/16, -72
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            const uint32_t sel = (b & 1) ? 0x7632u : 0x5410u;
-            const __half2 d01 = bits_h2(__byte_perm(vs[0][b / 2], vs[1][b / 2], sel));
-            const __half2 d23 = bits_h2(__byte_perm(vs[2][b / 2], vs[3][b / 2], sel));
+        for (int h = 0; h < 2; h++) {
+            const uint8_t *vp = unit + h * GB + 8 * HD + t * HD + g * (4 * NB), *sp = unit + h * GB + 16 * HD + 32 * NB + t * (4 * NB);
+            uint32_t v[2][NB], vs[2][NB];
+            lds_words<NB>(v[0], vp);
+            lds_words<NB>(v[1], vp + 4 * HD);
+            lds_words<NB>(vs[0], sp);
+            lds_words<NB>(vs[1], sp + 4 * (4 * NB));
+            if (cut) {
+                // positions behind the length may hold any bytes: their scales count as 0
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int byte = 2 * (b & 1) + j;
-                const uint32_t bs = byte | (byte << 4) | ((4 + byte) << 8) | ((4 + byte) << 12);
-                const uint32_t x01 = __byte_perm(cur.v[0][b / 2], cur.v[1][b / 2], bs);
-                const uint32_t x23 = __byte_perm(cur.v[2][b / 2], cur.v[3][b / 2], bs);
-                // 1024 + c, and 1024 + 16 c; then (c - 8) * d, every step exact
-                const __half2 a0 = __hmul2(__hsub2(bits_h2(and_or(x01, 0x000F000Fu, 0x64006400u)), bias_lo), d01);
-                const __half2 a1 = __hmul2(__hfma2(bits_h2(and_or(x01, 0x00F000F0u, 0x64006400u)), sixteenth, bias_hi), d01);
-                const __half2 a2 = __hmul2(__hsub2(bits_h2(and_or(x23, 0x000F000Fu, 0x64006400u)), bias_lo), d23);
-                const __half2 a3 = __hmul2(__hfma2(bits_h2(and_or(x23, 0x00F000F0u, 0x64006400u)), sixteenth, bias_hi), d23);
+                for (int j = 0; j < 2; j++) {
+                    const int left = (h ? ok1 : ok0) ? len - (p0 + 16 * h + 2 * t + 8 * j) : 0;
+                    const uint32_t keep = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0x0000FFFFu : 0u;
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-                    mma_f16(o[nt][b * 2 + j], h2bits(a0), h2bits(a1), h2bits(a2), h2bits(a3), pb[nt][0], pb[nt][1]);
+                    for (int b = 0; b < NB; b++) vs[j][b] &= keep;
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const __half2 d01 = bits_h2(vs[0][b]), d23 = bits_h2(vs[1][b]);
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const uint32_t x01 = j ? v[0][b] >> 8 : v[0][b], x23 = j ? v[1][b] >> 8 : v[1][b];
+                    // 1024 + c, and 1024 + 16 c; then (c - 8) * d, every step exact
+                    const __half2 a0 = __hmul2(__hsub2(bits_h2(and_or(x01, 0x000F000Fu, 0x64006400u)), bias_lo), d01);
+                    const __half2 a1 = __hmul2(__hfma2(bits_h2(and_or(x01, 0x00F000F0u, 0x64006400u)), sixteenth, bias_hi), d01);
+                    const __half2 a2 = __hmul2(__hsub2(bits_h2(and_or(x23, 0x000F000Fu, 0x64006400u)), bias_lo), d23);
+                    const __half2 a3 = __hmul2(__hfma2(bits_h2(and_or(x23, 0x00F000F0u, 0x64006400u)), sixteenth, bias_hi), d23);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        float(&c)[4] = o[nt][b * 2 + j];
+                        mma_f16(c, h2bits(a0), h2bits(a1), h2bits(a2), h2bits(a3), pb[nt][h][0], pb[nt][h][1], c[0], c[1],
+                                c[2], c[3]);
+                    }
+                }
             }
         }
+        __syncwarp();                              // the stage is free
+        stage ^= 1;
+        p0 = pn;
+        pn = p2;
+        ok0 = n0;
+        ok1 = n1;
     }
 
+    cp_async_wait_all();
+    __syncthreads();                               // the ring becomes the warps' results
     // ---- join the warps ----
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
@@ -347,7 +424,7 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_kernel(const Kv4AttnArg
     }
     __syncthreads();
     const int live = min(rows, R);
-    float *ws = a.ws + (((size_t)blockIdx.z * gridDim.y + blockIdx.y) * a.splits + blockIdx.x) * (R * PS);
+    float *ws = a.ws + (((size_t)blockIdx.z * gridDim.y + blockIdx.y) * a.parts + blockIdx.x) * (R * PS);
     for (int e = tid; e < live * HD; e += KD_THREADS) {
         const int r = e / HD, d = e - r * HD;
         float mm = -INFINITY;
@@ -361,7 +438,7 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_kernel(const Kv4AttnArg
             lv = fmaf(part[w][r][HD + 1], f, lv);
             ov = fmaf(part[w][r][d], f, ov);
         }
-        if (a.splits == 1) {
+        if (parts == 1) {
             const int rr = chunk_row + r, tok = rr / a.group, h = kv * a.group + rr % a.group;
             T *out = (T *)a.out + (int64_t)(s.row0 + tok) * a.out_tok + h * a.out_head;
             kv_round(lv == 0.0f ? 0.0f : ov / lv, &out[d]);
@@ -370,31 +447,58 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_kernel(const Kv4AttnArg
             if (d == 0) { ws[r * PS + HD] = mm; ws[r * PS + HD + 1] = lv; }
         }
     }
-    if (a.splits > 1) pdl_launch_dependents();
+    if (a.parts > 1) pdl_launch_dependents();
 }
 
-// The splits' partial results of one (kv head, row chunk, sequence) joined.
+// The splits' partial results of one row joined: the factors of all splits first,
+// then KJ_THREADS / HD slices of the splits side by side, added in a fixed order.
+constexpr int KJ_THREADS = 256;
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(KD_THREADS) kv4_join_kernel(const Kv4AttnArgs a) {
-    constexpr int R = 4 * NT, PS = HD + 4;
-    const int kv = blockIdx.x / a.chunks, chunk_row = (blockIdx.x - kv * a.chunks) * R;
+__global__ void __launch_bounds__(KJ_THREADS) kv4_join_kernel(const Kv4AttnArgs a) {
+    constexpr int R = 4 * NT, PS = KdLayout<HD, NT>::PS, SL = KJ_THREADS / HD;
+    extern __shared__ float fac[];                        // [parts]
+    __shared__ float red[KJ_THREADS / 32], part[SL][HD + 1];
+    const int tid = threadIdx.x, r = blockIdx.z;
+    const int kv = blockIdx.x / a.chunks, rr = (blockIdx.x - kv * a.chunks) * R + r;
     const Kv4Seq s = kv4_seq(a.b, blockIdx.y);
-    const int rows = min(min(s.rows, a.max_q) * a.group - chunk_row, R);
+    const int rows = min(s.rows, a.max_q) * a.group, chunk_row = rr - r;
+    // the parts that the row's CTAs made of it
+    const int pos0 = s.len - s.rows;
+    const KdRange range = kd_range(pos0 + chunk_row / a.group, pos0 + (min(rows, chunk_row + R) - 1) / a.group,
+                                   min(min(s.len, a.max_kv), a.b.cap), a.window, a.sinks);
+    const int n = (range.total + a.span - 1) / a.span;
     pdl_wait();
-    const float *ws = a.ws + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * a.splits * (R * PS);
-    for (int e = threadIdx.x; e < rows * HD; e += KD_THREADS) {
-        const int r = e / HD, d = e - r * HD;
-        float mm = -INFINITY;
-        for (int i = 0; i < a.splits; i++) mm = fmaxf(mm, ws[(size_t)i * R * PS + r * PS + HD]);
-        const float base = mm == -INFINITY ? 0.0f : mm;
-        float ov = 0.0f, lv = 0.0f;
-        for (int i = 0; i < a.splits; i++) {
-            const float *p = ws + (size_t)i * R * PS + r * PS;
-            const float f = kv4_exp2(p[HD] - base);
-            lv = fmaf(p[HD + 1], f, lv);
-            ov = fmaf(p[d], f, ov);
-        }
-        const int rr = chunk_row + r, tok = rr / a.group, h = kv * a.group + rr % a.group;
+    if (rr >= rows || n <= 1) return;
+    const float *ws = a.ws + (((size_t)blockIdx.y * gridDim.x + blockIdx.x) * a.parts * R + r) * PS;
+    float mm = -INFINITY;
+    for (int i = tid; i < n; i += KJ_THREADS) {
+        fac[i] = ws[(size_t)i * R * PS + HD];
+        mm = fmaxf(mm, fac[i]);
+    }
+    mm = warp_max(mm);
+    if ((tid & 31) == 0) red[tid >> 5] = mm;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < KJ_THREADS / 32; w++) mm = fmaxf(mm, red[w]);
+    const float base = mm == -INFINITY ? 0.0f : mm;
+    for (int i = tid; i < n; i += KJ_THREADS) fac[i] = kv4_exp2(fac[i] - base);
+    __syncthreads();
+    const int d = tid % HD, sl = tid / HD;
+    float ov = 0.0f, lv = 0.0f;
+#pragma unroll 4
+    for (int i = sl; i < n; i += SL) {
+        const float *p = ws + (size_t)i * R * PS;
+        ov = fmaf(p[d], fac[i], ov);
+        if (d == 0) lv = fmaf(p[HD + 1], fac[i], lv);
+    }
+    part[sl][d] = ov;
+    if (d == 0) part[sl][HD] = lv;
+    __syncthreads();
+    if (tid < HD) {
+        ov = lv = 0.0f;
+#pragma unroll
+        for (int k = 0; k < SL; k++) { ov += part[k][d]; lv += part[k][HD]; }
+        const int tok = rr / a.group, h = kv * a.group + rr % a.group;
         T *out = (T *)a.out + (int64_t)(s.row0 + tok) * a.out_tok + h * a.out_head;
         kv_round(lv == 0.0f ? 0.0f : ov / lv, &out[d]);
     }
@@ -403,14 +507,14 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_join_kernel(const Kv4AttnArgs 
 // ------------------------------------------------------------------- host ----
 
 struct Kv4Plan {
-    int nt, chunks, splits;
+    int nt, chunks, span, parts;
 };
 
-constexpr int KD_WANT = 148 * 6;   // CTAs to aim at when the cache is split
-
-static inline long long kd_most_splits(long long positions) {
-    return (positions + KD_UNIT - 1) / KD_UNIT / (2 * KD_WARPS);   // two units a warp at least
-}
+// CTAs that fit the GPU at once, three per SM; a call is cut into about KD_WAVES
+// times as many pieces of equal length, so that long sequences among short ones do
+// not leave SMs idle, but of KD_SPAN_MIN units at least (a CTA's start and end cost
+// as much as some 100 positions).
+constexpr int KD_SLOTS = 148 * 3, KD_WAVES = 2, KD_SPAN_MIN = 8;
 
 static inline Kv4Plan kv4_plan(const Kv4AttnArgs &a) {
     Kv4Plan p;
@@ -419,28 +523,45 @@ static inline Kv4Plan kv4_plan(const Kv4AttnArgs &a) {
     p.chunks = (int)((rows + 4 * p.nt - 1) / (4 * p.nt));
     const long long base = (long long)a.b.n_seqs * a.c.n_kv * p.chunks;
     long long seen = a.max_kv;
-    if (a.window > 0 && (long long)a.window + a.max_q + a.sinks < seen) seen = (long long)a.window + a.max_q + a.sinks;
-    long long splits = (KD_WANT + base - 1) / base;
-    if (splits > kd_most_splits(seen)) splits = kd_most_splits(seen);
-    p.splits = splits < 1 ? 1 : (int)splits;
+    if (a.window > 0 && (long long)a.window + a.max_q + a.sinks + 2 * KD_UNIT < seen)
+        seen = (long long)a.window + a.max_q + a.sinks + 2 * KD_UNIT;     // the ends may cut a unit each
+    const long long units = (seen + KD_UNIT - 1) / KD_UNIT;
+    long long span = (units * base + KD_SLOTS * KD_WAVES - 1) / (KD_SLOTS * KD_WAVES);
+    if (span < KD_SPAN_MIN) span = KD_SPAN_MIN;
+    if (span > units) span = units < 1 ? 1 : units;
+    p.span = (int)((span + KD_WARPS - 1) / KD_WARPS * KD_WARPS);
+    p.parts = (int)((units + p.span - 1) / p.span);
+    if (p.parts < 1) p.parts = 1;
     return p;
 }
 
-// Bytes of the partial results of any split call with this many positions: the
-// CTAs of a split call number fewer than 2 * KD_WANT, with at most 8 rows each.
+// Bytes of the partial results of any call with this many positions: base * parts
+// CTAs with base * units <= span * slots * waves, so at most slots * waves of them
+// and one more per (sequence, kv head, row chunk); where parts > 1, base itself is
+// below slots * waves. Eight rows each.
 static inline size_t kv4_attention_workspace(int hd, long long max_kv) {
-    return kd_most_splits(max_kv) < 2 ? 0 : (size_t)2 * KD_WANT * 8 * (hd + 4) * 4;
+    return max_kv <= KD_SPAN_MIN * KD_UNIT ? 0 : (size_t)2 * KD_SLOTS * KD_WAVES * 8 * (hd + 4) * 4;
 }
 
 template <typename T, int HD, int NT>
 static int kv4_decode_launch(const Kv4AttnArgs &a, int n_kv, cudaStream_t st) {
-    const dim3 grid((unsigned)a.splits, (unsigned)(n_kv * a.chunks), (unsigned)a.b.n_seqs);
-    kv4_decode_kernel<T, HD, NT><<<grid, KD_THREADS, 0, st>>>(a);
+    const dim3 grid((unsigned)a.parts, (unsigned)(n_kv * a.chunks), (unsigned)a.b.n_seqs);
+    using L = KdLayout<HD, NT>;
+    static std::atomic<unsigned long long> ready{0};      // devices whose limit is raised
+    int dev = 0;
+    CK(cudaGetDevice(&dev));
+    if (dev >= 64 || !((ready.load(std::memory_order_acquire) >> dev) & 1)) {
+        CK(cudaFuncSetAttribute(kv4_decode_kernel<T, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM));
+        if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
+    }
+    kv4_decode_kernel<T, HD, NT><<<grid, KD_THREADS, L::SMEM, st>>>(a);
     CK(cudaGetLastError());
-    if (a.splits > 1) {
+    if (a.parts > 1) {
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)(n_kv * a.chunks), (unsigned)a.b.n_seqs);
-        cfg.blockDim = dim3(KD_THREADS);
+        const long long live = (long long)a.max_q * a.group;
+        cfg.gridDim = dim3((unsigned)(n_kv * a.chunks), (unsigned)a.b.n_seqs, (unsigned)(live < 4 * NT ? live : 4 * NT));
+        cfg.blockDim = dim3(KJ_THREADS);
+        cfg.dynamicSmemBytes = (size_t)a.parts * 4;
         cfg.stream = st;
         cudaLaunchAttribute at[1];
         at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -465,7 +586,8 @@ template <typename T>
 static int kv4_attention_launch(Kv4AttnArgs a, int hd, cudaStream_t st) {
     const Kv4Plan p = kv4_plan(a);
     if ((long long)a.c.n_kv * p.chunks > 65535) return set_err("kv4 attention: max_q %d is too large", a.max_q);
-    a.splits = p.splits;
+    a.span = p.span;
+    a.parts = p.parts;
     a.chunks = p.chunks;
     return p.nt == 1 ? kv4_decode_hd<T, 1>(a, hd, st) : kv4_decode_hd<T, 2>(a, hd, st);
 }
