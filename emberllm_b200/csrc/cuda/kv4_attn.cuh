@@ -41,7 +41,8 @@ struct Kv4AttnArgs {
     int n_heads, group;
     float scale;
     int max_kv, max_q, window, sinks;
-    int span, parts, chunks;      // units of a CTA; CTAs of the longest sequence; row chunks per kv head
+    int chunks;                   // row chunks per kv head
+    int span, parts;              // units of a CTA; CTAs of the longest sequence
     float *ws;
 };
 
@@ -111,122 +112,86 @@ EMB_DEV KdRange kd_range(int first_pos, int last_pos, int len, int window, int s
     return r;
 }
 
-// NT column tiles of 4 query rows each. Grid: (split, kv head * row chunk, sequence).
-// A row's partial result: max (log2 units), sum, HD outputs, in units of 2^14.
+// An item is one (sequence, kv head, chunk of 4 * NT rows); its work is the units its
+// sequence's rows see, cut into pieces of `span` units where there are too few items
+// to fill the GPU. A piece is a CTA's work; kv4_join_kernel joins an item's pieces.
+// (Dealing out all units in even shares, across items, was slower: 64 ragged streams
+// 33 -> 35 us, 512 short and long ones 50 -> 76 us. More items then get cut, and a
+// cut costs the start and end of a CTA, some 8,000 cycles; the scheduler's own
+// filling of free slots does the rest as well.)
 template <int HD, int NT>
 struct KdLayout {
-    static constexpr int STAGES = 2;
+    static constexpr int STAGES = 2, R = 4 * NT;
     static constexpr int UNIT = 2 * kv4_group(HD);                      // bytes of a unit
     static constexpr int RING = KD_WARPS * STAGES * UNIT;
     static constexpr int PS = HD + 4;                                   // row stride of partials, in floats
-    static constexpr int PART = KD_WARPS * 4 * NT * PS * 4;             // takes the ring's place at the end
+    static constexpr int PART = KD_WARPS * R * PS * 4;                  // takes the ring's place at the end
     static constexpr int SMEM = RING > PART ? RING : PART;
     static constexpr int CTAS = NT == 1 ? (HD == 128 ? 4 : 5) : (HD == 128 ? 2 : 4);   // per SM, by registers
 };
+constexpr int KD_SPAN_MIN = 16;       // units of a piece, at least
+constexpr int KD_MAX_SLOTS = 148 * 5; // CTAs that fit the GPU, at most
+
+struct KdItem {
+    Kv4Seq s;
+    int len, pos0, rows;              // visible length, first row's position, rows (all heads of a group)
+    KdRange range;
+};
+EMB_DEV KdItem kd_item(const Kv4AttnArgs &a, int seq) {
+    KdItem it;
+    it.s = kv4_seq(a.b, seq);
+    it.rows = min(it.s.rows, a.max_q) * a.group;
+    it.pos0 = it.s.len - it.s.rows;
+    it.len = min(min(it.s.len, a.max_kv), a.b.cap);
+    it.range = kd_range(it.pos0, it.pos0 + min(it.s.rows, a.max_q) - 1, it.len, a.window, a.sinks);
+    return it;
+}
+
+// a piece's result: per row its max (log2 units), sum and HD outputs
+template <int HD, int NT>
+EMB_DEV float *kd_partial(const Kv4AttnArgs &a, int item, int piece) {
+    return a.ws + ((size_t)item * a.parts + piece) * (KdLayout<HD, NT>::R * KdLayout<HD, NT>::PS);
+}
 
 template <typename T, int HD, int NT>
 __global__ void __launch_bounds__(KD_THREADS, KdLayout<HD, NT>::CTAS) kv4_decode_kernel(const Kv4AttnArgs a) {
     using L = KdLayout<HD, NT>;
-    constexpr int NB = HD / 32, R = 4 * NT, PS = L::PS, GB = kv4_group(HD);
+    constexpr int NB = HD / 32, R = L::R, PS = L::PS, GB = kv4_group(HD);
     extern __shared__ __align__(128) uint8_t ring[];                    // [warp][stage][unit]
     float(*part)[R][PS] = reinterpret_cast<float(*)[R][PS]>(ring);      // [warp][row][PS]
     __shared__ __align__(16) uint4 qf[NT][NB][32];
+    __shared__ __align__(16) float x[R][HD];  // scaled queries
     __shared__ float xs8[R][NB], rscale[R];   // -8 * sum of a block's queries and the scores' factor, both in 2^-24
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int kv = blockIdx.y / a.chunks, chunk_row = (blockIdx.y - kv * a.chunks) * R;
-    const Kv4Seq s = kv4_seq(a.b, blockIdx.z);
-    const int rows = min(s.rows, a.max_q) * a.group - chunk_row;   // rows of this chunk (token-major, head in group)
-    if (rows <= 0) return;
-    const int pos0 = s.len - s.rows;                       // position of the sequence's first row
-    const int len = min(min(s.len, a.max_kv), a.b.cap);
-    const KdRange range = kd_range(pos0 + chunk_row / a.group, pos0 + (chunk_row + min(rows, R) - 1) / a.group, len,
-                                   a.window, a.sinks);
-    // CTA x works on units [x * span, x * span + span); a sequence that fits one CTA
-    // is finished by it, the others' partial results are joined by kv4_join_kernel
-    const int parts = max(1, (range.total + a.span - 1) / a.span);
-    if ((int)blockIdx.x >= parts) return;
+    const int seq = blockIdx.z, kv = blockIdx.y / a.chunks, chunk_row = (blockIdx.y - kv * a.chunks) * R;
+    const KdItem it = kd_item(a, seq);
+    const int rows = it.rows - chunk_row;                   // rows of this chunk (token-major, head in group)
+    const int len = it.len, pos0 = it.pos0;
+    const KdRange range = it.range;
+    const Kv4Seq &s = it.s;
     const int u0 = blockIdx.x * a.span, u1 = min(range.total, u0 + a.span);
+    if (rows <= 0 || (u0 >= range.total && u0 > 0)) return;
+    // a sequence that fits one piece is finished here
+    float *partial = range.total <= a.span
+                         ? nullptr
+                         : kd_partial<HD, NT>(a, blockIdx.z * gridDim.y + blockIdx.y, blockIdx.x);
 
-    // ---- queries into B fragments ----
-    {
-        float *x = &part[0][0][0];                         // [R][HD] scaled queries
+    // the warp's query rows, asked for before anything waits
+    float qv[NT][NB];
 #pragma unroll
-        for (int i = 0; i < NT; i++) {
-            const int r = warp * NT + i, rr = chunk_row + r;
-            float v[NB], m = 0.0f;
-            bool finite = true;
-            const int tok = rr / a.group, h = kv * a.group + rr % a.group;
+    for (int i = 0; i < NT; i++) {
+        const int rr = chunk_row + warp * NT + i, tok = rr / a.group, h = kv * a.group + rr - tok * a.group;
+        const T *src = (const T *)a.q + (int64_t)(s.row0 + tok) * a.q_tok + h * a.q_head + lane;
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                v[b] = 0.0f;
-                if (r < rows)
-                    v[b] = widen(((const T *)a.q)[(int64_t)(s.row0 + tok) * a.q_tok + h * a.q_head + b * 32 + lane]);
-                finite = finite && fabsf(v[b]) < INFINITY;
-                m = fmaxf(m, fabsf(v[b]));
-            }
-            m = warp_max(m);
-            finite = __all_sync(0xffffffffu, finite);
-            // 2^e with m * 2^e in [2^13, 2^14), in two factors that are normal numbers
-            const int e = m > 0.0f ? 13 - ilogbf(m) : 0;
-            const float f1 = __int_as_float((127 + e / 2) << 23), f2 = __int_as_float((127 + e - e / 2) << 23);
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                const float y = finite ? v[b] * f1 * f2 : __int_as_float(0x7fffffff);
-                const __half hi = __float2half_rn(y);
-                const __half lo = __float2half_rn(y - __half2float(hi));
-                float sum = __half2float(hi) + __half2float(lo);
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                x[r * HD + b * 32 + lane] = y;
-                if (lane == 0) xs8[r][b] = sum * (-8.0f / 16777216.0f);
-            }
-            if (lane == 0) rscale[r] = a.scale * (16777216.0f * KV4_LOG2E) / f1 / f2;
-        }
-        __syncthreads();
-        for (int f = warp; f < NT * NB; f += KD_WARPS) {
-            // column g: row nt*4 + g/2, its fp16 rounding (even g) or the rest (odd g)
-            const float *xr = x + (f / NB * 4 + (g >> 1)) * HD + (f % NB) * 32 + 8 * t;
-            float y[8];
-#pragma unroll
-            for (int n = 0; n < 8; n++) {
-                y[n] = xr[n] * ((n & 1) ? 0.0625f : 1.0f);
-                const float hi = __half2float(__float2half_rn(y[n]));
-                y[n] = (g & 1) ? y[n] - hi : hi;
-            }
-            qf[f / NB][f % NB][lane] = make_uint4(pack_half2(y[0], y[4]), pack_half2(y[1], y[5]),
-                                                  pack_half2(y[2], y[6]), pack_half2(y[3], y[7]));
-        }
-        __syncthreads();
+        for (int b = 0; b < NB; b++) qv[i][b] = warp * NT + i < rows ? widen(src[b * 32]) : 0.0f;
     }
-
-    float m[NT], l[NT], o[NT][HD / 16][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        m[nt] = -INFINITY;
-        l[nt] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < HD / 16; i++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) o[nt][i][j] = 0.0f;
-    }
-    const int ps = 1 << a.c.page_shift;
-    const float rest = (g & 1) ? -1.0f : 0.0f;             // odd columns hold what fp16 rounded away
-    int row_pos[NT];
-    float row_scale[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        row_pos[nt] = pos0 + (chunk_row + nt * 4 + t) / a.group;
-        row_scale[nt] = rscale[nt * 4 + t];
-    }
-    // positions that every row sees: up to the first row's, from the last row's window on
-    const int all_to = min(len, pos0 + chunk_row / a.group + 1);
-    const long long all_from = a.window > 0 ? (long long)pos0 + (chunk_row + min(rows, R) - 1) / a.group - a.window + 1 : 0;
 
     // The warp's units are u0 + warp, + KD_WARPS, ...: the next one is copied while
     // this one is worked on, and the page numbers of the one after are loaded a unit
     // ahead and looked at when needed. A group whose page is no page is not copied;
     // its positions are hidden like those behind the length.
-    const int32_t *table = a.b.table + (size_t)blockIdx.z * a.b.table_stride;
+    const int ps = 1 << a.c.page_shift;
+    const int32_t *table = a.b.table + (size_t)seq * a.b.table_stride;
     const uint8_t *base = a.c.data + (size_t)kv * a.c.chunk;
     const uint32_t stride = (uint32_t)a.c.n_kv * a.c.chunk;
     const bool small = ps == 16;                   // the groups lie in two pages
@@ -266,6 +231,76 @@ __global__ void __launch_bounds__(KD_THREADS, KdLayout<HD, NT>::CTAS) kv4_decode
     cp_async_commit();
     bool ok0 = valid(pg.p[0]), ok1 = valid(pg.p[1]);
     pg = pages_of(i + KD_WARPS, pn);
+    // ---- queries into B fragments ----
+    {
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+            const int r = warp * NT + i;
+            float m = 0.0f;
+            bool finite = true;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                finite = finite && fabsf(qv[i][b]) < INFINITY;
+                m = fmaxf(m, fabsf(qv[i][b]));
+            }
+            m = warp_max(m);
+            finite = __all_sync(0xffffffffu, finite);
+            // 2^e with m * 2^e in [2^13, 2^14), in two factors that are normal numbers
+            const int e = m > 0.0f ? 13 - ilogbf(m) : 0;
+            const float f1 = __int_as_float((127 + e / 2) << 23), f2 = __int_as_float((127 + e - e / 2) << 23);
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const float y = finite ? qv[i][b] * f1 * f2 : __int_as_float(0x7fffffff);
+                const __half hi = __float2half_rn(y);
+                const __half lo = __float2half_rn(y - __half2float(hi));
+                float sum = __half2float(hi) + __half2float(lo);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                x[r][b * 32 + lane] = y;
+                if (lane == 0) xs8[r][b] = sum * (-8.0f / 16777216.0f);
+            }
+            if (lane == 0) rscale[r] = a.scale * (16777216.0f * KV4_LOG2E) / f1 / f2;
+        }
+        __syncthreads();
+        for (int f = warp; f < NT * NB; f += KD_WARPS) {
+            // column g: row nt*4 + g/2, its fp16 rounding (even g) or the rest (odd g)
+            const float *xr = x[f / NB * 4 + (g >> 1)] + (f % NB) * 32 + 8 * t;
+            const float4 xa = *reinterpret_cast<const float4 *>(xr), xb = *reinterpret_cast<const float4 *>(xr + 4);
+            float y[8] = {xa.x, xa.y, xa.z, xa.w, xb.x, xb.y, xb.z, xb.w};
+#pragma unroll
+            for (int n = 0; n < 8; n++) {
+                y[n] *= (n & 1) ? 0.0625f : 1.0f;
+                const float hi = __half2float(__float2half_rn(y[n]));
+                y[n] = (g & 1) ? y[n] - hi : hi;
+            }
+            qf[f / NB][f % NB][lane] = make_uint4(pack_half2(y[0], y[4]), pack_half2(y[1], y[5]),
+                                                  pack_half2(y[2], y[6]), pack_half2(y[3], y[7]));
+        }
+        __syncthreads();
+    }
+
+    float m[NT], l[NT], o[NT][HD / 16][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        m[nt] = -INFINITY;
+        l[nt] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < HD / 16; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[nt][i][j] = 0.0f;
+    }
+    const float rest = (g & 1) ? -1.0f : 0.0f;             // odd columns hold what fp16 rounded away
+    int row_pos[NT];
+    float row_scale[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        row_pos[nt] = pos0 + (chunk_row + nt * 4 + t) / a.group;
+        row_scale[nt] = rscale[nt * 4 + t];
+    }
+    // positions that every row sees: up to the first row's, from the last row's window on
+    const int all_to = min(len, pos0 + chunk_row / a.group + 1);
+    const long long all_from = a.window > 0 ? (long long)pos0 + (chunk_row + min(rows, R) - 1) / a.group - a.window + 1 : 0;
+
     for (; i < u1; i += KD_WARPS) {
         if (i + KD_WARPS < u1) copy(pg, pn, stage ^ 1);
         cp_async_commit();
@@ -424,7 +459,6 @@ __global__ void __launch_bounds__(KD_THREADS, KdLayout<HD, NT>::CTAS) kv4_decode
     }
     __syncthreads();
     const int live = min(rows, R);
-    float *ws = a.ws + (((size_t)blockIdx.z * gridDim.y + blockIdx.y) * a.parts + blockIdx.x) * (R * PS);
     for (int e = tid; e < live * HD; e += KD_THREADS) {
         const int r = e / HD, d = e - r * HD;
         float mm = -INFINITY;
@@ -438,115 +472,100 @@ __global__ void __launch_bounds__(KD_THREADS, KdLayout<HD, NT>::CTAS) kv4_decode
             lv = fmaf(part[w][r][HD + 1], f, lv);
             ov = fmaf(part[w][r][d], f, ov);
         }
-        if (parts == 1) {
+        if (!partial) {
             const int rr = chunk_row + r, tok = rr / a.group, h = kv * a.group + rr % a.group;
             T *out = (T *)a.out + (int64_t)(s.row0 + tok) * a.out_tok + h * a.out_head;
             kv_round(lv == 0.0f ? 0.0f : ov / lv, &out[d]);
         } else {
-            ws[r * PS + d] = ov;
-            if (d == 0) { ws[r * PS + HD] = mm; ws[r * PS + HD + 1] = lv; }
+            partial[r * PS + d] = ov;
+            if (d == 0) { partial[r * PS + HD] = mm; partial[r * PS + HD + 1] = lv; }
         }
     }
     if (a.parts > 1) pdl_launch_dependents();
 }
 
-// The splits' partial results of one row joined: the factors of all splits first,
-// then KJ_THREADS / HD slices of the splits side by side, added in a fixed order.
-constexpr int KJ_THREADS = 256;
+// The pieces of one row of an item joined. Every warp finds the pieces' factors, then
+// takes every KJ_WARPS-th piece; the warps' sums are added in order.
+constexpr int KJ_WARPS = 8;
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(KJ_THREADS) kv4_join_kernel(const Kv4AttnArgs a) {
-    constexpr int R = 4 * NT, PS = KdLayout<HD, NT>::PS, SL = KJ_THREADS / HD;
-    extern __shared__ float fac[];                        // [parts]
-    __shared__ float red[KJ_THREADS / 32], part[SL][HD + 1];
-    const int tid = threadIdx.x, r = blockIdx.z;
-    const int kv = blockIdx.x / a.chunks, rr = (blockIdx.x - kv * a.chunks) * R + r;
-    const Kv4Seq s = kv4_seq(a.b, blockIdx.y);
-    const int rows = min(s.rows, a.max_q) * a.group, chunk_row = rr - r;
-    // the parts that the row's CTAs made of it
-    const int pos0 = s.len - s.rows;
-    const KdRange range = kd_range(pos0 + chunk_row / a.group, pos0 + (min(rows, chunk_row + R) - 1) / a.group,
-                                   min(min(s.len, a.max_kv), a.b.cap), a.window, a.sinks);
-    const int n = (range.total + a.span - 1) / a.span;
+__global__ void __launch_bounds__(32 * KJ_WARPS) kv4_join_kernel(const Kv4AttnArgs a) {
+    constexpr int R = 4 * NT, PS = KdLayout<HD, NT>::PS, Q = HD / 4;
+    __shared__ float fac[KJ_WARPS][KD_MAX_SLOTS];
+    __shared__ __align__(16) float4 part[KJ_WARPS][Q];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = blockIdx.y;
+    const int ny = a.c.n_kv * a.chunks, seq = blockIdx.x / ny, y = blockIdx.x - seq * ny;
+    const KdItem it = kd_item(a, seq);
+    const int kv = y / a.chunks, rr = (y - kv * a.chunks) * R + r;
+    const int n = (it.range.total + a.span - 1) / a.span;
     pdl_wait();
-    if (rr >= rows || n <= 1) return;
-    const float *ws = a.ws + (((size_t)blockIdx.y * gridDim.x + blockIdx.x) * a.parts * R + r) * PS;
-    float mm = -INFINITY;
-    for (int i = tid; i < n; i += KJ_THREADS) {
-        fac[i] = ws[(size_t)i * R * PS + HD];
-        mm = fmaxf(mm, fac[i]);
+    if (rr >= it.rows || n <= 1) return;
+    const Kv4Seq &s = it.s;
+    auto piece = [&](int i) { return kd_partial<HD, NT>(a, blockIdx.x, i) + r * PS; };
+    float mm = -INFINITY, l = 0.0f;
+    for (int i = lane; i < n; i += 32) {
+        fac[warp][i] = piece(i)[HD];
+        mm = fmaxf(mm, fac[warp][i]);
     }
     mm = warp_max(mm);
-    if ((tid & 31) == 0) red[tid >> 5] = mm;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < KJ_THREADS / 32; w++) mm = fmaxf(mm, red[w]);
     const float base = mm == -INFINITY ? 0.0f : mm;
-    for (int i = tid; i < n; i += KJ_THREADS) fac[i] = kv4_exp2(fac[i] - base);
-    __syncthreads();
-    const int d = tid % HD, sl = tid / HD;
-    float ov = 0.0f, lv = 0.0f;
-#pragma unroll 4
-    for (int i = sl; i < n; i += SL) {
-        const float *p = ws + (size_t)i * R * PS;
-        ov = fmaf(p[d], fac[i], ov);
-        if (d == 0) lv = fmaf(p[HD + 1], fac[i], lv);
+    for (int i = lane; i < n; i += 32) {
+        fac[warp][i] = kv4_exp2(fac[warp][i] - base);
+        l = fmaf(piece(i)[HD + 1], fac[warp][i], l);
     }
-    part[sl][d] = ov;
-    if (d == 0) part[sl][HD] = lv;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    __syncwarp();
+    if (lane < Q) {
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int i = warp; i < n; i += KJ_WARPS) {
+            const float4 p = reinterpret_cast<const float4 *>(piece(i))[lane];
+            const float f = fac[warp][i];
+            v.x = fmaf(p.x, f, v.x); v.y = fmaf(p.y, f, v.y); v.z = fmaf(p.z, f, v.z); v.w = fmaf(p.w, f, v.w);
+        }
+        part[warp][lane] = v;
+    }
     __syncthreads();
     if (tid < HD) {
-        ov = lv = 0.0f;
+        float v = 0.0f;
 #pragma unroll
-        for (int k = 0; k < SL; k++) { ov += part[k][d]; lv += part[k][HD]; }
-        const int tok = rr / a.group, h = kv * a.group + rr % a.group;
+        for (int w = 0; w < KJ_WARPS; w++) v += reinterpret_cast<const float *>(part[w])[tid];
+        const int tok = rr / a.group, h = kv * a.group + rr - tok * a.group;
         T *out = (T *)a.out + (int64_t)(s.row0 + tok) * a.out_tok + h * a.out_head;
-        kv_round(lv == 0.0f ? 0.0f : ov / lv, &out[d]);
+        kv_round(l == 0.0f ? 0.0f : v / l, &out[tid]);
     }
 }
 
 // ------------------------------------------------------------------- host ----
 
-struct Kv4Plan {
-    int nt, chunks, span, parts;
-};
-
-// CTAs that fit the GPU at once, three per SM; a call is cut into about KD_WAVES
-// times as many pieces of equal length, so that long sequences among short ones do
-// not leave SMs idle, but of KD_SPAN_MIN units at least (a CTA's start and end cost
-// as much as some 100 positions).
-constexpr int KD_SLOTS = 148 * 3, KD_WAVES = 2, KD_SPAN_MIN = 8;
-
-static inline Kv4Plan kv4_plan(const Kv4AttnArgs &a) {
-    Kv4Plan p;
-    const long long rows = (long long)a.max_q * a.group;
-    p.nt = rows <= 4 ? 1 : 2;
-    p.chunks = (int)((rows + 4 * p.nt - 1) / (4 * p.nt));
-    const long long base = (long long)a.b.n_seqs * a.c.n_kv * p.chunks;
-    long long seen = a.max_kv;
-    if (a.window > 0 && (long long)a.window + a.max_q + a.sinks + 2 * KD_UNIT < seen)
-        seen = (long long)a.window + a.max_q + a.sinks + 2 * KD_UNIT;     // the ends may cut a unit each
-    const long long units = (seen + KD_UNIT - 1) / KD_UNIT;
-    long long span = (units * base + KD_SLOTS * KD_WAVES - 1) / (KD_SLOTS * KD_WAVES);
-    if (span < KD_SPAN_MIN) span = KD_SPAN_MIN;
-    if (span > units) span = units < 1 ? 1 : units;
-    p.span = (int)((span + KD_WARPS - 1) / KD_WARPS * KD_WARPS);
-    p.parts = (int)((units + p.span - 1) / p.span);
-    if (p.parts < 1) p.parts = 1;
-    return p;
-}
-
-// Bytes of the partial results of any call with this many positions: base * parts
-// CTAs with base * units <= span * slots * waves, so at most slots * waves of them
-// and one more per (sequence, kv head, row chunk); where parts > 1, base itself is
-// below slots * waves. Eight rows each.
+// Bytes of the pieces of any call with this many positions: items * parts is at most
+// the number of slots wherever parts > 1. Eight rows each.
 static inline size_t kv4_attention_workspace(int hd, long long max_kv) {
-    return max_kv <= KD_SPAN_MIN * KD_UNIT ? 0 : (size_t)2 * KD_SLOTS * KD_WAVES * 8 * (hd + 4) * 4;
+    return max_kv <= KD_SPAN_MIN * KD_UNIT ? 0 : (size_t)KD_MAX_SLOTS * 8 * (hd + 4) * sizeof(float);
 }
 
 template <typename T, int HD, int NT>
-static int kv4_decode_launch(const Kv4AttnArgs &a, int n_kv, cudaStream_t st) {
-    const dim3 grid((unsigned)a.parts, (unsigned)(n_kv * a.chunks), (unsigned)a.b.n_seqs);
+static int kv4_decode_launch(Kv4AttnArgs a, cudaStream_t st) {
     using L = KdLayout<HD, NT>;
+    const long long rows = (long long)a.max_q * a.group;
+    const long long chunks = (rows + L::R - 1) / L::R, items = (long long)a.b.n_seqs * a.c.n_kv * chunks;
+    if (a.c.n_kv * chunks > 65535 || items > 0x7FFFFFFF)
+        return set_err("kv4 attention: max_q %d is too large", a.max_q);
+    a.chunks = (int)chunks;
+    // the units that an item has at most (a window's two ends may cut a unit each)
+    long long seen = a.max_kv;
+    if (a.window > 0 && (long long)a.window + a.max_q + a.sinks + 2 * KD_UNIT < seen)
+        seen = (long long)a.window + a.max_q + a.sinks + 2 * KD_UNIT;
+    const long long units = (seen + KD_UNIT - 1) / KD_UNIT;
+    // as many pieces as fill the slots once: two sequences of 40k positions take 33 us
+    // so, 37 us in two rounds, 43 us in three
+    long long parts = 148 * L::CTAS / items;
+    if (parts > units / KD_SPAN_MIN) parts = units / KD_SPAN_MIN;
+    if (parts < 1) parts = 1;
+    a.span = (int)((units + parts - 1) / parts);
+    if (a.span < 1) a.span = 1;
+    a.parts = (int)((units + a.span - 1) / a.span);
+    if (a.parts < 1) a.parts = 1;
     static std::atomic<unsigned long long> ready{0};      // devices whose limit is raised
     int dev = 0;
     CK(cudaGetDevice(&dev));
@@ -554,14 +573,13 @@ static int kv4_decode_launch(const Kv4AttnArgs &a, int n_kv, cudaStream_t st) {
         CK(cudaFuncSetAttribute(kv4_decode_kernel<T, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM));
         if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
     }
+    const dim3 grid((unsigned)a.parts, (unsigned)(a.c.n_kv * chunks), (unsigned)a.b.n_seqs);
     kv4_decode_kernel<T, HD, NT><<<grid, KD_THREADS, L::SMEM, st>>>(a);
     CK(cudaGetLastError());
     if (a.parts > 1) {
         cudaLaunchConfig_t cfg = {};
-        const long long live = (long long)a.max_q * a.group;
-        cfg.gridDim = dim3((unsigned)(n_kv * a.chunks), (unsigned)a.b.n_seqs, (unsigned)(live < 4 * NT ? live : 4 * NT));
-        cfg.blockDim = dim3(KJ_THREADS);
-        cfg.dynamicSmemBytes = (size_t)a.parts * 4;
+        cfg.gridDim = dim3((unsigned)items, (unsigned)(rows < L::R ? rows : L::R));
+        cfg.blockDim = dim3(32 * KJ_WARPS);
         cfg.stream = st;
         cudaLaunchAttribute at[1];
         at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -576,20 +594,15 @@ static int kv4_decode_launch(const Kv4AttnArgs &a, int n_kv, cudaStream_t st) {
 template <typename T, int NT>
 static int kv4_decode_hd(const Kv4AttnArgs &a, int hd, cudaStream_t st) {
     switch (hd) {
-    case 32: return kv4_decode_launch<T, 32, NT>(a, a.c.n_kv, st);
-    case 64: return kv4_decode_launch<T, 64, NT>(a, a.c.n_kv, st);
-    default: return kv4_decode_launch<T, 128, NT>(a, a.c.n_kv, st);
+    case 32: return kv4_decode_launch<T, 32, NT>(a, st);
+    case 64: return kv4_decode_launch<T, 64, NT>(a, st);
+    default: return kv4_decode_launch<T, 128, NT>(a, st);
     }
 }
 
 template <typename T>
-static int kv4_attention_launch(Kv4AttnArgs a, int hd, cudaStream_t st) {
-    const Kv4Plan p = kv4_plan(a);
-    if ((long long)a.c.n_kv * p.chunks > 65535) return set_err("kv4 attention: max_q %d is too large", a.max_q);
-    a.span = p.span;
-    a.parts = p.parts;
-    a.chunks = p.chunks;
-    return p.nt == 1 ? kv4_decode_hd<T, 1>(a, hd, st) : kv4_decode_hd<T, 2>(a, hd, st);
+static int kv4_attention_launch(const Kv4AttnArgs &a, int hd, cudaStream_t st) {
+    return (long long)a.max_q * a.group <= 4 ? kv4_decode_hd<T, 1>(a, hd, st) : kv4_decode_hd<T, 2>(a, hd, st);
 }
 
 }  // namespace emb

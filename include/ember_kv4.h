@@ -96,9 +96,9 @@ int ember_cuda_kv4_read(const EmberKv4Cache *cache, const EmberKv4Batch *batch, 
  * Arithmetic: the queries enter the products in 22 significant bits relative to
  * the row's largest element, the softmax weights in 22 bits (fp16 outputs of
  * many-row calls: 11 bits); scores, maxima, sums and outputs accumulate in fp32.
- * The result of a sequence does not depend on its neighbours in the batch, but it
- * depends in the last bits on the split of the cache, which follows from n_seqs,
- * max_q and max_kv. The same call gives the same bits.
+ * The same call gives the same bits. A row's result does not depend on its
+ * neighbours in the batch; in the last bits it depends on how the cache is cut into
+ * pieces, which follows from n_seqs, max_q, max_kv, window and sinks.
  *
  * max_kv bounds kv_len (positions behind it are not looked at). workspace: device
  * memory of at least ember_cuda_kv4_attention_workspace() bytes, 16-byte aligned,
