@@ -6,131 +6,522 @@
 // the kept weight is the smallest of the prefixes' weights, and the draw is again
 // a prefix: the first token whose running weight reaches floor(u * kept) + 1. All
 // of them ask one question -- where does a running sum (of weights or of ones)
-// reach a target -- answered by a radix descent over the 64-bit keys
-// (descending logit bits, index), eight bits a pass. The sums are integers:
-// no order of additions can change a token.
+// reach a target. It is answered without sorting: the distances max - logit are
+// binned, the bins' sums added up, and the bin in which the target lies is binned
+// again (by the bits of the distance, then by index) until its tokens fit a list;
+// there each token adds up the weights before it. The sums are integers: no order of
+// additions can change a token.
+//
+// A cluster of CTAs holds the row in shared memory, so the logits are read once;
+// they exchange maxima, bins and lists through distributed shared memory. Bound by
+// the exponentials (11 double-precision operations a token: the draw compares sums
+// of up to 393,216 weights, and a token next to a border must not change) and the
+// shared-memory atomics, not by memory.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
+
+#include <atomic>
 
 #include "common.cuh"
 #include "ember_kv4.h"
 #include "runtime_internal.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace emb {
 
-constexpr int SR_THREADS = 1024;
+constexpr int SR_THREADS = 512, SR_WARPS = SR_THREADS / 32;
+constexpr int SR_BINS = 1024;
+constexpr int SR_LIST = 768;              // tokens of a bin that are compared one by one
+constexpr int SR_MAX_CLUSTER = 8;
+static_assert(SR_BINS == 2 * SR_THREADS, "two bins a thread");
+
+typedef unsigned long long u64;
+
+// One CTA's shared memory; the row's slice of S logits follows.
+struct SrShared {
+    union {
+        struct {
+            u64 w[SR_BINS];               // this CTA's bins: weights ...
+            uint32_t c[SR_BINS];          // ... and tokens
+        } bin;
+        struct {
+            u64 key[SR_LIST], w[SR_LIST]; // the first CTA: tokens of the bin that is looked through
+        } list;
+    };
+    u64 run_w[SR_BINS];                   // running sums over the row's bins
+    uint32_t run_c[SR_BINS];
+    double pow2[64];                      // 2^(j/64)
+    u64 part_w[SR_WARPS], sum_w[2];       // block sums; the CTA's total and kept weight
+    uint32_t part_c[SR_WARPS];
+    float part_hi[SR_WARPS], part_lo[SR_WARPS], hi, lo;
+    int part_i[SR_WARPS], hi_i;
+    int list_n;
+    // result of a search: position in the order
+    u64 res_key, res_w;
+    int bin_at, hi_k, lo_k;
+};
 
 EMB_DEV float sr_logit(float v) { return v != v ? -INFINITY : v; }
-// ascending keys are descending logits (-0 and +0 alike)
-EMB_DEV uint32_t sr_key(float v) {
-    const uint32_t u = __float_as_uint(v + 0.0f);
-    return (u >> 31) ? u : ~(u | 0x80000000u);
+
+// exp(x) for x <= 0 in multiples of 2^-44, rounded to nearest: 2^(k/64) from the
+// table, times exp(f * ln2/64), |f| <= 1/2, by its Taylor polynomial of degree 4
+// (the next term is below 4e-14, a multiple's half being 2.8e-14)
+EMB_DEV double sr_exp(double x, const double *pow2) {
+    constexpr double C = 0.69314718055994530942 / 64.0;
+    const double y = x * (64.0 / 0.69314718055994530942);
+    const double t = y + 6755399441055744.0;                 // 1.5 * 2^52: the nearest integer
+    const int k = (int)__double_as_longlong(t);
+    const double f = y - (t - 6755399441055744.0);
+    double q = C * C * C * C / 24.0;
+    q = __fma_rn(q, f, C * C * C / 6.0);
+    q = __fma_rn(q, f, C * C / 2.0);
+    q = __fma_rn(q, f, C);
+    q = __fma_rn(q, f, 1.0);
+    q *= pow2[k & 63];
+    return __longlong_as_double(__double_as_longlong(q) + ((long long)(k >> 6) << 52));
 }
-EMB_DEV double sr_weight(float l, float mx, double t) {
-    if (l == mx) return 1.0;
-    if (l == -INFINITY) return 0.0;
-    return exp(((double)l - (double)mx) / t);
+
+struct SrRow {
+    float mx;
+    double inv_t;
+    float limit;                          // distances above it weigh nothing: w < 2^-45
+};
+EMB_DEV double sr_weight(const SrRow &r, float dist, const double *pow2) {
+    return dist == 0.0f ? 1.0 : dist > r.limit ? 0.0 : sr_exp(-(double)dist * r.inv_t, pow2);
 }
-EMB_DEV unsigned long long sr_units(double w) { return (unsigned long long)__double2ll_rn(w * 17592186044416.0); }
+// w is in [0, 1]: adding 2^52 to w * 2^44 leaves the integer in the mantissa
+EMB_DEV u64 sr_units(double w) {
+    return (u64)__double_as_longlong(__fma_rn(w, 17592186044416.0, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
+}
+
+// 64-bit addition in shared memory by 32-bit atomics: whoever makes the lower word
+// wrap carries into the upper one
+EMB_DEV void sr_add(u64 *at, u64 v) {
+    uint32_t *p = reinterpret_cast<uint32_t *>(at);
+    const uint32_t lo = (uint32_t)v, old = atomicAdd(p, lo);
+    const uint32_t hi = (uint32_t)(v >> 32) + (old + lo < old ? 1u : 0u);
+    if (hi) atomicAdd(p + 1, hi);
+}
+
+// where a running sum reaches its target
+struct SrFound {
+    u64 key;                              // (distance bits, index): ascending in the order
+    u64 w;                                // running weight there, inclusive
+};
 
 template <typename T>
-__global__ void __launch_bounds__(SR_THREADS) sample_rows_kernel(EmberSampleRows a) {
-    __shared__ unsigned long long hist[256], s_sum[32], s_out[4];
-    __shared__ float s_v[32];
-    __shared__ int s_i[32];
-    const int tid = threadIdx.x, row = blockIdx.x, n = a.vocab;
-    const T *x = (const T *)a.logits + (int64_t)row * a.stride;
+__global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleRows a, int slice, bool vec) {
+    extern __shared__ __align__(16) uint8_t sr_raw[];
+    SrShared &sh = *reinterpret_cast<SrShared *>(sr_raw);
+    float *val = reinterpret_cast<float *>(sr_raw + (sizeof(SrShared) + 15) / 16 * 16);   // distances max - logit
+    cg::cluster_group cl = cg::this_cluster();
+    const int nc = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.x / nc;
+    const int i0 = min(a.vocab, rank * slice), n = min(a.vocab, i0 + slice) - i0;
+    const T *x = (const T *)a.logits + (int64_t)row * a.stride + i0;
     const float temp = a.temperature ? a.temperature[row] : 1.0f;
-    float mx = -INFINITY;
-    int mi = 0x7FFFFFFF;
-    for (int i = tid; i < n; i += SR_THREADS) {
-        const float v = sr_logit(widen(x[i]));
-        if (v > mx) { mx = v; mi = i; }
-    }
+    const float top_p = a.top_p ? a.top_p[row] : 1.0f, min_p = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
+    const int top_k = a.top_k ? a.top_k[row] : 0;
+    if (tid < 64) sh.pow2[tid] = exp2((double)tid / 64.0);
+
+    // ---- the slice into shared memory; the row's maximum (first index) and minimum ----
+    float hi = -INFINITY, lo = INFINITY;
+    int hi_i = 0x7FFFFFFF;
     auto take = [&](float v, int i) {
-        if (v > mx || (v == mx && i < mi)) { mx = v; mi = i; }
+        if (v > hi || (v == hi && i < hi_i)) { hi = v; hi_i = i; }
     };
-    for (int o = 16; o; o >>= 1) take(__shfl_xor_sync(~0u, mx, o), __shfl_xor_sync(~0u, mi, o));
-    if (tid % 32 == 0) { s_v[tid / 32] = mx; s_i[tid / 32] = mi; }
+    constexpr int W = 16 / sizeof(T);
+    auto see = [&](float v, int i) {
+        v = sr_logit(v);
+        val[i] = v;
+        if (v > hi) { hi = v; hi_i = i0 + i; }
+        if (v > -INFINITY) lo = fminf(lo, v);
+    };
+    const int nv = vec ? n / W : 0;
+#pragma unroll 4
+    for (int j = tid; j < nv; j += SR_THREADS) {
+        const uint4 q = __ldg(reinterpret_cast<const uint4 *>(x) + j);
+        const T *e = reinterpret_cast<const T *>(&q);
+#pragma unroll
+        for (int k = 0; k < W; k++) see(widen(e[k]), j * W + k);
+    }
+    for (int i = nv * W + tid; i < n; i += SR_THREADS) see(widen(x[i]), i);
+    auto warp_take = [&]() {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            take(__shfl_xor_sync(~0u, hi, o), __shfl_xor_sync(~0u, hi_i, o));
+            lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
+        }
+    };
+    warp_take();
+    if (lane == 0) { sh.part_hi[warp] = hi; sh.part_lo[warp] = lo; sh.part_i[warp] = hi_i; }
     __syncthreads();
-    mx = s_v[tid % 32];
-    mi = s_i[tid % 32];
-    for (int o = 16; o; o >>= 1) take(__shfl_xor_sync(~0u, mx, o), __shfl_xor_sync(~0u, mi, o));
-    if (!(temp > 0.0f) || mx == -INFINITY) {
-        if (tid == 0) a.out[row] = mx == -INFINITY ? 0 : mi;
+    hi = lane < SR_WARPS ? sh.part_hi[lane] : -INFINITY;
+    lo = lane < SR_WARPS ? sh.part_lo[lane] : INFINITY;
+    hi_i = lane < SR_WARPS ? sh.part_i[lane] : 0x7FFFFFFF;
+    warp_take();
+    if (nc > 1) {
+        if (tid == 0) { sh.hi = hi; sh.lo = lo; sh.hi_i = hi_i; }
+        cl.sync();
+        hi = -INFINITY; lo = INFINITY; hi_i = 0x7FFFFFFF;
+        for (int r = 0; r < nc; r++) {
+            const SrShared *o = cl.map_shared_rank(&sh, r);
+            take(o->hi, o->hi_i);
+            lo = fminf(lo, o->lo);
+        }
+    }
+    const bool greedy = !(temp > 0.0f) || hi == -INFINITY;
+    if (greedy) {
+        if (rank == 0 && tid == 0) a.out[row] = hi == -INFINITY ? 0 : hi_i;
+        if (nc > 1) cl.sync();            // no CTA leaves while its maximum may be read
         return;
     }
-    const double t = (double)temp;
-    const int k = a.top_k ? a.top_k[row] : 0;
-    const float top_p = a.top_p ? a.top_p[row] : 1.0f, min_p = a.min_p ? a.min_p[row] : 0.0f;
-    // whole weight and the weight of what min_p keeps
-    auto block_sum = [&](unsigned long long v) {
-        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-        __syncthreads();
-        if (tid % 32 == 0) s_sum[tid / 32] = v;
-        __syncthreads();
-        v = s_sum[tid % 32];
-        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-        return v;
+
+    // ---- distances; what the row needs ----
+    SrRow R;
+    R.mx = hi;
+    R.inv_t = 1.0 / (double)temp;
+    R.limit = (float)fmin(31.25 * (double)temp, 3.4e38);   // exp(-31.25) < 2^-45
+    const bool use_k = top_k > 0 && top_k < a.vocab, use_p = top_p > 0.0f && top_p < 1.0f,
+               use_min = min_p > 0.0f && min_p < 1.0f;
+    const bool need_total = use_p || !(use_k || use_min);
+    // (an infinite maximum: the other infinite logits are as far as it, 0)
+    auto dist_of = [&](float v) { return v == R.mx ? 0.0f : R.mx - v; };
+    for (int i = tid; i < n; i += SR_THREADS) val[i] = dist_of(val[i]);
+    __syncthreads();
+    const float far = lo == INFINITY ? 0.0f : dist_of(lo);           // of the finite logits (inf if they overflow)
+    const float far_w = fminf(far, R.limit);
+
+    // ---- bins ----
+    // Bin of a distance: monotone, so a bin's tokens are neighbours in the order; the
+    // last bin holds what is farther than `to`.
+    auto binning = [&](float to) {
+        float scale = fminf((float)(SR_BINS - 2) / fmaxf(to, 1e-30f), 3.0e38f);
+        return scale;
     };
-    const bool use_min = min_p > 0.0f && min_p < 1.0f;
-    unsigned long long total = 0, kept = 0;
-    for (int i = tid; i < n; i += SR_THREADS) {
-        const double w = sr_weight(sr_logit(widen(x[i])), mx, t);
-        total += sr_units(w);
-        if (!use_min || w >= (double)min_p) kept += sr_units(w);
-    }
-    total = block_sum(total);
-    kept = block_sum(kept);
-    // the first token (in order) at which the running sum reaches target: its
-    // index, and the running weight there
-    auto find = [&](unsigned long long target, bool count, unsigned long long *weight) {
-        unsigned long long prefix = 0, acc = 0, wacc = 0;
-        for (int shift = 56; shift >= 0; shift -= 8) {
-            __syncthreads();
-            if (tid < 256) hist[tid] = 0;
-            __syncthreads();
-            unsigned long long below = 0;     // weight before the prefix's range
-            for (int i = tid; i < n; i += SR_THREADS) {
-                const float l = sr_logit(widen(x[i]));
-                const unsigned long long key = ((unsigned long long)sr_key(l) << 32) | (unsigned)i;
-                if (shift == 56 || (key >> (shift + 8)) == prefix)
-                    atomicAdd(&hist[(key >> shift) & 255], count ? 1ull : sr_units(sr_weight(l, mx, t)));
+    auto bin_of = [&](float scale, float d) { return (int)fminf(d * scale, (float)(SR_BINS - 1)); };
+    // the row's running sums over the bins, the same in every CTA
+    auto merge = [&]() {
+        if (nc > 1) cl.sync();
+        else __syncthreads();
+        // this CTA adds up its share of the bins and tells all
+        const int share = SR_BINS / nc;
+        for (int j = tid; j < share; j += SR_THREADS) {
+            const int b = rank * share + j;
+            u64 w = 0;
+            uint32_t c = 0;
+            for (int r = 0; r < nc; r++) {
+                const SrShared *o = cl.map_shared_rank(&sh, r);
+                w += o->bin.w[b];
+                c += o->bin.c[b];
             }
-            __syncthreads();
-            if (tid == 0) {
-                int b = 0;
-                for (; b < 255 && acc + hist[b] < target; b++) acc += hist[b];
-                s_out[0] = (prefix << 8) | b;
-                s_out[1] = acc;
+            for (int r = 0; r < nc; r++) {
+                SrShared *o = cl.map_shared_rank(&sh, r);
+                o->run_w[b] = w;
+                o->run_c[b] = c;
             }
-            __syncthreads();
-            prefix = s_out[0];
-            acc = s_out[1];
-            (void)below;
         }
+        if (nc > 1) cl.sync();
+        else __syncthreads();
+        u64 w0 = sh.run_w[2 * tid], w1 = sh.run_w[2 * tid + 1], w = w0 + w1;
+        uint32_t c0 = sh.run_c[2 * tid], c1 = sh.run_c[2 * tid + 1], c = c0 + c1;
+        const u64 mw = w;
+        const uint32_t mc = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 vw = __shfl_up_sync(~0u, w, o);
+            const uint32_t vc = __shfl_up_sync(~0u, c, o);
+            if (lane >= o) { w += vw; c += vc; }
+        }
+        if (lane == 31) { sh.part_w[warp] = w; sh.part_c[warp] = c; }
+        __syncthreads();
+        for (int k = 0; k < warp; k++) { w += sh.part_w[k]; c += sh.part_c[k]; }
+        sh.run_w[2 * tid] = w - mw + w0;
+        sh.run_c[2 * tid] = c - mc + c0;
+        sh.run_w[2 * tid + 1] = w;
+        sh.run_c[2 * tid + 1] = c;
+        __syncthreads();
+    };
+    auto clear = [&]() {
+        if (nc > 1) cl.sync();            // nobody reads the bins or the list any more
+        else __syncthreads();
+        for (int b = tid; b < SR_BINS; b += SR_THREADS) { sh.bin.w[b] = 0; sh.bin.c[b] = 0; }
+        __syncthreads();
+    };
+    auto add = [&](int b, u64 w, bool on) {
+        if (!on) return;
+        atomicAdd(&sh.bin.c[b], 1u);
+        if (w) sr_add(&sh.bin.w[b], w);
+    };
+
+    // the whole row, its weights where the row needs them
+    float top = binning(use_k ? far : far_w);
+    bool top_valid = false;
+    float weigh_to = INFINITY;            // distances up to which weights are needed
+    u64 kept_min = ~0ull;
+    auto bin_row = [&](bool weights) {
+        clear();
+        u64 k = 0;
         for (int i = tid; i < n; i += SR_THREADS) {
-            const float l = sr_logit(widen(x[i]));
-            const unsigned long long key = ((unsigned long long)sr_key(l) << 32) | (unsigned)i;
-            if (key <= prefix) wacc += sr_units(sr_weight(l, mx, t));
+            const float d = val[i];
+            u64 w = 0;
+            if (weights && d <= weigh_to) {
+                const double e = sr_weight(R, d, sh.pow2);
+                w = sr_units(e);
+                if (e >= (double)min_p) k += w;
+            }
+            add(bin_of(top, d), w, true);
         }
-        *weight = block_sum(wacc);
-        return (int)(prefix & 0xFFFFFFFFu);
+        merge();
+        top_valid = true;
+        return k;
     };
-    unsigned long long w;
-    if (k > 0 && k < n) {
-        find((unsigned long long)k, true, &w);
-        kept = min(kept, w);
+    auto sync = [&]() {
+        if (nc > 1) cl.sync();
+        else __syncthreads();
+    };
+    // the bin in which the running sum, `before` at the first one's start, reaches the
+    // target (the last bin, should it reach it nowhere)
+    auto bin_at = [&](u64 target, bool count, u64 before_w, u64 before_c) {
+        if (tid == 0) sh.bin_at = SR_BINS - 1;
+        __syncthreads();
+        for (int j = tid; j < SR_BINS; j += SR_THREADS) {
+            const u64 s = count ? before_c + sh.run_c[j] : before_w + sh.run_w[j];
+            const u64 s0 = j == 0 ? (count ? before_c : before_w)
+                                  : (count ? before_c + sh.run_c[j - 1] : before_w + sh.run_w[j - 1]);
+            if (s >= target && s0 < target) sh.bin_at = j;
+        }
+        __syncthreads();
+        return sh.bin_at;
+    };
+    // the tokens that `inside` picks to the first CTA's list
+    auto gather = [&](auto inside) {
+        SrShared *first = cl.map_shared_rank(&sh, 0);
+        sync();
+        if (rank == 0 && tid == 0) sh.list_n = 0;
+        sync();
+        for (int i = tid; i < n; i += SR_THREADS) {
+            const float d = val[i];
+            if (inside(d, i0 + i)) {
+                const int k = atomicAdd(&first->list_n, 1);
+                if (k < SR_LIST) {
+                    first->list.key[k] = ((u64)__float_as_uint(d) << 32) | (uint32_t)(i0 + i);
+                    first->list.w[k] = sr_units(sr_weight(R, d, sh.pow2));
+                }
+            }
+        }
+        sync();
+    };
+    // the first place in the order where the running sum reaches target
+    auto find = [&](u64 target, bool count) {
+        if (!top_valid) bin_row(true);
+        u64 before_w = 0, before_c = 0;
+        // level 0: the row by distance; 1: distances in [klo, khi] by their bits; 2: one
+        // distance, indices in [ilo, ihi]. A level that does not leave fewer tokens
+        // cannot come twice: a bin of bits or indices holds fewer than the whole range.
+        int level = 0, shift = 0, klo = 0, khi = 0x7FFFFFFF, ilo = 0, ihi = 0x7FFFFFFF;
+        for (;;) {
+            const int at = bin_at(target, count, before_w, before_c);
+            const uint32_t tokens = sh.run_c[at] - (at ? sh.run_c[at - 1] : 0);
+            before_w += at ? sh.run_w[at - 1] : 0;
+            before_c += at ? sh.run_c[at - 1] : 0;
+            const int l = level, sf = shift, k0 = klo, k1 = khi, j0 = ilo, j1 = ihi;
+            auto ranged = [=](int k, int i) { return k >= k0 && k <= k1 && i >= j0 && i <= j1; };
+            auto inside = [&](float d, int i) {
+                const int k = __float_as_int(d);
+                return l == 0 ? bin_of(top, d) == at : ranged(k, i) && ((l == 1 ? k - k0 : i - j0) >> sf) == at;
+            };
+            if (tokens <= SR_LIST) {
+                gather(inside);
+                if (rank == 0)
+                    for (int i = tid; i < (int)tokens; i += SR_THREADS) {
+                        const u64 key = sh.list.key[i];
+                        u64 w = before_w, c = before_c;
+                        for (int j = 0; j < (int)tokens; j++)
+                            if (sh.list.key[j] < key) { w += sh.list.w[j]; c++; }
+                        const u64 s0 = count ? c : w, s = count ? c + 1 : w + sh.list.w[i];
+                        if (s0 < target && s >= target)
+                            for (int q = 0; q < nc; q++) {
+                                SrShared *o = cl.map_shared_rank(&sh, q);
+                                o->res_key = key;
+                                o->res_w = w + sh.list.w[i];
+                            }
+                    }
+                sync();
+                return SrFound{sh.res_key, sh.res_w};
+            }
+            // too many: the ranges that its tokens span
+            int a0 = 0x7FFFFFFF, a1 = 0, b0 = 0x7FFFFFFF, b1 = 0;
+            for (int i = tid; i < n; i += SR_THREADS)
+                if (inside(val[i], i0 + i)) {
+                    const int k = __float_as_int(val[i]);
+                    a0 = min(a0, k);
+                    a1 = max(a1, k);
+                    b0 = min(b0, i0 + i);
+                    b1 = max(b1, i0 + i);
+                }
+            a0 = __reduce_min_sync(~0u, a0);
+            a1 = __reduce_max_sync(~0u, a1);
+            b0 = __reduce_min_sync(~0u, b0);
+            b1 = __reduce_max_sync(~0u, b1);
+            __syncthreads();
+            if (tid == 0) { sh.lo_k = sh.hi_i = 0x7FFFFFFF; sh.hi_k = 0; sh.list_n = 0; }
+            __syncthreads();
+            if (lane == 0) {
+                atomicMin(&sh.lo_k, a0);
+                atomicMax(&sh.hi_k, a1);
+                atomicMin(&sh.hi_i, b0);
+                atomicMax(&sh.list_n, b1);
+            }
+            sync();
+            klo = ilo = 0x7FFFFFFF;
+            khi = ihi = 0;
+            for (int q = 0; q < nc; q++) {
+                const SrShared *o = cl.map_shared_rank(&sh, q);
+                klo = min(klo, o->lo_k);
+                khi = max(khi, o->hi_k);
+                ilo = min(ilo, o->hi_i);
+                ihi = max(ihi, o->list_n);
+            }
+            level = klo == khi ? 2 : 1;
+            const int width = level == 1 ? khi - klo : ihi - ilo;
+            shift = 0;
+            while ((width >> shift) >= SR_BINS) shift++;
+            clear();
+            for (int i = tid; i < n; i += SR_THREADS) {
+                const float d = val[i];
+                const int k = __float_as_int(d), j = i0 + i;
+                if (k >= klo && k <= khi && j >= ilo && j <= ihi)
+                    add((level == 1 ? k - klo : j - ilo) >> shift, sr_units(sr_weight(R, d, sh.pow2)), true);
+            }
+            merge();
+            top_valid = false;
+        }
+    };
+
+    // ---- the kept weight ----
+    u64 kept = ~0ull, k_sum = 0;
+    SrFound f;
+    if (use_k && !need_total) {
+        // no weights beyond the last of the k: bin by tokens alone
+        bin_row(false);
+        const int at = bin_at((u64)top_k, true, 0, 0);
+        const int tokens = (int)sh.run_c[at];
+        if (tokens <= SR_LIST) {
+            // they and the rest of their bin fit the list: the first CTA does the rest
+            gather([&](float d, int) { return bin_of(top, d) <= at; });
+            if (rank != 0) return;
+            u64 mine[(SR_LIST + SR_THREADS - 1) / SR_THREADS], sum = 0;
+#pragma unroll
+            for (int q = 0; q < (SR_LIST + SR_THREADS - 1) / SR_THREADS; q++) {
+                const int i = q * SR_THREADS + tid;
+                mine[q] = ~0ull;
+                if (i >= tokens) continue;
+                const u64 key = sh.list.key[i];
+                u64 w = 0;
+                int c = 0;
+                for (int j = 0; j < tokens; j++)
+                    if (sh.list.key[j] < key) { w += sh.list.w[j]; c++; }
+                if (c >= top_k) continue;
+                mine[q] = w;
+                if (!use_min || sr_weight(R, __uint_as_float((uint32_t)(key >> 32)), sh.pow2) >= (double)min_p)
+                    sum += sh.list.w[i];
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+            if (lane == 0) sh.part_w[warp] = sum;
+            __syncthreads();
+            sum = 0;
+            for (int k = 0; k < SR_WARPS; k++) sum += sh.part_w[k];
+            const u64 r = min((u64)((u > 0.0f ? (double)fminf(u, 1.0f) : 0.0) * (double)sum), sum - 1);
+#pragma unroll
+            for (int q = 0; q < (SR_LIST + SR_THREADS - 1) / SR_THREADS; q++) {
+                const int i = q * SR_THREADS + tid;
+                if (mine[q] <= r && r < mine[q] + sh.list.w[min(i, SR_LIST - 1)]) a.out[row] = (int)(sh.list.key[i] & 0xFFFFFFFFu);
+            }
+            return;
+        }
+        f = find((u64)top_k, true);
+        weigh_to = __uint_as_float((uint32_t)(f.key >> 32));
+        top = binning(weigh_to);
+        k_sum = bin_row(true);
+        f = find((u64)top_k, true);
+        kept = f.w;
+    } else {
+        if (!need_total) {                // min_p alone, with a margin for the rounding of this bound
+            weigh_to = (float)fmin(-log((double)min_p) * (double)temp * 1.0001 + 1e-30, 3.4e38);
+            top = binning(fminf(far, weigh_to));
+        }
+        k_sum = bin_row(true);
+        kept = sh.run_w[SR_BINS - 1];
+        const u64 total = kept;
+        if (use_p) {
+            const double want = ceil((double)top_p * (double)total);
+            f = find(max(1ull, min((u64)want, total)), false);
+            kept = min(kept, f.w);
+        }
+        if (use_k) {
+            f = find((u64)top_k, true);
+            kept = min(kept, f.w);
+        }
     }
-    if (top_p > 0.0f && top_p < 1.0f) {
-        const unsigned long long target = (unsigned long long)ceil((double)top_p * (double)total);
-        find(max(1ull, min(target, total)), false, &w);
-        kept = min(kept, w);
+    if (use_min) {
+        // the weight of what min_p keeps, over the cluster
+#pragma unroll
+        for (int o = 16; o; o >>= 1) k_sum += __shfl_xor_sync(~0u, k_sum, o);
+        __syncthreads();
+        if (lane == 0) sh.part_w[warp] = k_sum;
+        __syncthreads();
+        k_sum = 0;
+        for (int k = 0; k < SR_WARPS; k++) k_sum += sh.part_w[k];
+        if (nc > 1) {
+            if (tid == 0) sh.sum_w[0] = k_sum;
+            cl.sync();
+            k_sum = 0;
+            for (int q = 0; q < nc; q++) k_sum += cl.map_shared_rank(&sh, q)->sum_w[0];
+        }
+        kept = min(kept, k_sum);
     }
-    const float u = a.u[row];
-    const double r = (u > 0.0f ? (double)fminf(u, 1.0f) : 0.0) * (double)kept;
-    const unsigned long long before = min((unsigned long long)r, kept - 1);
-    const int tok = find(before + 1, false, &w);
-    if (tid == 0) a.out[row] = tok;
+    // ---- the draw ----
+    const double at = (u > 0.0f ? (double)fminf(u, 1.0f) : 0.0) * (double)kept;
+    const u64 before = min((u64)at, kept - 1);
+    f = find(before + 1, false);
+    if (rank == 0 && tid == 0) a.out[row] = (int)(f.key & 0xFFFFFFFFu);
+}
+
+template <typename T>
+static int sample_rows_launch(const EmberSampleRows &a, int n_sm, cudaStream_t st) {
+    constexpr int W = 16 / sizeof(T);
+    // as few CTAs a row as hold it with two of them on an SM, more while SMs are idle
+    int nc = 1;
+    while (nc < SR_MAX_CLUSTER && (a.vocab + nc - 1) / nc > 20480) nc *= 2;
+    while (nc < SR_MAX_CLUSTER && (long long)a.n_rows * nc * 2 <= n_sm && a.vocab / (nc * 2) >= 2048) nc *= 2;
+    const int slice = (a.vocab + nc * W - 1) / (nc * W) * W;
+    const size_t smem = (sizeof(SrShared) + 15) / 16 * 16 + (size_t)slice * 4;
+    const bool vec = !((uintptr_t)a.logits % 16 || (a.stride * (int64_t)sizeof(T)) % 16);
+    int dev = 0;
+    CK(cudaGetDevice(&dev));
+    static std::atomic<unsigned long long> ready{0};      // devices whose limit is raised
+    if (dev >= 64 || !((ready.load(std::memory_order_acquire) >> dev) & 1)) {
+        const size_t most = (sizeof(SrShared) + 15) / 16 * 16 + (size_t)EMBER_SAMPLE_MAX_VOCAB / SR_MAX_CLUSTER * 4;
+        CK(cudaFuncSetAttribute(sample_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+        if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
+    }
+    if ((long long)a.n_rows * nc > 0x7FFFFFFFll) return set_err("sample rows: too many rows");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.n_rows * nc));
+    cfg.blockDim = dim3(SR_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)nc;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    CK(cudaLaunchKernelEx(&cfg, sample_rows_kernel<T>, a, slice, vec));
+    return 0;
 }
 
 }  // namespace emb
@@ -169,10 +560,7 @@ extern "C" int ember_cuda_sample_rows(const EmberSampleRows *args, void *stream)
     CK(cudaGetDevice(&prev));
     if (prev != dev) CK(cudaSetDevice(dev));
     cudaStream_t st = (cudaStream_t)stream;
-    if (a.dtype == EMBER_DT_F32) sample_rows_kernel<float><<<a.n_rows, SR_THREADS, 0, st>>>(a);
-    else sample_rows_kernel<__half><<<a.n_rows, SR_THREADS, 0, st>>>(a);
-    const cudaError_t e = cudaGetLastError();
+    const int rc = a.dtype == EMBER_DT_F32 ? sample_rows_launch<float>(a, 148, st) : sample_rows_launch<__half>(a, 148, st);
     if (prev != dev) cudaSetDevice(prev);
-    if (e != cudaSuccess) return set_err("%s: %s", who, cudaGetErrorString(e));
-    return 0;
+    return rc;
 }
