@@ -38,12 +38,15 @@ static_assert(SR_BINS == 2 * SR_THREADS, "two bins a thread");
 
 typedef unsigned long long u64;
 
-// One CTA's shared memory; the row's slice of S logits follows.
+constexpr int SR_SUB = SR_THREADS;        // finer bins of the listed tokens
+constexpr int SR_FEW = 64;                // listed tokens compared with each other at once
+
+// One CTA's shared memory; the row's slice of logits follows.
 struct SrShared {
     union {
         struct {
             u64 w[SR_BINS];               // this CTA's bins: weights ...
-            uint32_t c[SR_BINS];          // ... and tokens
+            uint32_t c[SR_BINS];          // ... and, where top_k needs them, tokens
         } bin;
         struct {
             u64 key[SR_LIST], w[SR_LIST]; // the first CTA: tokens of the bin that is looked through
@@ -51,25 +54,28 @@ struct SrShared {
     };
     u64 run_w[SR_BINS];                   // running sums over the row's bins
     uint32_t run_c[SR_BINS];
+    u64 sub_w[SR_SUB];                    // the first CTA: sums of the finer bins
+    uint32_t sub_c[SR_SUB];
+    int few[SR_LIST];                     // tokens of one of them
     double pow2[64];                      // 2^(j/64)
-    u64 part_w[SR_WARPS], sum_w[2];       // block sums; the CTA's total and kept weight
+    u64 part_w[SR_WARPS], sum_w;          // block sums; the CTA's weight within min_p
     uint32_t part_c[SR_WARPS];
     float part_hi[SR_WARPS], part_lo[SR_WARPS], hi, lo;
     int part_i[SR_WARPS], hi_i;
-    int list_n;
-    // result of a search: position in the order
-    u64 res_key, res_w;
-    int bin_at, hi_k, lo_k;
+    int list_n[2], few_n;
+    u64 at_w, at_c;                       // running sums before a bin that is looked through
+    u64 res_key, res_w;                   // a search's result
+    int bin_at;
 };
 
 EMB_DEV float sr_logit(float v) { return v != v ? -INFINITY : v; }
 
-// exp(x) for x <= 0 in multiples of 2^-44, rounded to nearest: 2^(k/64) from the
-// table, times exp(f * ln2/64), |f| <= 1/2, by its Taylor polynomial of degree 4
-// (the next term is below 4e-14, a multiple's half being 2.8e-14)
-EMB_DEV double sr_exp(double x, const double *pow2) {
+// 2^(y/64) for -2000 < y <= 0: 2^(k/64) from the table, k the nearest integer, times
+// exp(f * ln2/64), |f| <= 1/2, by its Taylor polynomial of degree 4 (the next term is
+// below 4e-14, a weight's rounding 2.8e-14). 11 double-precision operations; the
+// library's exp takes some 30.
+EMB_DEV double sr_exp2_64(double y, const double *pow2) {
     constexpr double C = 0.69314718055994530942 / 64.0;
-    const double y = x * (64.0 / 0.69314718055994530942);
     const double t = y + 6755399441055744.0;                 // 1.5 * 2^52: the nearest integer
     const int k = (int)__double_as_longlong(t);
     const double f = y - (t - 6755399441055744.0);
@@ -83,12 +89,11 @@ EMB_DEV double sr_exp(double x, const double *pow2) {
 }
 
 struct SrRow {
-    float mx;
-    double inv_t;
-    float limit;                          // distances above it weigh nothing: w < 2^-45
+    float mx, limit;                      // distances above limit weigh nothing: w < 2^-45
+    double slope;                         // -64 / (temperature * ln 2)
 };
 EMB_DEV double sr_weight(const SrRow &r, float dist, const double *pow2) {
-    return dist == 0.0f ? 1.0 : dist > r.limit ? 0.0 : sr_exp(-(double)dist * r.inv_t, pow2);
+    return dist > r.limit ? 0.0 : sr_exp2_64((double)dist * r.slope, pow2);
 }
 // w is in [0, 1]: adding 2^52 to w * 2^44 leaves the integer in the mantissa
 EMB_DEV u64 sr_units(double w) {
@@ -102,6 +107,26 @@ EMB_DEV void sr_add(u64 *at, u64 v) {
     const uint32_t lo = (uint32_t)v, old = atomicAdd(p, lo);
     const uint32_t hi = (uint32_t)(v >> 32) + (old + lo < old ? 1u : 0u);
     if (hi) atomicAdd(p + 1, hi);
+}
+
+// Level 0 bins: proportional to the distance, so a bin's tokens are neighbours in the
+// order; the last bin holds what is farther than the scale's reach (also inf * 0).
+EMB_DEV int sr_bin(float scale, float d) { return (int)fminf(d * scale, (float)(SR_BINS - 1)); }
+
+// The bits of the smallest distance in bin `at` or a later one, by a whole warp: next
+// to at / scale, as rounding has it; by bisection should it not be there.
+EMB_DEV int sr_bin_start(float scale, int at, int lane) {
+    if (at == 0) return 0;
+    const int guess = max(0, __float_as_int(fminf((float)at / scale, 3.0e38f)) - 16) + lane;
+    const unsigned in = __ballot_sync(~0u, sr_bin(scale, __int_as_float(guess)) >= at);
+    if (in && !(in & 1)) return __shfl_sync(~0u, guess, __ffs(in) - 1);
+    int k0 = 0, k1 = 0x7F800000;          // k1 is in bin `at` or later: infinity is in the last one
+    while (k1 - k0 > 1) {
+        const int m = k0 + (k1 - k0) / 2;
+        if (sr_bin(scale, __int_as_float(m)) >= at) k1 = m;
+        else k0 = m;
+    }
+    return k1;
 }
 
 // where a running sum reaches its target
@@ -123,7 +148,20 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
     const float temp = a.temperature ? a.temperature[row] : 1.0f;
     const float top_p = a.top_p ? a.top_p[row] : 1.0f, min_p = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
     const int top_k = a.top_k ? a.top_k[row] : 0;
+
+    // ---- what the row needs (while its logits are on their way) ----
+    if (tid < 2) sh.list_n[tid] = 0;
     if (tid < 64) sh.pow2[tid] = exp2((double)tid / 64.0);
+    for (int b = tid; b < SR_BINS; b += SR_THREADS) { sh.bin.w[b] = 0; sh.bin.c[b] = 0; }
+    SrRow R;
+    R.slope = -64.0 / 0.69314718055994530942 / (double)temp;
+    R.limit = (float)fmin(31.25 * (double)temp, 3.4e38);   // exp(-31.25) < 2^-45
+    const bool use_k = top_k > 0 && top_k < a.vocab, use_p = top_p > 0.0f && top_p < 1.0f,
+               use_min = min_p > 0.0f && min_p < 1.0f;
+    const bool need_total = use_p || !(use_k || use_min);
+    float weigh_to = R.limit;             // distances up to which weights are needed
+    if (use_min && !need_total)           // (with a margin for the rounding of this bound)
+        weigh_to = fminf(weigh_to, (float)fmin(-log((double)min_p) * (double)temp * 1.0001 + 1e-30, 3.4e38));
 
     // ---- the slice into shared memory; the row's maximum (first index) and minimum ----
     float hi = -INFINITY, lo = INFINITY;
@@ -164,12 +202,11 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
     if (nc > 1) {
         if (tid == 0) { sh.hi = hi; sh.lo = lo; sh.hi_i = hi_i; }
         cl.sync();
-        hi = -INFINITY; lo = INFINITY; hi_i = 0x7FFFFFFF;
-        for (int r = 0; r < nc; r++) {
-            const SrShared *o = cl.map_shared_rank(&sh, r);
-            take(o->hi, o->hi_i);
-            lo = fminf(lo, o->lo);
-        }
+        const SrShared *o = cl.map_shared_rank(&sh, min(lane, nc - 1));
+        hi = o->hi;
+        lo = o->lo;
+        hi_i = o->hi_i;
+        warp_take();
     }
     const bool greedy = !(temp > 0.0f) || hi == -INFINITY;
     if (greedy) {
@@ -178,52 +215,61 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
         return;
     }
 
-    // ---- distances; what the row needs ----
-    SrRow R;
+    // ---- distances ----
     R.mx = hi;
-    R.inv_t = 1.0 / (double)temp;
-    R.limit = (float)fmin(31.25 * (double)temp, 3.4e38);   // exp(-31.25) < 2^-45
-    const bool use_k = top_k > 0 && top_k < a.vocab, use_p = top_p > 0.0f && top_p < 1.0f,
-               use_min = min_p > 0.0f && min_p < 1.0f;
-    const bool need_total = use_p || !(use_k || use_min);
     // (an infinite maximum: the other infinite logits are as far as it, 0)
     auto dist_of = [&](float v) { return v == R.mx ? 0.0f : R.mx - v; };
-    for (int i = tid; i < n; i += SR_THREADS) val[i] = dist_of(val[i]);
-    __syncthreads();
+    const int n4 = n / 4;
+    float4 *val4 = reinterpret_cast<float4 *>(val);
+    for (int i = tid; i < n4; i += SR_THREADS) {
+        const float4 v = val4[i];
+        val4[i] = make_float4(dist_of(v.x), dist_of(v.y), dist_of(v.z), dist_of(v.w));
+    }
+    for (int i = 4 * n4 + tid; i < n; i += SR_THREADS) val[i] = dist_of(val[i]);
+    // f(distance, index) for every token of the slice, four at a time
+    auto each = [&](auto f) {
+        for (int i = tid; i < n4; i += SR_THREADS) {
+            const float4 v = val4[i];
+            f(v.x, i0 + 4 * i); f(v.y, i0 + 4 * i + 1); f(v.z, i0 + 4 * i + 2); f(v.w, i0 + 4 * i + 3);
+        }
+        for (int i = 4 * n4 + tid; i < n; i += SR_THREADS) f(val[i], i0 + i);
+    };
+    auto sync = [&]() {
+        if (nc > 1) cl.sync();
+        else __syncthreads();
+    };
     const float far = lo == INFINITY ? 0.0f : dist_of(lo);           // of the finite logits (inf if they overflow)
-    const float far_w = fminf(far, R.limit);
 
     // ---- bins ----
-    // Bin of a distance: monotone, so a bin's tokens are neighbours in the order; the
-    // last bin holds what is farther than `to`.
-    auto binning = [&](float to) {
-        float scale = fminf((float)(SR_BINS - 2) / fmaxf(to, 1e-30f), 3.0e38f);
-        return scale;
+    auto binning = [&](float to) { return fminf((float)(SR_BINS - 2) / fmaxf(to, 1e-30f), 3.0e38f); };
+    auto clear = [&]() {
+        sync();                           // nobody reads the bins or the list any more
+        for (int b = tid; b < SR_BINS; b += SR_THREADS) { sh.bin.w[b] = 0; sh.bin.c[b] = 0; }
+        __syncthreads();
     };
-    auto bin_of = [&](float scale, float d) { return (int)fminf(d * scale, (float)(SR_BINS - 1)); };
+    auto add = [&](int b, u64 w) {
+        if (use_k) atomicAdd(&sh.bin.c[b], 1u);
+        if (w) sr_add(&sh.bin.w[b], w);
+    };
     // the row's running sums over the bins, the same in every CTA
     auto merge = [&]() {
-        if (nc > 1) cl.sync();
-        else __syncthreads();
-        // this CTA adds up its share of the bins and tells all
-        const int share = SR_BINS / nc;
-        for (int j = tid; j < share; j += SR_THREADS) {
-            const int b = rank * share + j;
-            u64 w = 0;
-            uint32_t c = 0;
-            for (int r = 0; r < nc; r++) {
-                const SrShared *o = cl.map_shared_rank(&sh, r);
-                w += o->bin.w[b];
-                c += o->bin.c[b];
+        sync();
+        // this CTA adds up its share of the bins and tells all; nc lanes a bin, each with
+        // one CTA's, so that the remote reads are under way together
+        const int per = SR_THREADS / nc, q = tid & (nc - 1);
+        SrShared *o = cl.map_shared_rank(&sh, q);
+        for (int j = tid / nc; j < SR_BINS / nc; j += per) {
+            const int b = rank * (SR_BINS / nc) + j;
+            u64 w = o->bin.w[b];
+            uint32_t c = use_k ? o->bin.c[b] : 0;
+            for (int d = nc / 2; d; d /= 2) {
+                w += __shfl_xor_sync(~0u, w, d);
+                c += __shfl_xor_sync(~0u, c, d);
             }
-            for (int r = 0; r < nc; r++) {
-                SrShared *o = cl.map_shared_rank(&sh, r);
-                o->run_w[b] = w;
-                o->run_c[b] = c;
-            }
+            o->run_w[b] = w;
+            o->run_c[b] = c;
         }
-        if (nc > 1) cl.sync();
-        else __syncthreads();
+        sync();
         u64 w0 = sh.run_w[2 * tid], w1 = sh.run_w[2 * tid + 1], w = w0 + w1;
         uint32_t c0 = sh.run_c[2 * tid], c1 = sh.run_c[2 * tid + 1], c = c0 + c1;
         const u64 mw = w;
@@ -243,47 +289,31 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
         sh.run_c[2 * tid + 1] = c;
         __syncthreads();
     };
-    auto clear = [&]() {
-        if (nc > 1) cl.sync();            // nobody reads the bins or the list any more
-        else __syncthreads();
-        for (int b = tid; b < SR_BINS; b += SR_THREADS) { sh.bin.w[b] = 0; sh.bin.c[b] = 0; }
-        __syncthreads();
-    };
-    auto add = [&](int b, u64 w, bool on) {
-        if (!on) return;
-        atomicAdd(&sh.bin.c[b], 1u);
-        if (w) sr_add(&sh.bin.w[b], w);
-    };
 
     // the whole row, its weights where the row needs them
-    float top = binning(use_k ? far : far_w);
-    bool top_valid = false;
-    float weigh_to = INFINITY;            // distances up to which weights are needed
-    u64 kept_min = ~0ull;
+    float top = binning(use_k ? far : fminf(far, weigh_to));
+    bool top_valid = false, clean = true;
+    u64 in_min = 0;                       // this thread's weight within min_p
     auto bin_row = [&](bool weights) {
-        clear();
-        u64 k = 0;
-        for (int i = tid; i < n; i += SR_THREADS) {
-            const float d = val[i];
+        if (!clean) clear();              // the first time the bins are zeros
+        clean = false;
+        in_min = 0;
+        each([&](float d, int) {
             u64 w = 0;
             if (weights && d <= weigh_to) {
-                const double e = sr_weight(R, d, sh.pow2);
+                const double e = sr_exp2_64((double)d * R.slope, sh.pow2);
                 w = sr_units(e);
-                if (e >= (double)min_p) k += w;
+                if (use_min && e >= (double)min_p) in_min += w;
             }
-            add(bin_of(top, d), w, true);
-        }
+            add(sr_bin(top, d), w);
+        });
         merge();
         top_valid = true;
-        return k;
     };
-    auto sync = [&]() {
-        if (nc > 1) cl.sync();
-        else __syncthreads();
-    };
-    // the bin in which the running sum, `before` at the first one's start, reaches the
-    // target (the last bin, should it reach it nowhere)
-    auto bin_at = [&](u64 target, bool count, u64 before_w, u64 before_c) {
+    // the bin in which the running sum, before_* at the first one's start, reaches the
+    // target (the last bin, should it reach it nowhere), and, for level 0, its distances
+    int k_first = 0, k_last = 0x7F800000;
+    auto bin_at = [&](u64 target, bool count, u64 before_w, u64 before_c, bool bounds) {
         if (tid == 0) sh.bin_at = SR_BINS - 1;
         __syncthreads();
         for (int j = tid; j < SR_BINS; j += SR_THREADS) {
@@ -293,201 +323,227 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
             if (s >= target && s0 < target) sh.bin_at = j;
         }
         __syncthreads();
-        return sh.bin_at;
+        const int at = sh.bin_at;
+        if (bounds) {
+            k_first = sr_bin_start(top, at, lane);
+            k_last = at < SR_BINS - 1 ? sr_bin_start(top, at + 1, lane) - 1 : 0x7F800000;
+        }
+        return at;
     };
-    // the tokens that `inside` picks to the first CTA's list
-    auto gather = [&](auto inside) {
+    // tokens with a distance (its bits) in [k0, k1] and an index in [j0, j1] to the
+    // first CTA's list; their number, list_n, may be more than the list holds
+    int turn = 0;
+    auto gather = [&](int k0, int k1, int j0, int j1) {
+        // (the list's place was last read before a sync that all have passed; so was the
+        // other counter, which is made ready for the next time)
         SrShared *first = cl.map_shared_rank(&sh, 0);
-        sync();
-        if (rank == 0 && tid == 0) sh.list_n = 0;
-        sync();
-        for (int i = tid; i < n; i += SR_THREADS) {
-            const float d = val[i];
-            if (inside(d, i0 + i)) {
-                const int k = atomicAdd(&first->list_n, 1);
-                if (k < SR_LIST) {
-                    first->list.key[k] = ((u64)__float_as_uint(d) << 32) | (uint32_t)(i0 + i);
-                    first->list.w[k] = sr_units(sr_weight(R, d, sh.pow2));
+        if (rank == 0 && tid == 0) sh.list_n[turn ^ 1] = 0;
+        each([&](float d, int i) {
+            const int k = __float_as_int(d);
+            if (k >= k0 && k <= k1 && i >= j0 && i <= j1) {
+                const int e = atomicAdd(&first->list_n[turn], 1);
+                if (e < SR_LIST) {
+                    first->list.key[e] = ((u64)(uint32_t)k << 32) | (uint32_t)i;
+                    first->list.w[e] = sr_units(sr_weight(R, d, sh.pow2));
                 }
             }
-        }
+        });
         sync();
+        turn ^= 1;
+    };
+    // in the first CTA: which of the list's tokens takes the running sum to target; all
+    // CTAs learn its key and the running weight
+    auto resolve = [&](int tokens, u64 target, bool count, u64 before_w, u64 before_c, int k0, int k1) {
+        int m = tokens;
+        if (tokens > SR_FEW) {
+            // finer bins, by the bits of the distance or, among equals, by index
+            const bool ties = k0 == k1;
+            int j0 = 0, width = k1 - k0;
+            if (ties) width = a.vocab - 1;
+            int shift = 0;
+            while ((width >> shift) >= SR_SUB) shift++;
+            auto sub_of = [&](u64 key) {
+                return (ties ? (int)(uint32_t)key - j0 : (int)(key >> 32) - k0) >> shift;
+            };
+            sh.sub_w[tid] = 0;
+            sh.sub_c[tid] = 0;
+            if (tid == 0) sh.few_n = 0;
+            __syncthreads();
+            for (int i = tid; i < tokens; i += SR_THREADS) {
+                const int b = sub_of(sh.list.key[i]);
+                atomicAdd(&sh.sub_c[b], 1u);
+                sr_add(&sh.sub_w[b], sh.list.w[i]);
+            }
+            __syncthreads();
+            const u64 mw = sh.sub_w[tid];
+            const uint32_t mc = sh.sub_c[tid];
+            u64 w = mw;
+            uint32_t c = mc;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const u64 vw = __shfl_up_sync(~0u, w, o);
+                const uint32_t vc = __shfl_up_sync(~0u, c, o);
+                if (lane >= o) { w += vw; c += vc; }
+            }
+            if (lane == 31) { sh.part_w[warp] = w; sh.part_c[warp] = c; }
+            __syncthreads();
+            for (int k = 0; k < warp; k++) { w += sh.part_w[k]; c += sh.part_c[k]; }
+            const u64 s = count ? before_c + c : before_w + w, s0 = count ? s - mc : s - mw;
+            if (s0 < target && s >= target) {
+                sh.bin_at = tid;
+                sh.at_w = before_w + w - mw;
+                sh.at_c = before_c + c - mc;
+            }
+            __syncthreads();
+            for (int i = tid; i < tokens; i += SR_THREADS)
+                if (sub_of(sh.list.key[i]) == sh.bin_at) sh.few[atomicAdd(&sh.few_n, 1)] = i;
+            __syncthreads();
+            m = sh.few_n;
+            before_w = sh.at_w;
+            before_c = sh.at_c;
+        } else {
+            if (tid < tokens) sh.few[tid] = tid;
+            __syncthreads();
+        }
+        for (int e = tid; e < m; e += SR_THREADS) {
+            const int i = sh.few[e];
+            const u64 key = sh.list.key[i];
+            u64 w = before_w, c = before_c;
+            for (int j = 0; j < m; j++)
+                if (sh.list.key[sh.few[j]] < key) { w += sh.list.w[sh.few[j]]; c++; }
+            const u64 s0 = count ? c : w, s = count ? c + 1 : w + sh.list.w[i];
+            if (s0 < target && s >= target)
+                for (int q = 0; q < nc; q++) {
+                    SrShared *o = cl.map_shared_rank(&sh, q);
+                    o->res_key = key;
+                    o->res_w = w + sh.list.w[i];
+                }
+        }
     };
     // the first place in the order where the running sum reaches target
     auto find = [&](u64 target, bool count) {
-        if (!top_valid) bin_row(true);
         u64 before_w = 0, before_c = 0;
-        // level 0: the row by distance; 1: distances in [klo, khi] by their bits; 2: one
-        // distance, indices in [ilo, ihi]. A level that does not leave fewer tokens
-        // cannot come twice: a bin of bits or indices holds fewer than the whole range.
-        int level = 0, shift = 0, klo = 0, khi = 0x7FFFFFFF, ilo = 0, ihi = 0x7FFFFFFF;
+        // the part of the row that is binned: level 0, all by distance; 1, distances in
+        // [k0, k1] by their bits; 2, one distance, by index. Each level's bin is a
+        // 1/1024 of its range, so there are at most 4 of bits and 2 of indices.
+        int level = 0, shift = 0, k0 = 0, k1 = 0x7F800000, j0 = 0, j1 = 0x7FFFFFFF;
         for (;;) {
-            const int at = bin_at(target, count, before_w, before_c);
-            const uint32_t tokens = sh.run_c[at] - (at ? sh.run_c[at - 1] : 0);
+            const int at = bin_at(target, count, before_w, before_c, level == 0);
             before_w += at ? sh.run_w[at - 1] : 0;
             before_c += at ? sh.run_c[at - 1] : 0;
-            const int l = level, sf = shift, k0 = klo, k1 = khi, j0 = ilo, j1 = ihi;
-            auto ranged = [=](int k, int i) { return k >= k0 && k <= k1 && i >= j0 && i <= j1; };
-            auto inside = [&](float d, int i) {
-                const int k = __float_as_int(d);
-                return l == 0 ? bin_of(top, d) == at : ranged(k, i) && ((l == 1 ? k - k0 : i - j0) >> sf) == at;
-            };
+            if (level == 0) {
+                k0 = k_first;
+                k1 = k_last;
+            } else if (level == 1) {
+                k1 = min((long long)k1, k0 + ((at + 1ll) << shift) - 1);
+                k0 += at << shift;
+            } else {
+                j1 = min((long long)j1, j0 + ((at + 1ll) << shift) - 1);
+                j0 += at << shift;
+            }
+            gather(k0, k1, j0, j1);
+            const int tokens = cl.map_shared_rank(&sh, 0)->list_n[turn ^ 1];
             if (tokens <= SR_LIST) {
-                gather(inside);
-                if (rank == 0)
-                    for (int i = tid; i < (int)tokens; i += SR_THREADS) {
-                        const u64 key = sh.list.key[i];
-                        u64 w = before_w, c = before_c;
-                        for (int j = 0; j < (int)tokens; j++)
-                            if (sh.list.key[j] < key) { w += sh.list.w[j]; c++; }
-                        const u64 s0 = count ? c : w, s = count ? c + 1 : w + sh.list.w[i];
-                        if (s0 < target && s >= target)
-                            for (int q = 0; q < nc; q++) {
-                                SrShared *o = cl.map_shared_rank(&sh, q);
-                                o->res_key = key;
-                                o->res_w = w + sh.list.w[i];
-                            }
-                    }
+                if (rank == 0) resolve(tokens, target, count, before_w, before_c, k0, k1);
                 sync();
                 return SrFound{sh.res_key, sh.res_w};
             }
-            // too many: the ranges that its tokens span
-            int a0 = 0x7FFFFFFF, a1 = 0, b0 = 0x7FFFFFFF, b1 = 0;
-            for (int i = tid; i < n; i += SR_THREADS)
-                if (inside(val[i], i0 + i)) {
-                    const int k = __float_as_int(val[i]);
-                    a0 = min(a0, k);
-                    a1 = max(a1, k);
-                    b0 = min(b0, i0 + i);
-                    b1 = max(b1, i0 + i);
-                }
-            a0 = __reduce_min_sync(~0u, a0);
-            a1 = __reduce_max_sync(~0u, a1);
-            b0 = __reduce_min_sync(~0u, b0);
-            b1 = __reduce_max_sync(~0u, b1);
-            __syncthreads();
-            if (tid == 0) { sh.lo_k = sh.hi_i = 0x7FFFFFFF; sh.hi_k = 0; sh.list_n = 0; }
-            __syncthreads();
-            if (lane == 0) {
-                atomicMin(&sh.lo_k, a0);
-                atomicMax(&sh.hi_k, a1);
-                atomicMin(&sh.hi_i, b0);
-                atomicMax(&sh.list_n, b1);
-            }
-            sync();
-            klo = ilo = 0x7FFFFFFF;
-            khi = ihi = 0;
-            for (int q = 0; q < nc; q++) {
-                const SrShared *o = cl.map_shared_rank(&sh, q);
-                klo = min(klo, o->lo_k);
-                khi = max(khi, o->hi_k);
-                ilo = min(ilo, o->hi_i);
-                ihi = max(ihi, o->list_n);
-            }
-            level = klo == khi ? 2 : 1;
-            const int width = level == 1 ? khi - klo : ihi - ilo;
+            if (k0 == k1 && level != 2) { j0 = 0; j1 = a.vocab - 1; }
+            level = k0 == k1 ? 2 : 1;
+            const int width = level == 1 ? k1 - k0 : j1 - j0;
             shift = 0;
             while ((width >> shift) >= SR_BINS) shift++;
             clear();
-            for (int i = tid; i < n; i += SR_THREADS) {
-                const float d = val[i];
-                const int k = __float_as_int(d), j = i0 + i;
-                if (k >= klo && k <= khi && j >= ilo && j <= ihi)
-                    add((level == 1 ? k - klo : j - ilo) >> shift, sr_units(sr_weight(R, d, sh.pow2)), true);
-            }
+            each([&](float d, int i) {
+                const int k = __float_as_int(d);
+                if (k >= k0 && k <= k1 && i >= j0 && i <= j1)
+                    add((level == 1 ? k - k0 : i - j0) >> shift, sr_units(sr_weight(R, d, sh.pow2)));
+            });
             merge();
             top_valid = false;
         }
     };
 
-    // ---- the kept weight ----
-    u64 kept = ~0ull, k_sum = 0;
-    SrFound f;
-    if (use_k && !need_total) {
-        // no weights beyond the last of the k: bin by tokens alone
-        bin_row(false);
-        const int at = bin_at((u64)top_k, true, 0, 0);
-        const int tokens = (int)sh.run_c[at];
-        if (tokens <= SR_LIST) {
-            // they and the rest of their bin fit the list: the first CTA does the rest
-            gather([&](float d, int) { return bin_of(top, d) <= at; });
-            if (rank != 0) return;
-            u64 mine[(SR_LIST + SR_THREADS - 1) / SR_THREADS], sum = 0;
+    // ---- the searches: the last of the k where no total is needed, then top_p, top_k
+    // and the draw (one loop, so that the search is in the code once) ----
+    u64 kept = ~0ull;
+    for (int stage = 0; stage < 4; stage++) {
+        if ((stage == 0 && (!use_k || need_total)) || (stage == 1 && !use_p) || (stage == 2 && !use_k)) continue;
+        if (!top_valid) bin_row(stage > 0);
+        u64 target = (u64)top_k;
+        if (stage == 0) {
+            // no weights beyond the last of the k: binned by tokens alone
+            const int at = bin_at(target, true, 0, 0, true);
+            const int tokens = (int)sh.run_c[at];
+            if (tokens <= SR_LIST) {
+                // they and the rest of their bin fit the list: the first CTA does the rest
+                gather(0, k_last, 0, 0x7FFFFFFF);
+                if (rank != 0) return;
+                constexpr int Q = (SR_LIST + SR_THREADS - 1) / SR_THREADS;
+                u64 mine[Q], sum = 0;
 #pragma unroll
-            for (int q = 0; q < (SR_LIST + SR_THREADS - 1) / SR_THREADS; q++) {
-                const int i = q * SR_THREADS + tid;
-                mine[q] = ~0ull;
-                if (i >= tokens) continue;
-                const u64 key = sh.list.key[i];
+                for (int q = 0; q < Q; q++) {
+                    const int i = q * SR_THREADS + tid;
+                    mine[q] = ~0ull;
+                    if (i >= tokens) continue;
+                    const u64 key = sh.list.key[i];
+                    u64 w = 0;
+                    int c = 0;
+                    for (int j = 0; j < tokens; j++)
+                        if (sh.list.key[j] < key) { w += sh.list.w[j]; c++; }
+                    if (c >= top_k) continue;
+                    mine[q] = w;
+                    if (!use_min || sr_weight(R, __uint_as_float((uint32_t)(key >> 32)), sh.pow2) >= (double)min_p)
+                        sum += sh.list.w[i];
+                }
+#pragma unroll
+                for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+                if (lane == 0) sh.part_w[warp] = sum;
+                __syncthreads();
+                sum = 0;
+                for (int k = 0; k < SR_WARPS; k++) sum += sh.part_w[k];
+                const u64 r = min((u64)((u > 0.0f ? (double)fminf(u, 1.0f) : 0.0) * (double)sum), sum - 1);
+#pragma unroll
+                for (int q = 0; q < Q; q++) {
+                    const int i = min(q * SR_THREADS + tid, SR_LIST - 1);
+                    if (mine[q] <= r && r < mine[q] + sh.list.w[i]) a.out[row] = (int)(sh.list.key[i] & 0xFFFFFFFFu);
+                }
+                return;
+            }
+        } else if (stage == 1) {
+            const u64 total = sh.run_w[SR_BINS - 1];
+            target = max(1ull, min((u64)ceil((double)top_p * (double)total), total));
+        } else if (stage == 3) {
+            kept = min(kept, sh.run_w[SR_BINS - 1]);
+            if (use_min) {
+                // the weight of what min_p keeps, over the cluster
+#pragma unroll
+                for (int o = 16; o; o >>= 1) in_min += __shfl_xor_sync(~0u, in_min, o);
+                if (lane == 0) sh.part_w[warp] = in_min;
+                __syncthreads();
+                if (tid == 0) {
+                    u64 w = 0;
+                    for (int k = 0; k < SR_WARPS; k++) w += sh.part_w[k];
+                    sh.sum_w = w;
+                }
+                sync();
                 u64 w = 0;
-                int c = 0;
-                for (int j = 0; j < tokens; j++)
-                    if (sh.list.key[j] < key) { w += sh.list.w[j]; c++; }
-                if (c >= top_k) continue;
-                mine[q] = w;
-                if (!use_min || sr_weight(R, __uint_as_float((uint32_t)(key >> 32)), sh.pow2) >= (double)min_p)
-                    sum += sh.list.w[i];
+                for (int q = 0; q < nc; q++) w += cl.map_shared_rank(&sh, q)->sum_w;
+                kept = min(kept, w);
             }
-#pragma unroll
-            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-            if (lane == 0) sh.part_w[warp] = sum;
-            __syncthreads();
-            sum = 0;
-            for (int k = 0; k < SR_WARPS; k++) sum += sh.part_w[k];
-            const u64 r = min((u64)((u > 0.0f ? (double)fminf(u, 1.0f) : 0.0) * (double)sum), sum - 1);
-#pragma unroll
-            for (int q = 0; q < (SR_LIST + SR_THREADS - 1) / SR_THREADS; q++) {
-                const int i = q * SR_THREADS + tid;
-                if (mine[q] <= r && r < mine[q] + sh.list.w[min(i, SR_LIST - 1)]) a.out[row] = (int)(sh.list.key[i] & 0xFFFFFFFFu);
-            }
-            return;
+            target = min((u64)((u > 0.0f ? (double)fminf(u, 1.0f) : 0.0) * (double)kept), kept - 1) + 1;
         }
-        f = find((u64)top_k, true);
-        weigh_to = __uint_as_float((uint32_t)(f.key >> 32));
-        top = binning(weigh_to);
-        k_sum = bin_row(true);
-        f = find((u64)top_k, true);
-        kept = f.w;
-    } else {
-        if (!need_total) {                // min_p alone, with a margin for the rounding of this bound
-            weigh_to = (float)fmin(-log((double)min_p) * (double)temp * 1.0001 + 1e-30, 3.4e38);
-            top = binning(fminf(far, weigh_to));
-        }
-        k_sum = bin_row(true);
-        kept = sh.run_w[SR_BINS - 1];
-        const u64 total = kept;
-        if (use_p) {
-            const double want = ceil((double)top_p * (double)total);
-            f = find(max(1ull, min((u64)want, total)), false);
+        const SrFound f = find(target, stage == 0 || stage == 2);
+        if (stage == 0) {
+            weigh_to = fminf(weigh_to, __uint_as_float((uint32_t)(f.key >> 32)));
+            top = binning(weigh_to);
+            top_valid = false;
+        } else if (stage < 3) {
             kept = min(kept, f.w);
-        }
-        if (use_k) {
-            f = find((u64)top_k, true);
-            kept = min(kept, f.w);
+        } else if (rank == 0 && tid == 0) {
+            a.out[row] = (int)(f.key & 0xFFFFFFFFu);
         }
     }
-    if (use_min) {
-        // the weight of what min_p keeps, over the cluster
-#pragma unroll
-        for (int o = 16; o; o >>= 1) k_sum += __shfl_xor_sync(~0u, k_sum, o);
-        __syncthreads();
-        if (lane == 0) sh.part_w[warp] = k_sum;
-        __syncthreads();
-        k_sum = 0;
-        for (int k = 0; k < SR_WARPS; k++) k_sum += sh.part_w[k];
-        if (nc > 1) {
-            if (tid == 0) sh.sum_w[0] = k_sum;
-            cl.sync();
-            k_sum = 0;
-            for (int q = 0; q < nc; q++) k_sum += cl.map_shared_rank(&sh, q)->sum_w[0];
-        }
-        kept = min(kept, k_sum);
-    }
-    // ---- the draw ----
-    const double at = (u > 0.0f ? (double)fminf(u, 1.0f) : 0.0) * (double)kept;
-    const u64 before = min((u64)at, kept - 1);
-    f = find(before + 1, false);
-    if (rank == 0 && tid == 0) a.out[row] = (int)(f.key & 0xFFFFFFFFu);
 }
 
 template <typename T>
