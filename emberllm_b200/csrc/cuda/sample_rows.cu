@@ -251,6 +251,18 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
         if (use_k) atomicAdd(&sh.bin.c[b], 1u);
         if (w) sr_add(&sh.bin.w[b], w);
     };
+    // adds the sums of the earlier warps (part_*)
+    auto before = [&](u64 &w, uint32_t &c) {
+        u64 pw = lane < warp ? sh.part_w[lane] : 0;
+        uint32_t pc = lane < warp ? sh.part_c[lane] : 0;
+#pragma unroll
+        for (int o = SR_WARPS / 2; o; o >>= 1) {
+            pw += __shfl_xor_sync(~0u, pw, o);
+            pc += __shfl_xor_sync(~0u, pc, o);
+        }
+        w += __shfl_sync(~0u, pw, 0);
+        c += __shfl_sync(~0u, pc, 0);
+    };
     // the row's running sums over the bins, the same in every CTA
     auto merge = [&]() {
         sync();
@@ -282,7 +294,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
         }
         if (lane == 31) { sh.part_w[warp] = w; sh.part_c[warp] = c; }
         __syncthreads();
-        for (int k = 0; k < warp; k++) { w += sh.part_w[k]; c += sh.part_c[k]; }
+        before(w, c);
         sh.run_w[2 * tid] = w - mw + w0;
         sh.run_c[2 * tid] = c - mc + c0;
         sh.run_w[2 * tid + 1] = w;
@@ -298,15 +310,28 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
         if (!clean) clear();              // the first time the bins are zeros
         clean = false;
         in_min = 0;
-        each([&](float d, int) {
-            u64 w = 0;
-            if (weights && d <= weigh_to) {
-                const double e = sr_exp2_64((double)d * R.slope, sh.pow2);
-                w = sr_units(e);
+        if (need_total) {
+            // every token has its weight, one beyond the limit the 0 units of the limit:
+            // no branch but those that all lanes take alike
+            each([&](float d, int) {
+                const double e = sr_exp2_64((double)fminf(d, R.limit) * R.slope, sh.pow2);
+                const u64 w = sr_units(e);
+                const int b = sr_bin(top, d);
                 if (use_min && e >= (double)min_p) in_min += w;
-            }
-            add(sr_bin(top, d), w);
-        });
+                if (use_k) atomicAdd(&sh.bin.c[b], 1u);
+                sr_add(&sh.bin.w[b], w);
+            });
+        } else {
+            each([&](float d, int) {
+                u64 w = 0;
+                if (weights && d <= weigh_to) {
+                    const double e = sr_exp2_64((double)d * R.slope, sh.pow2);
+                    w = sr_units(e);
+                    if (use_min && e >= (double)min_p) in_min += w;
+                }
+                add(sr_bin(top, d), w);
+            });
+        }
         merge();
         top_valid = true;
     };
@@ -338,16 +363,26 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
         // other counter, which is made ready for the next time)
         SrShared *first = cl.map_shared_rank(&sh, 0);
         if (rank == 0 && tid == 0) sh.list_n[turn ^ 1] = 0;
-        each([&](float d, int i) {
-            const int k = __float_as_int(d);
-            if (k >= k0 && k <= k1 && i >= j0 && i <= j1) {
-                const int e = atomicAdd(&first->list_n[turn], 1);
-                if (e < SR_LIST) {
-                    first->list.key[e] = ((u64)(uint32_t)k << 32) | (uint32_t)i;
-                    first->list.w[e] = sr_units(sr_weight(R, d, sh.pow2));
-                }
+        const float d0 = __int_as_float(k0), d1 = __int_as_float(k1);
+        auto push = [&](float d, int i) {
+            if (i < j0 || i > j1) return;
+            const int e = atomicAdd(&first->list_n[turn], 1);
+            if (e < SR_LIST) {
+                first->list.key[e] = ((u64)__float_as_uint(d) << 32) | (uint32_t)i;
+                first->list.w[e] = sr_units(sr_weight(R, d, sh.pow2));
             }
-        });
+        };
+        for (int i = tid; i < n4; i += SR_THREADS) {
+            const float4 v = val4[i];
+            int in = (v.x >= d0 && v.x <= d1) | (v.y >= d0 && v.y <= d1) << 1 | (v.z >= d0 && v.z <= d1) << 2 |
+                     (v.w >= d0 && v.w <= d1) << 3;
+            for (; in; in &= in - 1) {    // mostly none
+                const int e = __ffs(in) - 1;
+                push(e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w, i0 + 4 * i + e);
+            }
+        }
+        for (int i = 4 * n4 + tid; i < n; i += SR_THREADS)
+            if (val[i] >= d0 && val[i] <= d1) push(val[i], i0 + i);
         sync();
         turn ^= 1;
     };
@@ -387,7 +422,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
             }
             if (lane == 31) { sh.part_w[warp] = w; sh.part_c[warp] = c; }
             __syncthreads();
-            for (int k = 0; k < warp; k++) { w += sh.part_w[k]; c += sh.part_c[k]; }
+            before(w, c);
             const u64 s = count ? before_c + c : before_w + w, s0 = count ? s - mc : s - mw;
             if (s0 < target && s >= target) {
                 sh.bin_at = tid;
