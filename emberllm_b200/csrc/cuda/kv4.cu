@@ -1,11 +1,12 @@
 // kv4.cu — the paged 4-bit KV cache: store, read, and the host side of the
-// attention over it (kernels in kv4_attn.cuh).
+// attention over it (kernels in kv4_attn.cuh for few rows
+// per sequence and kv4_prompt.cuh for many).
 #include <cuda_runtime.h>
 
 #include <math.h>
 
 #include "kv4.cuh"
-#include "kv4_attn.cuh"
+#include "kv4_prompt.cuh"
 #include "runtime_internal.cuh"
 
 namespace emb {
@@ -143,6 +144,17 @@ __global__ void __launch_bounds__(KV4_IO_THREADS) kv4_io_kernel(Kv4View c, Kv4Ro
                 for (int j = 0; j < 4; j++) o[j] = __float2half_rn(x[j]);
         }
     }
+}
+
+// Up to this many rows (tokens x query heads of a kv head) a sequence's rows are taken
+// eight at a time, the cache read once for each eight; beyond, 128 at a time.
+constexpr int KV4_FEW_ROWS = 16;
+
+template <typename T>
+static int kv4_attention_launch(const Kv4AttnArgs &a, int hd, cudaStream_t st) {
+    const long long rows = (long long)a.max_q * a.group;
+    if (rows > KV4_FEW_ROWS) return kv4_prompt_hd<T>(a, hd, st);
+    return rows <= 4 ? kv4_decode_hd<T, 1>(a, hd, st) : kv4_decode_hd<T, 2>(a, hd, st);
 }
 
 // ------------------------------------------------------------ host checks ----

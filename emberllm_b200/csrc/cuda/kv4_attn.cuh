@@ -600,9 +600,4 @@ static int kv4_decode_hd(const Kv4AttnArgs &a, int hd, cudaStream_t st) {
     }
 }
 
-template <typename T>
-static int kv4_attention_launch(const Kv4AttnArgs &a, int hd, cudaStream_t st) {
-    return (long long)a.max_q * a.group <= 4 ? kv4_decode_hd<T, 1>(a, hd, st) : kv4_decode_hd<T, 2>(a, hd, st);
-}
-
 }  // namespace emb
