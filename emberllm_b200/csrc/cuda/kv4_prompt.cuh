@@ -349,10 +349,12 @@ __global__ void __launch_bounds__(KP_THREADS, 2) kv4_prompt_kernel(const Kv4Attn
         const uint8_t *base = a.c.data + (size_t)kv * a.c.chunk;
         const uint64_t stride = (uint64_t)a.c.n_kv * a.c.chunk;
         uint8_t *dst = sm + (keys ? L::OFF_K : L::OFF_V);
-        // the group of 16 positions at p0 + 16 i, or null
-        auto group = [&](int p) -> const uint8_t * {
-            if (p >= len) return nullptr;
-            const int page = __ldg(table + (p >> a.c.page_shift));
+        // page of position p (-1: none), asked for two tiles ahead; its group of 16, or null
+        auto page_at = [&](int j, int in_tile) {
+            const int p = range.pos(j) + in_tile;
+            return j < n && p < len ? __ldg(table + (p >> a.c.page_shift)) : -1;
+        };
+        auto group = [&](int page, int p) -> const uint8_t * {
             if ((unsigned)page >= (unsigned)a.c.n_pages) return nullptr;
             return base + (uint64_t)(uint32_t)page * stride + ((p & (ps - 1)) >> 4) * GB;
         };
@@ -384,32 +386,70 @@ __global__ void __launch_bounds__(KP_THREADS, 2) kv4_prompt_kernel(const Kv4Attn
         };
         int done = 0;                     // tiles whose products into O were issued
         bool fine = true;
-        for (int j = 0; j < n; j++) {
-            const int p0 = range.pos(j);
+        // A tile's packed words are loaded while the tile before is made operands.
+        // keys: word column t of the positions half*32 + 8 i + low; values: words g of the
+        // positions 8 c ..
+        const int t = (t64 >> 3) & 3, half = t64 >> 5, low = t64 & 7, c = t64 & 7, g = t64 >> 3;
+        uint32_t nw[4][NB], nd[4][NB];
+        int pg[2] = {-1, -1};
+        auto pages = [&](int j) {
             if (keys) {
-                // thread: word column t of the rows p = 8 k + (lane & 7)
-                const int t = (t64 >> 3) & 3, half = t64 >> 5, low = t64 & 7;
-                uint32_t w[4][NB], d[4][NB < 2 ? 1 : NB / 2];
-                uint64_t ok = 0;
+                pg[0] = page_at(j, half * 32);
+                pg[1] = page_at(j, half * 32 + 16);
+            } else {
+                pg[0] = page_at(j, (c >> 1) * 16);
+            }
+        };
+        uint32_t nok = 0;                 // keys: which of the four positions there are
+        auto load = [&](int j) {
+            const int p0 = range.pos(j);
+            nok = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+#pragma unroll
+                for (int b = 0; b < NB; b++) nw[i][b] = nd[i][b] = 0;
+            }
+            if (j >= n) return;
+            if (keys) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const int p = half * 32 + i * 8 + low;           // position in the tile
-                    const uint8_t *g = group(p0 + (p & ~15));
-                    if (g) {
-                        const int r = p & 15;
-                        lds_words<NB>(w[i], g + r * (HD / 2) + t * (4 * NB));
-                        lds_words<NB / 2>(d[i], g + 16 * HD + r * (2 * NB));
-                        if (p0 + p < len) ok |= 1ull << p;
-                    } else {
+                    const int p = half * 32 + i * 8 + low, r = p & 15;
+                    const uint8_t *gr = group(pg[i >> 1], p0 + p);
+                    if (!gr) continue;
+                    lds_words<NB>(nw[i], gr + r * (HD / 2) + t * (4 * NB));
+                    uint32_t ks[NB < 2 ? 1 : NB / 2];
+                    lds_words<NB / 2>(ks, gr + 16 * HD + r * (2 * NB));
 #pragma unroll
-                        for (int b = 0; b < NB; b++) w[i][b] = 0;
-#pragma unroll
-                        for (int b = 0; b < (NB < 2 ? 1 : NB / 2); b++) d[i][b] = 0;
-                    }
+                    for (int b = 0; b < (NB < 2 ? 1 : NB / 2); b++) nd[i][b] = ks[b];
+                    if (p0 + p < len) nok |= 1u << (i * 8 + low);
                 }
+            } else {
+                const uint8_t *gr = group(pg[0], p0 + (c >> 1) * 16);
+                if (!gr) return;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int pair = (c & 1) * 4 + i;
+                    lds_words<NB>(nw[i], gr + 8 * HD + pair * HD + g * (4 * NB));
+                    lds_words<NB>(nd[i], gr + 16 * HD + 32 * NB + pair * (4 * NB));
+                }
+            }
+        };
+        pages(0);
+        load(0);
+        pages(1);
+        for (int j = 0; j < n; j++) {
+            uint32_t w[4][NB], d[4][NB];
+            const uint32_t ok = nok;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int b = 0; b < NB; b++) { w[i][b] = nw[i][b]; d[i][b] = nd[i][b]; }
+            load(j + 1);
+            pages(j + 2);
+            const int p0 = range.pos(j);
+            if (keys) {
                 // the tile's positions, as a mask (both warps have a half)
-                uint32_t bits = half ? (uint32_t)(ok >> 32) : (uint32_t)ok;
-                bits = __reduce_or_sync(0xffffffffu, bits);
+                const uint32_t bits = __reduce_or_sync(0xffffffffu, ok);
                 if (!__all_sync(0xffffffffu, j == 0 || kp_wait(&sh.k_empty, (j - 1) & 1, abort))) break;
                 if (lane == 0) reinterpret_cast<uint32_t *>(&sh.valid[j & 3])[half] = bits;
 #pragma unroll
@@ -441,25 +481,15 @@ __global__ void __launch_bounds__(KP_THREADS, 2) kv4_prompt_kernel(const Kv4Attn
                 }
                 __syncwarp();
             } else {
-                // thread: value words g of the 8 positions 8 c ..
-                const int c = t64 & 7, g = t64 >> 3;
-                const uint8_t *gr = group(p0 + (c >> 1) * 16);
-                uint32_t w[4][NB], d[4][NB];
+                // positions behind the length may hold any bytes: their scales count as 0
+                if (p0 + KP_POS > len) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int pair = (c & 1) * 4 + i;
-                    if (gr) {
-                        lds_words<NB>(w[i], gr + 8 * HD + pair * HD + g * (4 * NB));
-                        lds_words<NB>(d[i], gr + 16 * HD + 32 * NB + pair * (4 * NB));
-                    } else {
+                    for (int i = 0; i < 4; i++) {
+                        const int left = len - (p0 + 8 * c + 2 * i);
+                        const uint32_t keep = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0x0000FFFFu : 0u;
 #pragma unroll
-                        for (int b = 0; b < NB; b++) w[i][b] = d[i][b] = 0;
+                        for (int b = 0; b < NB; b++) d[i][b] &= keep;
                     }
-                    // positions behind the length may hold any bytes: their scales count as 0
-                    const int left = len - (p0 + 8 * c + 2 * i);
-                    const uint32_t keep = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0x0000FFFFu : 0u;
-#pragma unroll
-                    for (int b = 0; b < NB; b++) d[i][b] &= keep;
                 }
                 if (!__all_sync(0xffffffffu, j == 0 || kp_wait(&sh.v_empty, (j - 1) & 1, abort))) break;
 #pragma unroll
