@@ -1,17 +1,18 @@
 // kv4_prompt.cuh — attention over the paged 4-bit KV cache, many rows per sequence.
 //
-// The same mathematics as kv4_attn.cuh with 128 query rows (tokens x the query heads
-// of a kv head) against tiles of 64 positions on tcgen05, one CTA per (row tile, kv
-// head, sequence), two CTAs on an SM so that one's softmax runs under the other's
-// products. Warps have roles:
-//   0-3  softmax: a thread owns a row; it reads the row's 64 scores from tensor memory,
-//        raises the maximum if a score passes it by 2^8 (then O is rescaled in tensor
-//        memory, which is rare), and writes the weights over the scores
-//   4,5  keys, 6,7 values: packed codes from global memory to exact fp16 numbers
-//        (code - 8) * d in shared memory, swizzled as the products read them; the
-//        values are transposed on the way, so both operands are K-major
-//   4    its first lane also issues the products: S = Q K^T, two tiles in turn, O += P V
-//        with P from tensor memory (a ninth warp for it would leave 96 registers a thread)
+// The same mathematics as kv4_attn.cuh with tiles of 128 query rows (tokens x the query
+// heads of a kv head) against tiles of 64 positions on tcgen05. A CTA takes RT = 2 row
+// tiles, which share the keys and values it unpacks (one CTA on an SM), or 1 where there
+// are few rows (two CTAs on an SM). Warps have roles:
+//   4 per row tile   softmax: a thread owns a row; it reads the row's 64 scores from
+//        tensor memory, raises the maximum if a score passes it by 2^8 (then O is
+//        rescaled in tensor memory, which is rare), and writes the weights over the scores
+//   1   issues the products: S = Q K^T, two position tiles in turn, O += P V with P from
+//        tensor memory (issuing alone takes some 1,200 cycles a tile; when a warp that
+//        unpacks did it too, that warp was what the others waited for)
+//   2   values, 1 or 4   keys: packed codes from global memory, asked for a tile ahead, to
+//        exact fp16 numbers (code - 8) * d in shared memory, swizzled as the products read
+//        them; the values are transposed on the way, so both operands are K-major
 // fp32 queries and weights enter as an fp16 rounding and its rest (two products into
 // the same sums, 22 bits); fp16 queries are exact as they are, and their weights are
 // rounded to 11 bits, which changes an output by less than its own rounding does.
@@ -21,25 +22,32 @@
 
 namespace emb {
 
-constexpr int KP_THREADS = 256, KP_ROWS = 128, KP_POS = 64;
+constexpr int KP_ROWS = 128, KP_POS = 64;
 constexpr unsigned long long KP_WAIT_NS = 1000000000ull;
 
-template <typename T, int HD>
+template <typename T, int HD, int RT>
 struct KpLayout {
     static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;    // fp16 parts of a query and of a weight
+    static constexpr int BUF = RT == 1 && PARTS == 2 ? 1 : 2;   // tiles of keys and of values held
     static constexpr int PANELS = (HD + 63) / 64;           // panels of 64 fp16 (128 bytes) of a row
-    static constexpr int Q_PART = PANELS * KP_ROWS * 128, K_BYTES = PANELS * KP_POS * 128, V_BYTES = HD * 128;
-    static constexpr int OFF_K = PARTS * Q_PART, OFF_V = OFF_K + K_BYTES, OFF_X = OFF_V + V_BYTES;
-    static constexpr int SMEM = OFF_X + 1024;               // + slack to align the base to 1024
-    static constexpr int COLS = 256, COL_O = 128;           // tensor memory: S / P of two tiles, then O
+    static constexpr int Q_PART = PANELS * KP_ROWS * 128, Q_TILE = PARTS * Q_PART;
+    static constexpr int K_BYTES = PANELS * KP_POS * 128, V_BYTES = HD * 128;
+    static constexpr int OFF_K = RT * Q_TILE, OFF_V = OFF_K + BUF * K_BYTES;
+    static constexpr int SMEM = OFF_V + BUF * V_BYTES + 1024;   // + slack to align the base to 1024
+    // tensor memory: S / P of two position tiles per row tile, then O per row tile
+    static constexpr int COLS = RT * 256, COL_O = RT * 128;
+    static constexpr int SOFT = 4 * RT, ISSUE = SOFT, VALS = SOFT + 1, KEYS = SOFT + 3;   // first warps of the roles
+    static constexpr int KEY_WARPS = RT == 2 ? 4 : 1, WARPS = RT == 2 ? 16 : 8;
+    static constexpr int KN = 8 / KEY_WARPS;                // positions a key thread unpacks
 };
 
+template <int RT>
 struct KpShared {
-    uint64_t k_full, k_empty, v_full, v_empty, s_full[2], p_full[2];
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[RT][2], p_full[RT][2], o_done[RT], drain;
     uint32_t tmem;
     int abort;
     uint64_t valid[4];          // which positions of a tile there are, by tile number mod 4
-    float rscale[KP_ROWS];
+    float rscale[RT * KP_ROWS];
 };
 
 // Wait for a phase; gives up after KP_WAIT_NS or as soon as another role has given up,
@@ -133,12 +141,12 @@ EMB_DEV KpRange kp_range(int first_pos, int last_pos, int len, int window, int s
     return r;
 }
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(KP_THREADS, 2) kv4_prompt_kernel(const Kv4AttnArgs a) {
-    using L = KpLayout<T, HD>;
-    constexpr int NB = HD / 32, GB = kv4_group(HD), PARTS = L::PARTS;
+template <typename T, int HD, int RT>
+__global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_prompt_kernel(const Kv4AttnArgs a) {
+    using L = KpLayout<T, HD, RT>;
+    constexpr int NB = HD / 32, GB = kv4_group(HD), PARTS = L::PARTS, BUF = L::BUF;
     extern __shared__ uint8_t kp_raw[];
-    __shared__ KpShared sh;
+    __shared__ KpShared<RT> sh;
     const uint32_t raw = smem_u32(kp_raw);
     uint8_t *sm = kp_raw + ((1024u - (raw & 1023u)) & 1023u);
     const uint32_t sm32 = smem_u32(sm);
@@ -147,90 +155,99 @@ __global__ void __launch_bounds__(KP_THREADS, 2) kv4_prompt_kernel(const Kv4Attn
     const Kv4Seq s = kv4_seq(a.b, seq);
     const int rows = min(s.rows, a.max_q) * a.group;
     // the latest rows see the most positions: they go first
-    const int row_first = ((int)gridDim.x - 1 - (int)blockIdx.x) * KP_ROWS;
+    const int row_first = ((int)gridDim.x - 1 - (int)blockIdx.x) * (RT * KP_ROWS);
     if (row_first >= rows) return;
+    const int row_end = min(rows, row_first + RT * KP_ROWS);
     const int pos0 = s.len - s.rows, len = min(min(s.len, a.max_kv), a.b.cap);
-    const int first_pos = pos0 + row_first / a.group,
-              last_pos = pos0 + (min(rows, row_first + KP_ROWS) - 1) / a.group;
-    const KpRange range = kp_range(first_pos, last_pos, len, a.window, a.sinks);
+    const KpRange range = kp_range(pos0 + row_first / a.group, pos0 + (row_end - 1) / a.group, len, a.window, a.sinks);
     const int n = range.total;
+    const int tiles = RT == 1 || row_end - row_first <= KP_ROWS ? 1 : 2;   // row tiles with rows
 
     if (tid == 0) {
-        mbar_init(&sh.k_full, 64);
-        mbar_init(&sh.k_empty, 1);
-        mbar_init(&sh.v_full, 64);
-        mbar_init(&sh.v_empty, 1);
-        for (int i = 0; i < 2; i++) { mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_full[i], 128); }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&sh.k_full[i], 32 * L::KEY_WARPS);
+            mbar_init(&sh.k_empty[i], 1);
+            mbar_init(&sh.v_full[i], 64);
+            mbar_init(&sh.v_empty[i], 1);
+            for (int r = 0; r < RT; r++) { mbar_init(&sh.s_full[r][i], 1); mbar_init(&sh.p_full[r][i], KP_ROWS); }
+        }
+        for (int r = 0; r < RT; r++) mbar_init(&sh.o_done[r], 1);
+        mbar_init(&sh.drain, 1);
         fence_mbar_init();
         sh.abort = 0;
     }
-    if (warp == 4) {
+    if (warp == L::ISSUE) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
                      "r"((uint32_t)L::COLS)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    {
-        // queries: a warp takes 16 rows; within 8 dims the order is 0,4,1,5,2,6,3,7, as
-        // the keys come out of their words
-        for (int i = 0; i < KP_ROWS / 8; i++) {
-            const int r = warp * (KP_ROWS / 8) + i, rr = row_first + r;
-            float v[NB], m = 0.0f;
-            bool finite = true;
-            const int tok = rr / a.group, h = kv * a.group + rr - tok * a.group;
-            const T *src = (const T *)a.q + (int64_t)(s.row0 + tok) * a.q_tok + h * a.q_head + lane;
+    // queries: a warp takes 16 rows; within 8 dims the order is 0,4,1,5,2,6,3,7, as the
+    // keys come out of their words
+#pragma unroll 4
+    for (int i = 0; i < 16; i++) {
+        const int r = warp * 16 + i, rr = row_first + r;
+        float v[NB], m = 0.0f;
+        bool finite = true;
+        const int tok = rr / a.group, h = kv * a.group + rr - tok * a.group;
+        const T *src = (const T *)a.q + (int64_t)(s.row0 + tok) * a.q_tok + h * a.q_head + lane;
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                v[b] = rr < rows ? widen(src[b * 32]) : 0.0f;
-                finite = finite && fabsf(v[b]) < INFINITY;
-                m = fmaxf(m, fabsf(v[b]));
-            }
-            m = warp_max(m);
-            finite = __all_sync(0xffffffffu, finite);
-            // |q| * 2^e below 2^14; the sign of the scale goes into the queries, so that
-            // a row's largest product is its largest score
-            const int e = m > 0.0f ? 13 - ilogbf(m) : 0;
-            float f1 = __int_as_float((127 + e / 2) << 23);
-            const float f2 = __int_as_float((127 + e - e / 2) << 23);
-            // (never 0: a hidden score, -inf, must stay -inf)
-            if (lane == 0)
-                sh.rscale[r] = a.scale == 0.0f ? 1.0f : fmaxf(fabsf(a.scale) * KV4_LOG2E / f1 / f2, 1.2e-38f);
-            if (a.scale < 0.0f) f1 = -f1;
-            if (a.scale == 0.0f) f1 = 0.0f;
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                const float y = finite ? v[b] * f1 * f2 : __int_as_float(0x7fffffff);
-                const int d = b * 32 + lane, c = d >> 3, k = d & 7, p = k < 4 ? 2 * k : 2 * k - 7;
-                const uint32_t at = (c >> 3) * (KP_ROWS * 128) + kp_chunk(r, c & 7) + 2 * p;
-                const __half hi = __float2half_rn(y);
-                *reinterpret_cast<__half *>(sm + at) = hi;
-                if (PARTS == 2)
-                    *reinterpret_cast<__half *>(sm + L::Q_PART + at) = __float2half_rn(y - __half2float(hi));
-            }
+        for (int b = 0; b < NB; b++) {
+            v[b] = rr < rows ? widen(src[b * 32]) : 0.0f;
+            finite = finite && fabsf(v[b]) < INFINITY;
+            m = fmaxf(m, fabsf(v[b]));
         }
-        kp_fence_smem();
+        m = warp_max(m);
+        finite = __all_sync(0xffffffffu, finite);
+        // |q| * 2^e below 2^14; the sign of the scale goes into the queries, so that a
+        // row's largest product is its largest score
+        const int e = m > 0.0f ? 13 - ilogbf(m) : 0;
+        float f1 = __int_as_float((127 + e / 2) << 23);
+        const float f2 = __int_as_float((127 + e - e / 2) << 23);
+        // (never 0: a hidden score, -inf, must stay -inf)
+        if (lane == 0)
+            sh.rscale[r] = a.scale == 0.0f ? 1.0f : fmaxf(fabsf(a.scale) * KV4_LOG2E / f1 / f2, 1.2e-38f);
+        if (a.scale < 0.0f) f1 = -f1;
+        if (a.scale == 0.0f) f1 = 0.0f;
+        uint8_t *tile = sm + (r / KP_ROWS) * L::Q_TILE;
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            const float y = finite ? v[b] * f1 * f2 : __int_as_float(0x7fffffff);
+            const int d = b * 32 + lane, c = d >> 3, k = d & 7, p = k < 4 ? 2 * k : 2 * k - 7;
+            const uint32_t at = (c >> 3) * (KP_ROWS * 128) + kp_chunk(r & (KP_ROWS - 1), c & 7) + 2 * p;
+            const __half hi = __float2half_rn(y);
+            *reinterpret_cast<__half *>(tile + at) = hi;
+            if (PARTS == 2) *reinterpret_cast<__half *>(tile + L::Q_PART + at) = __float2half_rn(y - __half2float(hi));
+        }
     }
+    kp_fence_smem();
     kp_fence_before();
     __syncthreads();
     kp_fence_after();
     const uint32_t tmem = sh.tmem;
     volatile int *abort = &sh.abort;
 
-    if (warp < 4) {
+    if (warp < L::SOFT) {
         // ---------------------------------------------------------- softmax ----
-        const int r = tid, rr = row_first + r, pos = pos0 + min(rr, rows - 1) / a.group;
-        const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
+        const int rt = warp >> 2, r = tid, rr = row_first + r;
+        const int pos = pos0 + min(rr, rows - 1) / a.group;
+        const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t col_o = mine + L::COL_O + rt * 128;
         const float rs = sh.rscale[r];
-        // positions that every row sees: up to the first row's, from the last row's window on
+        // positions that every row of the tile sees: up to the first row's, from the last
+        // row's window on
+        const int first_pos = pos0 + min(row_first + rt * KP_ROWS, rows - 1) / a.group;
+        const int last_pos = pos0 + (min(rows, row_first + (rt + 1) * KP_ROWS) - 1) / a.group;
         const long long all_from = a.window > 0 ? (long long)last_pos - a.window + 1 : 0;
         float m = -INFINITY, l = 0.0f;
         bool ok = true;
-        for (int j = 0; j < n; j++) {
-            ok = kp_wait(&sh.s_full[j & 1], (j >> 1) & 1, abort);
+        const int todo = rt < tiles ? n : 0;
+        for (int j = 0; j < todo; j++) {
+            ok = kp_wait(&sh.s_full[rt][j & 1], (j >> 1) & 1, abort);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             kp_fence_after();
-            const uint32_t at = mine + (j & 1) * 64;
+            const uint32_t at = mine + rt * 128 + (j & 1) * 64;
             float v[64];
             kp_ld32<0>(v, at);
             kp_ld32<32>(v, at + 32);
@@ -256,36 +273,38 @@ __global__ void __launch_bounds__(KP_THREADS, 2) kv4_prompt_kernel(const Kv4Attn
                     if (!((s1 >> p) & 1)) v[32 + p] = -INFINITY;
                 }
             }
-            float mx = v[0];
+            float mx[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-            for (int p = 1; p < 64; p++) mx = fmaxf(mx, v[p]);
-            mx *= rs;
-            if (__any_sync(0xffffffffu, mx > m + 8.0f)) {
-                const float mn = fmaxf(m, mx);
+            for (int p = 4; p < 64; p += 4)
+#pragma unroll
+                for (int k = 0; k < 4; k++) mx[k] = fmaxf(mx[k], v[p + k]);
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * rs;
+            if (__any_sync(0xffffffffu, top > m + 8.0f)) {
+                const float mn = fmaxf(m, top);
                 const float f = mn == m ? 1.0f : kv4_exp2(m - mn);
                 m = mn;
                 l *= f;
                 if (j > 0) {
-                    ok = kp_wait(&sh.v_empty, (j - 1) & 1, abort);   // the products into O so far
+                    ok = kp_wait(&sh.o_done[rt], (j - 1) & 1, abort);    // the products into O so far
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     kp_fence_after();
 #pragma unroll 1
                     for (int c = 0; c < HD; c += 32) {
                         float o[32];
-                        kp_ld32<0>(o, mine + L::COL_O + c);
+                        kp_ld32<0>(o, col_o + c);
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
                             uint32_t u[16];
 #pragma unroll
                             for (int k = 0; k < 16; k++) u[k] = __float_as_uint(o[16 * h + k] * f);
-                            kp_st16(mine + L::COL_O + c + 16 * h, u);
+                            kp_st16(col_o + c + 16 * h, u);
                         }
                     }
                 }
             }
             const float base = m == -INFINITY ? 0.0f : m - 6.0f;
-            float sum = 0.0f;
+            float sum[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 uint32_t hi[16], lo[16];
@@ -293,7 +312,8 @@ __global__ void __launch_bounds__(KP_THREADS, 2) kv4_prompt_kernel(const Kv4Attn
                 for (int k = 0; k < 16; k++) {
                     const float e0 = kv4_exp2(fmaf(v[h * 32 + 2 * k], rs, -base));
                     const float e1 = kv4_exp2(fmaf(v[h * 32 + 2 * k + 1], rs, -base));
-                    sum += e0 + e1;
+                    sum[0] += e0;
+                    sum[1] += e1;
                     hi[k] = pack_half2(e0, e1);
                     if (PARTS == 2) {
                         const float2 q = __half22float2(bits_h2(hi[k]));
@@ -303,13 +323,16 @@ __global__ void __launch_bounds__(KP_THREADS, 2) kv4_prompt_kernel(const Kv4Attn
                 kp_st16(at + h * 16, hi);
                 if (PARTS == 2) kp_st16(at + 32 + h * 16, lo);
             }
-            l += sum;
+            l += sum[0] + sum[1];
             kp_wait_st();
             kp_fence_before();
-            mbar_arrive(&sh.p_full[j & 1]);
+            mbar_arrive(&sh.p_full[rt][j & 1]);
         }
-        if (n > 0 && ok) {
-            ok = kp_wait(&sh.v_empty, (n - 1) & 1, abort);
+        if (todo > 0 && ok) {
+            // the last two products into O may both be under way: one phase after the other
+            // (a wait for the second alone would take the phase before the first for it)
+            ok = (todo == 1 || kp_wait(&sh.o_done[rt], todo & 1, abort)) &&
+                 kp_wait(&sh.o_done[rt], (todo - 1) & 1, abort);
             ok = __all_sync(0xffffffffu, ok);
             kp_fence_after();
         }
@@ -321,11 +344,12 @@ __global__ void __launch_bounds__(KP_THREADS, 2) kv4_prompt_kernel(const Kv4Attn
 #pragma unroll 1
         for (int c = 0; c < HD; c += 32) {
             float o[32];
-            if (n > 0 && ok) kp_ld32<0>(o, mine + L::COL_O + c);
+            if (todo > 0 && ok) kp_ld32<0>(o, col_o + c);
 #pragma unroll
             for (int k = 0; k < 32; k++) o[k] = !ok ? __int_as_float(0x7fffffff) : l == 0.0f ? 0.0f : o[k] * inv;
-            if (!live) continue;
-            if (vec && sizeof(T) == 4) {
+            // (no lane may run ahead to the next, warp-wide, load)
+            if (!live) {
+            } else if (vec && sizeof(T) == 4) {
 #pragma unroll
                 for (int k = 0; k < 32; k += 4)
                     *reinterpret_cast<float4 *>(out + c + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
@@ -339,159 +363,176 @@ __global__ void __launch_bounds__(KP_THREADS, 2) kv4_prompt_kernel(const Kv4Attn
 #pragma unroll
                 for (int k = 0; k < 32; k++) kv_round(o[k], &out[c + k]);
             }
+            __syncwarp();
         }
         kp_fence_before();
-    } else {
-        // --------------------------------------- keys and values, products ----
-        const bool keys = warp < 6;
-        const int t64 = (tid - 128) & 63, ps = 1 << a.c.page_shift;
+    } else if (warp == L::ISSUE) {
+        // --------------------------------------------------------- products ----
+        if (lane == 0 && n > 0) {
+            constexpr uint32_t kind = 1u << 4 | (uint32_t)(KP_ROWS >> 4) << 24;      // fp16 x fp16 -> fp32, M = 128
+            constexpr uint32_t idesc_s = kind | (uint32_t)(KP_POS >> 3) << 17, idesc_o = kind | (uint32_t)(HD >> 3) << 17;
+            const uint64_t dq = kp_desc(sm32), dk = kp_desc(sm32 + L::OFF_K), dv = kp_desc(sm32 + L::OFF_V);
+            // (offsets inside shared memory are added to a descriptor's address field, in 16 bytes)
+            auto outputs = [&](int j) {
+                bool ok = kp_wait(&sh.v_full[j % BUF], (j / BUF) & 1, abort);
+                const uint64_t v = dv + (uint32_t)(j % BUF) * (L::V_BYTES >> 4);
+                for (int rt = 0; ok && rt < tiles; rt++) {
+                    ok = kp_wait(&sh.p_full[rt][j & 1], (j >> 1) & 1, abort);
+                    if (!ok) break;
+                    kp_fence_after();
+                    const uint32_t p = tmem + rt * 128 + (j & 1) * 64, o = tmem + L::COL_O + rt * 128;
+#pragma unroll
+                    for (int q = 0; q < PARTS; q++)
+#pragma unroll
+                        for (int k = 0; k < KP_POS / 16; k++)
+                            kp_mma_ts(o, p + q * 32 + k * 8, v + k * 2, idesc_o, j > 0 || q + k > 0);
+                    kp_commit(&sh.o_done[rt]);
+                }
+                if (ok) kp_commit(&sh.v_empty[j % BUF]);
+                return ok;
+            };
+            bool ok = true;
+            for (int j = 0; ok && j < n; j++) {
+                ok = kp_wait(&sh.k_full[j % BUF], (j / BUF) & 1, abort);
+                const uint64_t k0 = dk + (uint32_t)(j % BUF) * (L::K_BYTES >> 4);
+                for (int rt = 0; ok && rt < tiles; rt++) {
+                    // the weights that tile j - 2 left where these scores go have been used
+                    if (j > 1) ok = kp_wait(&sh.o_done[rt], j & 1, abort);
+                    if (!ok) break;
+                    kp_fence_after();
+                    const uint32_t d = tmem + rt * 128 + (j & 1) * 64;
+                    const uint64_t q0 = dq + (uint32_t)rt * (L::Q_TILE >> 4);
+#pragma unroll
+                    for (int q = 0; q < PARTS; q++)
+#pragma unroll
+                        for (int k = 0; k < HD / 16; k++)
+                            kp_mma_ss(d, q0 + ((q * L::Q_PART + (k >> 2) * (KP_ROWS * 128) + (k & 3) * 32) >> 4),
+                                      k0 + (((k >> 2) * (KP_POS * 128) + (k & 3) * 32) >> 4), idesc_s, q + k > 0);
+                    kp_commit(&sh.s_full[rt][j & 1]);
+                }
+                if (ok) kp_commit(&sh.k_empty[j % BUF]);
+                if (ok && j > 0) ok = outputs(j - 1);
+            }
+            if (ok) outputs(n - 1);
+            // products in flight end before tensor memory is given back
+            int never = 0;
+            kp_commit(&sh.drain);
+            kp_wait(&sh.drain, 0, &never);
+        }
+    } else if (warp < L::KEYS + L::KEY_WARPS) {
+        // ------------------------------------------------- keys and values ----
+        // A tile's packed words are loaded while the tile before is made operands, and
+        // the numbers of its pages a tile before that. Where there is no page, page 0 is
+        // read: its positions count as hidden, its values' scales as 0.
+        const bool keys = warp >= L::KEYS;
+        const int ps = 1 << a.c.page_shift;
         const int32_t *table = a.b.table + (size_t)seq * a.b.table_stride;
         const uint8_t *base = a.c.data + (size_t)kv * a.c.chunk;
         const uint64_t stride = (uint64_t)a.c.n_kv * a.c.chunk;
-        uint8_t *dst = sm + (keys ? L::OFF_K : L::OFF_V);
-        // page of position p (-1: none), asked for two tiles ahead; its group of 16, or null
         auto page_at = [&](int j, int in_tile) {
             const int p = range.pos(j) + in_tile;
             return j < n && p < len ? __ldg(table + (p >> a.c.page_shift)) : -1;
         };
-        auto group = [&](int page, int p) -> const uint8_t * {
-            if ((unsigned)page >= (unsigned)a.c.n_pages) return nullptr;
-            return base + (uint64_t)(uint32_t)page * stride + ((p & (ps - 1)) >> 4) * GB;
+        auto group = [&](int page, int p) {
+            const bool is = (unsigned)page < (unsigned)a.c.n_pages;
+            return base + (is ? (uint64_t)(uint32_t)page * stride + ((p & (ps - 1)) >> 4) * GB : 0);
         };
-        const bool issuer = tid == 128;
-        constexpr uint32_t kind = 1u << 4 | (uint32_t)(KP_ROWS >> 4) << 24;      // fp16 x fp16 -> fp32, M = 128
-        constexpr uint32_t idesc_s = kind | (uint32_t)(KP_POS >> 3) << 17, idesc_o = kind | (uint32_t)(HD >> 3) << 17;
-        auto scores = [&](int j) {
-            kp_fence_after();
-            const uint32_t d = tmem + (j & 1) * 64;
+        if (keys) {
+            // thread: word column t of the positions first + 8 i + low
+            constexpr int KN = L::KN;
+            const int t = lane >> 3, low = lane & 7, first = (warp - L::KEYS) * (8 * KN);
+            struct Packed {
+                uint32_t w[KN][NB], d[KN][NB < 2 ? 1 : NB / 2];
+                uint64_t ok;              // which of the positions there are
+            };
+            int pg[(KN + 1) / 2];
+            auto pages = [&](int j) {
 #pragma unroll
-            for (int q = 0; q < PARTS; q++)
+                for (int i = 0; i < KN; i += 2) pg[i / 2] = page_at(j, first + 8 * i);
+            };
+            auto load = [&](Packed &u, int j) {
+                const int p0 = range.pos(j);
+                u.ok = 0;
+                if (j >= n) return;
 #pragma unroll
-                for (int k = 0; k < HD / 16; k++)
-                    kp_mma_ss(d, kp_desc(sm32 + q * L::Q_PART + (k >> 2) * (KP_ROWS * 128) + (k & 3) * 32),
-                              kp_desc(sm32 + L::OFF_K + (k >> 2) * (KP_POS * 128) + (k & 3) * 32), idesc_s, q + k > 0);
-            kp_commit(&sh.s_full[j & 1]);
-            kp_commit(&sh.k_empty);
-        };
-        auto outputs = [&](int j) {
-            kp_fence_after();
-            const uint32_t p = tmem + (j & 1) * 64;
-#pragma unroll
-            for (int q = 0; q < PARTS; q++)
-#pragma unroll
-                for (int k = 0; k < KP_POS / 16; k++)
-                    kp_mma_ts(tmem + L::COL_O, p + q * 32 + k * 8, kp_desc(sm32 + L::OFF_V + k * 32), idesc_o,
-                              j > 0 || q + k > 0);
-            kp_commit(&sh.v_empty);
-        };
-        int done = 0;                     // tiles whose products into O were issued
-        bool fine = true;
-        // A tile's packed words are loaded while the tile before is made operands.
-        // keys: word column t of the positions half*32 + 8 i + low; values: words g of the
-        // positions 8 c ..
-        const int t = (t64 >> 3) & 3, half = t64 >> 5, low = t64 & 7, c = t64 & 7, g = t64 >> 3;
-        uint32_t nw[4][NB], nd[4][NB];
-        int pg[2] = {-1, -1};
-        auto pages = [&](int j) {
-            if (keys) {
-                pg[0] = page_at(j, half * 32);
-                pg[1] = page_at(j, half * 32 + 16);
-            } else {
-                pg[0] = page_at(j, (c >> 1) * 16);
-            }
-        };
-        uint32_t nok = 0;                 // keys: which of the four positions there are
-        auto load = [&](int j) {
-            const int p0 = range.pos(j);
-            nok = 0;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-#pragma unroll
-                for (int b = 0; b < NB; b++) nw[i][b] = nd[i][b] = 0;
-            }
-            if (j >= n) return;
-            if (keys) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int p = half * 32 + i * 8 + low, r = p & 15;
-                    const uint8_t *gr = group(pg[i >> 1], p0 + p);
-                    if (!gr) continue;
-                    lds_words<NB>(nw[i], gr + r * (HD / 2) + t * (4 * NB));
-                    uint32_t ks[NB < 2 ? 1 : NB / 2];
-                    lds_words<NB / 2>(ks, gr + 16 * HD + r * (2 * NB));
-#pragma unroll
-                    for (int b = 0; b < (NB < 2 ? 1 : NB / 2); b++) nd[i][b] = ks[b];
-                    if (p0 + p < len) nok |= 1u << (i * 8 + low);
+                for (int i = 0; i < KN; i++) {
+                    const int p = first + i * 8 + low, r = p & 15;
+                    const uint8_t *g = group(pg[i / 2], p0 + p);
+                    lds_words<NB>(u.w[i], g + r * (HD / 2) + t * (4 * NB));
+                    lds_words<NB / 2>(u.d[i], g + 16 * HD + r * (2 * NB));
+                    if (p0 + p < len && (unsigned)pg[i / 2] < (unsigned)a.c.n_pages) u.ok |= 1ull << (i * 8 + low);
                 }
-            } else {
-                const uint8_t *gr = group(pg[0], p0 + (c >> 1) * 16);
-                if (!gr) return;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int pair = (c & 1) * 4 + i;
-                    lds_words<NB>(nw[i], gr + 8 * HD + pair * HD + g * (4 * NB));
-                    lds_words<NB>(nd[i], gr + 16 * HD + 32 * NB + pair * (4 * NB));
+            };
+            auto make = [&](const Packed &u, int j) {
+                // which of the warp's positions there are, for the softmax
+                const uint32_t ok0 = __reduce_or_sync(0xffffffffu, (uint32_t)u.ok);
+                const uint32_t ok1 = KN == 8 ? __reduce_or_sync(0xffffffffu, (uint32_t)(u.ok >> 32)) : 0;
+                if (!__all_sync(0xffffffffu, j < BUF || kp_wait(&sh.k_empty[j % BUF], ((j / BUF) + 1) & 1, abort)))
+                    return false;
+                uint8_t *dst = sm + L::OFF_K + (j % BUF) * L::K_BYTES;
+                if (lane == 0) {
+                    if (KN == 8) sh.valid[j & 3] = (uint64_t)ok1 << 32 | ok0;
+                    else reinterpret_cast<uint16_t *>(&sh.valid[j & 3])[warp - L::KEYS] = (uint16_t)ok0;
                 }
-            }
-        };
-        pages(0);
-        load(0);
-        pages(1);
-        for (int j = 0; j < n; j++) {
-            uint32_t w[4][NB], d[4][NB];
-            const uint32_t ok = nok;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int b = 0; b < NB; b++) { w[i][b] = nw[i][b]; d[i][b] = nd[i][b]; }
-            load(j + 1);
-            pages(j + 2);
-            const int p0 = range.pos(j);
-            if (keys) {
-                // the tile's positions, as a mask (both warps have a half)
-                const uint32_t bits = __reduce_or_sync(0xffffffffu, ok);
-                if (!__all_sync(0xffffffffu, j == 0 || kp_wait(&sh.k_empty, (j - 1) & 1, abort))) break;
-                if (lane == 0) reinterpret_cast<uint32_t *>(&sh.valid[j & 3])[half] = bits;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int p = half * 32 + i * 8 + low;
+                for (int i = 0; i < KN; i++) {
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
-                        const __half2 dd = bits_h2(__byte_perm(d[i][b / 2], 0, (b & 1) ? 0x3232 : 0x1010));
-                        const uint32_t x = w[i][b], y = x >> 8;
+                        const __half2 dd = bits_h2(__byte_perm(u.d[i][b / 2], 0, (b & 1) ? 0x3232 : 0x1010));
+                        const uint32_t x = u.w[i][b], y = x >> 8;
                         const uint4 q = make_uint4(kp_low(x, dd), kp_high(x, dd), kp_low(y, dd), kp_high(y, dd));
-                        *reinterpret_cast<uint4 *>(dst + (b >> 1) * (KP_POS * 128) + kp_chunk(p, 4 * (b & 1) + t)) = q;
+                        *reinterpret_cast<uint4 *>(dst + (b >> 1) * (KP_POS * 128) +
+                                                   kp_chunk(first + i * 8 + low, 4 * (b & 1) + t)) = q;
                     }
                 }
                 kp_fence_smem();
-                mbar_arrive(&sh.k_full);
-                if (issuer && fine) {
-                    fine = kp_wait(&sh.k_full, j & 1, abort);
-                    // the weights that tile j - 2 left where these scores go have been used
-                    if (fine && j > 1) fine = kp_wait(&sh.v_empty, j & 1, abort);
-                    if (fine) scores(j);
-                    if (fine && j > 0) {
-                        fine = kp_wait(&sh.p_full[(j - 1) & 1], ((j - 1) >> 1) & 1, abort) &&
-                               kp_wait(&sh.v_full, (j - 1) & 1, abort);
-                        if (fine) {
-                            outputs(j - 1);
-                            done = j;
-                        }
-                    }
+                mbar_arrive(&sh.k_full[j % BUF]);
+                return true;
+            };
+            Packed ua, ub;
+            pages(0);
+            load(ua, 0);
+            pages(1);
+            for (int j = 0; j < n; j += 2) {
+                load(ub, j + 1);
+                pages(j + 2);
+                if (!make(ua, j)) break;
+                if (j + 1 >= n) break;
+                load(ua, j + 2);
+                pages(j + 3);
+                if (!make(ub, j + 1)) break;
+            }
+        } else {
+            // thread: value words g of the 8 positions 8 c ..
+            const int t64 = tid - 32 * L::VALS, c = t64 & 7, g = t64 >> 3;
+            struct Packed { uint32_t w[4][NB], d[4][NB]; };
+            int pg;
+            auto load = [&](Packed &u, int j) {
+                if (j >= n) return;
+                const int p0 = range.pos(j);
+                const uint8_t *gr = group(pg, p0 + 8 * c);
+                const bool is = (unsigned)pg < (unsigned)a.c.n_pages;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int pair = (c & 1) * 4 + i;
+                    lds_words<NB>(u.w[i], gr + 8 * HD + pair * HD + g * (4 * NB));
+                    lds_words<NB>(u.d[i], gr + 16 * HD + 32 * NB + pair * (4 * NB));
                 }
-                __syncwarp();
-            } else {
                 // positions behind the length may hold any bytes: their scales count as 0
-                if (p0 + KP_POS > len) {
+                if (!is || p0 + KP_POS > len) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const int left = len - (p0 + 8 * c + 2 * i);
+                        const int left = is ? len - (p0 + 8 * c + 2 * i) : 0;
                         const uint32_t keep = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0x0000FFFFu : 0u;
 #pragma unroll
-                        for (int b = 0; b < NB; b++) d[i][b] &= keep;
+                        for (int b = 0; b < NB; b++) u.d[i][b] &= keep;
                     }
                 }
-                if (!__all_sync(0xffffffffu, j == 0 || kp_wait(&sh.v_empty, (j - 1) & 1, abort))) break;
+            };
+            auto make = [&](const Packed &u, int j) {
+                if (!__all_sync(0xffffffffu, j < BUF || kp_wait(&sh.v_empty[j % BUF], ((j / BUF) + 1) & 1, abort)))
+                    return false;
+                uint8_t *dst = sm + L::OFF_V + (j % BUF) * L::V_BYTES;
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
 #pragma unroll
@@ -499,66 +540,72 @@ __global__ void __launch_bounds__(KP_THREADS, 2) kv4_prompt_kernel(const Kv4Attn
                         uint32_t x[4];
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            const uint32_t u = k < 2 ? w[i][b] : w[i][b] >> 8;
-                            x[i] = (k & 1) ? kp_high(u, bits_h2(d[i][b])) : kp_low(u, bits_h2(d[i][b]));
+                            const uint32_t w = k < 2 ? u.w[i][b] : u.w[i][b] >> 8;
+                            x[i] = (k & 1) ? kp_high(w, bits_h2(u.d[i][b])) : kp_low(w, bits_h2(u.d[i][b]));
                         }
                         *reinterpret_cast<uint4 *>(dst + kp_chunk(b * 32 + 4 * g + k, c)) = make_uint4(x[0], x[1], x[2], x[3]);
                     }
                 }
                 kp_fence_smem();
-                mbar_arrive(&sh.v_full);
-            }
-        }
-        if (issuer && n > 0) {
-            fine = fine && kp_wait(&sh.p_full[(n - 1) & 1], ((n - 1) >> 1) & 1, abort) &&
-                   kp_wait(&sh.v_full, (n - 1) & 1, abort);
-            if (fine) {
-                outputs(n - 1);
-                done = n;
-            }
-            // products in flight end before tensor memory is given back
-            int never = 0;
-            if (done > 0) kp_wait(&sh.v_empty, (done - 1) & 1, &never);
-            if (done < n) {               // given up: a last commit covers the scores too
-                kp_commit(&sh.v_empty);
-                kp_wait(&sh.v_empty, done & 1, &never);
+                mbar_arrive(&sh.v_full[j % BUF]);
+                return true;
+            };
+            Packed ua, ub;
+            pg = page_at(0, 8 * c);
+            load(ua, 0);
+            pg = page_at(1, 8 * c);
+            for (int j = 0; j < n; j += 2) {
+                load(ub, j + 1);
+                pg = page_at(j + 2, 8 * c);
+                if (!make(ua, j)) break;
+                if (j + 1 >= n) break;
+                load(ua, j + 2);
+                pg = page_at(j + 3, 8 * c);
+                if (!make(ub, j + 1)) break;
             }
         }
     }
     __syncwarp();
     __syncthreads();
     kp_fence_after();
-    if (warp == 4)
+    if (warp == L::ISSUE)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)L::COLS) : "memory");
 }
 
 // ------------------------------------------------------------------- host ----
 
-template <typename T, int HD>
+template <typename T, int HD, int RT>
 static int kv4_prompt_launch(const Kv4AttnArgs &a, cudaStream_t st) {
-    using L = KpLayout<T, HD>;
+    using L = KpLayout<T, HD, RT>;
     static std::atomic<unsigned long long> ready{0};      // devices whose limit is raised
     int dev = 0;
     CK(cudaGetDevice(&dev));
     if (dev >= 64 || !((ready.load(std::memory_order_acquire) >> dev) & 1)) {
-        CK(cudaFuncSetAttribute(kv4_prompt_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM));
+        CK(cudaFuncSetAttribute(kv4_prompt_kernel<T, HD, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM));
         if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
     }
-    const long long tiles = ((long long)a.max_q * a.group + KP_ROWS - 1) / KP_ROWS;
+    const long long tiles = ((long long)a.max_q * a.group + RT * KP_ROWS - 1) / (RT * KP_ROWS);
     if (tiles > 0x7FFFFFFF) return set_err("kv4 attention: max_q %d is too large", a.max_q);
     const dim3 grid((unsigned)tiles, (unsigned)a.c.n_kv, (unsigned)a.b.n_seqs);
-    kv4_prompt_kernel<T, HD><<<grid, KP_THREADS, L::SMEM, st>>>(a);
+    kv4_prompt_kernel<T, HD, RT><<<grid, 32 * L::WARPS, L::SMEM, st>>>(a);
     CK(cudaGetLastError());
     return 0;
 }
 
+template <typename T, int RT>
+static int kv4_prompt_rt(const Kv4AttnArgs &a, int hd, cudaStream_t st) {
+    switch (hd) {
+    case 32: return kv4_prompt_launch<T, 32, RT>(a, st);
+    case 64: return kv4_prompt_launch<T, 64, RT>(a, st);
+    default: return kv4_prompt_launch<T, 128, RT>(a, st);
+    }
+}
+
 template <typename T>
 static int kv4_prompt_hd(const Kv4AttnArgs &a, int hd, cudaStream_t st) {
-    switch (hd) {
-    case 32: return kv4_prompt_launch<T, 32>(a, st);
-    case 64: return kv4_prompt_launch<T, 64>(a, st);
-    default: return kv4_prompt_launch<T, 128>(a, st);
-    }
+    // two row tiles a CTA once there are CTAs of them for every SM
+    const long long pairs = ((long long)a.max_q * a.group + 2 * KP_ROWS - 1) / (2 * KP_ROWS) * a.c.n_kv * a.b.n_seqs;
+    return pairs >= 148 ? kv4_prompt_rt<T, 2>(a, hd, st) : kv4_prompt_rt<T, 1>(a, hd, st);
 }
 
 }  // namespace emb
