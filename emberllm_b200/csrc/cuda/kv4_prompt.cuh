@@ -92,6 +92,12 @@ EMB_DEV void kp_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool 
                  "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
                  : "memory");
 }
+// one lane of a converged warp
+EMB_DEV bool kp_elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
 EMB_DEV void kp_commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                  : "memory");
@@ -368,55 +374,66 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
         kp_fence_before();
     } else if (warp == L::ISSUE) {
         // --------------------------------------------------------- products ----
-        if (lane == 0 && n > 0) {
+        // the warp stays together and one elected lane issues
+        if (n > 0) {
             constexpr uint32_t kind = 1u << 4 | (uint32_t)(KP_ROWS >> 4) << 24;      // fp16 x fp16 -> fp32, M = 128
             constexpr uint32_t idesc_s = kind | (uint32_t)(KP_POS >> 3) << 17, idesc_o = kind | (uint32_t)(HD >> 3) << 17;
             const uint64_t dq = kp_desc(sm32), dk = kp_desc(sm32 + L::OFF_K), dv = kp_desc(sm32 + L::OFF_V);
+            auto wait = [&](uint64_t *bar, uint32_t parity) {
+                return (bool)__all_sync(0xffffffffu, kp_wait(bar, parity, abort));
+            };
             // (offsets inside shared memory are added to a descriptor's address field, in 16 bytes)
             auto outputs = [&](int j) {
-                bool ok = kp_wait(&sh.v_full[j % BUF], (j / BUF) & 1, abort);
+                bool ok = wait(&sh.v_full[j % BUF], (j / BUF) & 1);
                 const uint64_t v = dv + (uint32_t)(j % BUF) * (L::V_BYTES >> 4);
                 for (int rt = 0; ok && rt < tiles; rt++) {
-                    ok = kp_wait(&sh.p_full[rt][j & 1], (j >> 1) & 1, abort);
+                    ok = wait(&sh.p_full[rt][j & 1], (j >> 1) & 1);
                     if (!ok) break;
                     kp_fence_after();
                     const uint32_t p = tmem + rt * 128 + (j & 1) * 64, o = tmem + L::COL_O + rt * 128;
+                    if (kp_elect()) {
 #pragma unroll
-                    for (int q = 0; q < PARTS; q++)
+                        for (int q = 0; q < PARTS; q++)
 #pragma unroll
-                        for (int k = 0; k < KP_POS / 16; k++)
-                            kp_mma_ts(o, p + q * 32 + k * 8, v + k * 2, idesc_o, j > 0 || q + k > 0);
-                    kp_commit(&sh.o_done[rt]);
+                            for (int k = 0; k < KP_POS / 16; k++)
+                                kp_mma_ts(o, p + q * 32 + k * 8, v + k * 2, idesc_o, j > 0 || q + k > 0);
+                        kp_commit(&sh.o_done[rt]);
+                        if (rt == tiles - 1) kp_commit(&sh.v_empty[j % BUF]);
+                    }
+                    __syncwarp();
                 }
-                if (ok) kp_commit(&sh.v_empty[j % BUF]);
                 return ok;
             };
             bool ok = true;
             for (int j = 0; ok && j < n; j++) {
-                ok = kp_wait(&sh.k_full[j % BUF], (j / BUF) & 1, abort);
+                ok = wait(&sh.k_full[j % BUF], (j / BUF) & 1);
                 const uint64_t k0 = dk + (uint32_t)(j % BUF) * (L::K_BYTES >> 4);
                 for (int rt = 0; ok && rt < tiles; rt++) {
                     // the weights that tile j - 2 left where these scores go have been used
-                    if (j > 1) ok = kp_wait(&sh.o_done[rt], j & 1, abort);
+                    if (j > 1) ok = wait(&sh.o_done[rt], j & 1);
                     if (!ok) break;
                     kp_fence_after();
                     const uint32_t d = tmem + rt * 128 + (j & 1) * 64;
                     const uint64_t q0 = dq + (uint32_t)rt * (L::Q_TILE >> 4);
+                    if (kp_elect()) {
 #pragma unroll
-                    for (int q = 0; q < PARTS; q++)
+                        for (int q = 0; q < PARTS; q++)
 #pragma unroll
-                        for (int k = 0; k < HD / 16; k++)
-                            kp_mma_ss(d, q0 + ((q * L::Q_PART + (k >> 2) * (KP_ROWS * 128) + (k & 3) * 32) >> 4),
-                                      k0 + (((k >> 2) * (KP_POS * 128) + (k & 3) * 32) >> 4), idesc_s, q + k > 0);
-                    kp_commit(&sh.s_full[rt][j & 1]);
+                            for (int k = 0; k < HD / 16; k++)
+                                kp_mma_ss(d, q0 + ((q * L::Q_PART + (k >> 2) * (KP_ROWS * 128) + (k & 3) * 32) >> 4),
+                                          k0 + (((k >> 2) * (KP_POS * 128) + (k & 3) * 32) >> 4), idesc_s, q + k > 0);
+                        kp_commit(&sh.s_full[rt][j & 1]);
+                        if (rt == tiles - 1) kp_commit(&sh.k_empty[j % BUF]);
+                    }
+                    __syncwarp();
                 }
-                if (ok) kp_commit(&sh.k_empty[j % BUF]);
                 if (ok && j > 0) ok = outputs(j - 1);
             }
             if (ok) outputs(n - 1);
             // products in flight end before tensor memory is given back
             int never = 0;
-            kp_commit(&sh.drain);
+            if (kp_elect()) kp_commit(&sh.drain);
+            __syncwarp();
             kp_wait(&sh.drain, 0, &never);
         }
     } else if (warp < L::KEYS + L::KEY_WARPS) {
