@@ -1,16 +1,17 @@
 // kv4_prompt.cuh — attention over the paged 4-bit KV cache, many rows per sequence.
 //
 // The same mathematics as kv4_attn.cuh with tiles of 128 query rows (tokens x the query
-// heads of a kv head) against tiles of 64 positions on tcgen05. A CTA takes RT = 2 row
-// tiles, which share the keys and values it unpacks (one CTA on an SM), or 1 where there
-// are few rows (two CTAs on an SM). Warps have roles:
-//   4 per row tile   softmax: a thread owns a row; it reads the row's 64 scores from
-//        tensor memory, raises the maximum if a score passes it by 2^8 (then O is
-//        rescaled in tensor memory, which is rare), and writes the weights over the scores
-//   1   issues the products: S = Q K^T, two position tiles in turn, O += P V with P from
-//        tensor memory (issuing alone takes some 1,200 cycles a tile; when a warp that
-//        unpacks did it too, that warp was what the others waited for)
-//   2   values, 1 or 4   keys: packed codes from global memory, asked for a tile ahead, to
+// heads of a kv head) on tcgen05. A CTA takes RT = 2 row tiles against tiles of 128
+// positions, both row tiles sharing the keys and values it unpacks (one CTA on an SM);
+// where there are few rows, 1 against tiles of 64 positions (two CTAs on an SM). One
+// row tile's softmax runs under the other's products. Warps have roles:
+//   4 per row tile   softmax: a thread owns a row; it reads the row's scores from tensor
+//        memory, raises the maximum if a score passes it by 2^8 (then O is rescaled in
+//        tensor memory, which is rare), and writes the weights over the scores
+//   1    issues the products: S = Q K^T and O += P V with P from tensor memory. Issuing
+//        was what all others waited for: a product of 64 positions costs this warp some
+//        100 cycles whatever its size, so larger tiles halved their number
+//   2 values, 4 (1) keys   packed codes from global memory, asked for a tile ahead, to
 //        exact fp16 numbers (code - 8) * d in shared memory, swizzled as the products read
 //        them; the values are transposed on the way, so both operands are K-major
 // fp32 queries and weights enter as an fp16 rounding and its rest (two products into
@@ -22,31 +23,36 @@
 
 namespace emb {
 
-constexpr int KP_ROWS = 128, KP_POS = 64;
+constexpr int KP_ROWS = 128;
 constexpr unsigned long long KP_WAIT_NS = 1000000000ull;
 
 template <typename T, int HD, int RT>
 struct KpLayout {
     static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;    // fp16 parts of a query and of a weight
-    static constexpr int BUF = RT == 1 && PARTS == 2 ? 1 : 2;   // tiles of keys and of values held
+    static constexpr int NP = 64 * RT, H = NP / 64;         // positions of a tile, and its halves of 64
+    static constexpr int SB = 3 - RT;                       // tiles of scores per row tile in tensor memory
+    static constexpr int BUF = PARTS == 2 ? 1 : 2;          // tiles of keys and of values in shared memory
     static constexpr int PANELS = (HD + 63) / 64;           // panels of 64 fp16 (128 bytes) of a row
     static constexpr int Q_PART = PANELS * KP_ROWS * 128, Q_TILE = PARTS * Q_PART;
-    static constexpr int K_BYTES = PANELS * KP_POS * 128, V_BYTES = HD * 128;
+    static constexpr int K_PANEL = NP * 128, K_BYTES = PANELS * K_PANEL;
+    static constexpr int V_PANEL = HD * 128, V_BYTES = H * V_PANEL;
     static constexpr int OFF_K = RT * Q_TILE, OFF_V = OFF_K + BUF * K_BYTES;
     static constexpr int SMEM = OFF_V + BUF * V_BYTES + 1024;   // + slack to align the base to 1024
-    // tensor memory: S / P of two position tiles per row tile, then O per row tile
+    // tensor memory: S / P per row tile (SB tiles of NP columns: 128), then O per row tile
     static constexpr int COLS = RT * 256, COL_O = RT * 128;
     static constexpr int SOFT = 4 * RT, ISSUE = SOFT, VALS = SOFT + 1, KEYS = SOFT + 3;   // first warps of the roles
     static constexpr int KEY_WARPS = RT == 2 ? 4 : 1, WARPS = RT == 2 ? 16 : 8;
-    static constexpr int KN = 8 / KEY_WARPS;                // positions a key thread unpacks
+    static constexpr int KN = NP / 8 / KEY_WARPS;           // positions a key thread unpacks
+    static_assert(SB * NP == 128, "scores take 128 columns");
+    static_assert(SMEM <= (RT == 2 ? 227 : 113) * 1024, "shared memory");
 };
 
 template <int RT>
 struct KpShared {
-    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[RT][2], p_full[RT][2], o_done[RT], drain;
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[RT][2], p_full[RT][2], o_done[RT], o_last[RT], drain;
     uint32_t tmem;
     int abort;
-    uint64_t valid[4];          // which positions of a tile there are, by tile number mod 4
+    uint64_t valid[4][RT];      // which positions of a tile there are, by tile number mod 4
     float rscale[RT * KP_ROWS];
 };
 
@@ -132,17 +138,19 @@ EMB_DEV uint32_t kp_high(uint32_t w, __half2 d) {
         __hfma2(bits_h2(and_or(w, 0x00F000F0u, 0x64006400u)), bits_h2(0x2C002C00u), bits_h2(0xD480D480u)), d));
 }
 
-// tiles of KP_POS positions that a row tile sees
+// tiles of NP positions that a CTA's rows see
+template <int NP>
 struct KpRange {
     int sink_tiles, lo, total;
-    __device__ __forceinline__ int pos(int j) const { return (j < sink_tiles ? j : j + (lo - sink_tiles)) * KP_POS; }
+    __device__ __forceinline__ int pos(int j) const { return (j < sink_tiles ? j : j + (lo - sink_tiles)) * NP; }
 };
-EMB_DEV KpRange kp_range(int first_pos, int last_pos, int len, int window, int sinks) {
-    KpRange r;
-    const int stop = max(0, min(len, last_pos + 1)), end = (stop + KP_POS - 1) / KP_POS;
+template <int NP>
+EMB_DEV KpRange<NP> kp_range(int first_pos, int last_pos, int len, int window, int sinks) {
+    KpRange<NP> r;
+    const int stop = max(0, min(len, last_pos + 1)), end = (stop + NP - 1) / NP;
     const long long from = window > 0 ? (long long)first_pos - window + 1 : 0;
-    r.lo = (int)max(0ll, min(from, (long long)stop)) / KP_POS;
-    r.sink_tiles = min((int)(((long long)sinks + KP_POS - 1) / KP_POS), r.lo);
+    r.lo = (int)max(0ll, min(from, (long long)stop)) / NP;
+    r.sink_tiles = min((int)(((long long)sinks + NP - 1) / NP), r.lo);
     r.total = r.sink_tiles + end - r.lo;
     return r;
 }
@@ -150,7 +158,7 @@ EMB_DEV KpRange kp_range(int first_pos, int last_pos, int len, int window, int s
 template <typename T, int HD, int RT>
 __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_prompt_kernel(const Kv4AttnArgs a) {
     using L = KpLayout<T, HD, RT>;
-    constexpr int NB = HD / 32, GB = kv4_group(HD), PARTS = L::PARTS, BUF = L::BUF;
+    constexpr int NB = HD / 32, GB = kv4_group(HD), PARTS = L::PARTS, BUF = L::BUF, NP = L::NP, H = L::H, SB = L::SB;
     extern __shared__ uint8_t kp_raw[];
     __shared__ KpShared<RT> sh;
     const uint32_t raw = smem_u32(kp_raw);
@@ -165,7 +173,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
     if (row_first >= rows) return;
     const int row_end = min(rows, row_first + RT * KP_ROWS);
     const int pos0 = s.len - s.rows, len = min(min(s.len, a.max_kv), a.b.cap);
-    const KpRange range = kp_range(pos0 + row_first / a.group, pos0 + (row_end - 1) / a.group, len, a.window, a.sinks);
+    const KpRange<NP> range = kp_range<NP>(pos0 + row_first / a.group, pos0 + (row_end - 1) / a.group, len, a.window, a.sinks);
     const int n = range.total;
     const int tiles = RT == 1 || row_end - row_first <= KP_ROWS ? 1 : 2;   // row tiles with rows
 
@@ -177,7 +185,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
             mbar_init(&sh.v_empty[i], 1);
             for (int r = 0; r < RT; r++) { mbar_init(&sh.s_full[r][i], 1); mbar_init(&sh.p_full[r][i], KP_ROWS); }
         }
-        for (int r = 0; r < RT; r++) mbar_init(&sh.o_done[r], 1);
+        for (int r = 0; r < RT; r++) { mbar_init(&sh.o_done[r], 1); mbar_init(&sh.o_last[r], 1); }
         mbar_init(&sh.drain, 1);
         fence_mbar_init();
         sh.abort = 0;
@@ -249,17 +257,19 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
         bool ok = true;
         const int todo = rt < tiles ? n : 0;
         for (int j = 0; j < todo; j++) {
-            ok = kp_wait(&sh.s_full[rt][j & 1], (j >> 1) & 1, abort);
+            ok = kp_wait(&sh.s_full[rt][j % SB], (j / SB) & 1, abort);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             kp_fence_after();
-            const uint32_t at = mine + rt * 128 + (j & 1) * 64;
+            const uint32_t at = mine + rt * 128 + (j % SB) * NP;
             float v[64];
-            kp_ld32<0>(v, at);
-            kp_ld32<32>(v, at + 32);
-            const int p0 = range.pos(j);
-            const uint64_t valid = sh.valid[j & 3];
-            if (!(p0 >= all_from && p0 + KP_POS - 1 <= first_pos && valid == ~0ull)) {
+            // a half's scores, the hidden ones -inf
+            auto read = [&](int h) {
+                kp_ld32<0>(v, at + h * 64);
+                kp_ld32<32>(v, at + h * 64 + 32);
+                const int p0 = range.pos(j) + h * 64;
+                const uint64_t valid = sh.valid[j & 3][h];
+                if (p0 >= all_from && p0 + 63 <= first_pos && valid == ~0ull) return;
                 // bit p: the row sees position p0 + p
                 uint64_t see = 0;
                 const int upto = pos - p0;                           // p <= upto
@@ -278,12 +288,14 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
                     if (!((s0 >> p) & 1)) v[p] = -INFINITY;
                     if (!((s1 >> p) & 1)) v[32 + p] = -INFINITY;
                 }
+            };
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int h = 0; h < H; h++) {
+                read(h);
+#pragma unroll
+                for (int p = 0; p < 64; p++) mx[p & 3] = fmaxf(mx[p & 3], v[p]);
             }
-            float mx[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-            for (int p = 4; p < 64; p += 4)
-#pragma unroll
-                for (int k = 0; k < 4; k++) mx[k] = fmaxf(mx[k], v[p + k]);
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * rs;
             if (__any_sync(0xffffffffu, top > m + 8.0f)) {
                 const float mn = fmaxf(m, top);
@@ -311,34 +323,38 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
             }
             const float base = m == -INFINITY ? 0.0f : m - 6.0f;
             float sum[2] = {0.0f, 0.0f};
+            // the last half is still in registers; a half's weights take its scores' place,
+            // first the roundings, then the rests
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                uint32_t hi[16], lo[16];
+            for (int h = H - 1; h >= 0; h--) {
+                if (h < H - 1) read(h);
 #pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    const float e0 = kv4_exp2(fmaf(v[h * 32 + 2 * k], rs, -base));
-                    const float e1 = kv4_exp2(fmaf(v[h * 32 + 2 * k + 1], rs, -base));
-                    sum[0] += e0;
-                    sum[1] += e1;
-                    hi[k] = pack_half2(e0, e1);
-                    if (PARTS == 2) {
-                        const float2 q = __half22float2(bits_h2(hi[k]));
-                        lo[k] = pack_half2(e0 - q.x, e1 - q.y);
+                for (int i = 0; i < 2; i++) {
+                    uint32_t hi[16], lo[16];
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        const float e0 = kv4_exp2(fmaf(v[i * 32 + 2 * k], rs, -base));
+                        const float e1 = kv4_exp2(fmaf(v[i * 32 + 2 * k + 1], rs, -base));
+                        sum[0] += e0;
+                        sum[1] += e1;
+                        hi[k] = pack_half2(e0, e1);
+                        if (PARTS == 2) {
+                            const float2 q = __half22float2(bits_h2(hi[k]));
+                            lo[k] = pack_half2(e0 - q.x, e1 - q.y);
+                        }
                     }
+                    kp_st16(at + h * 64 + i * 16, hi);
+                    if (PARTS == 2) kp_st16(at + h * 64 + 32 + i * 16, lo);
                 }
-                kp_st16(at + h * 16, hi);
-                if (PARTS == 2) kp_st16(at + 32 + h * 16, lo);
             }
             l += sum[0] + sum[1];
             kp_wait_st();
             kp_fence_before();
-            mbar_arrive(&sh.p_full[rt][j & 1]);
+            mbar_arrive(&sh.p_full[rt][j % SB]);
         }
         if (todo > 0 && ok) {
-            // the last two products into O may both be under way: one phase after the other
-            // (a wait for the second alone would take the phase before the first for it)
-            ok = (todo == 1 || kp_wait(&sh.o_done[rt], todo & 1, abort)) &&
-                 kp_wait(&sh.o_done[rt], (todo - 1) & 1, abort);
+            // (a barrier of its own: o_done may be one or two phases behind here)
+            ok = kp_wait(&sh.o_last[rt], 0, abort);
             ok = __all_sync(0xffffffffu, ok);
             kp_fence_after();
         }
@@ -377,59 +393,65 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
         // the warp stays together and one elected lane issues
         if (n > 0) {
             constexpr uint32_t kind = 1u << 4 | (uint32_t)(KP_ROWS >> 4) << 24;      // fp16 x fp16 -> fp32, M = 128
-            constexpr uint32_t idesc_s = kind | (uint32_t)(KP_POS >> 3) << 17, idesc_o = kind | (uint32_t)(HD >> 3) << 17;
+            constexpr uint32_t idesc_s = kind | (uint32_t)(NP >> 3) << 17, idesc_o = kind | (uint32_t)(HD >> 3) << 17;
             const uint64_t dq = kp_desc(sm32), dk = kp_desc(sm32 + L::OFF_K), dv = kp_desc(sm32 + L::OFF_V);
             auto wait = [&](uint64_t *bar, uint32_t parity) {
                 return (bool)__all_sync(0xffffffffu, kp_wait(bar, parity, abort));
             };
             // (offsets inside shared memory are added to a descriptor's address field, in 16 bytes)
-            auto outputs = [&](int j) {
-                bool ok = wait(&sh.v_full[j % BUF], (j / BUF) & 1);
+            auto outputs = [&](int rt, int j) {
+                if (!wait(&sh.v_full[j % BUF], (j / BUF) & 1) || !wait(&sh.p_full[rt][j % SB], (j / SB) & 1)) return false;
+                kp_fence_after();
                 const uint64_t v = dv + (uint32_t)(j % BUF) * (L::V_BYTES >> 4);
-                for (int rt = 0; ok && rt < tiles; rt++) {
-                    ok = wait(&sh.p_full[rt][j & 1], (j >> 1) & 1);
-                    if (!ok) break;
-                    kp_fence_after();
-                    const uint32_t p = tmem + rt * 128 + (j & 1) * 64, o = tmem + L::COL_O + rt * 128;
-                    if (kp_elect()) {
+                const uint32_t p = tmem + rt * 128 + (j % SB) * NP, o = tmem + L::COL_O + rt * 128;
+                if (kp_elect()) {
+#pragma unroll
+                    for (int h = 0; h < H; h++)
 #pragma unroll
                         for (int q = 0; q < PARTS; q++)
 #pragma unroll
-                            for (int k = 0; k < KP_POS / 16; k++)
-                                kp_mma_ts(o, p + q * 32 + k * 8, v + k * 2, idesc_o, j > 0 || q + k > 0);
-                        kp_commit(&sh.o_done[rt]);
-                        if (rt == tiles - 1) kp_commit(&sh.v_empty[j % BUF]);
-                    }
-                    __syncwarp();
+                            for (int k = 0; k < 4; k++)
+                                kp_mma_ts(o, p + h * 64 + q * 32 + k * 8, v + ((h * L::V_PANEL + k * 32) >> 4), idesc_o,
+                                          j > 0 || h + q + k > 0);
+                    kp_commit(&sh.o_done[rt]);
+                    if (rt == tiles - 1) kp_commit(&sh.v_empty[j % BUF]);
+                    if (j == n - 1) kp_commit(&sh.o_last[rt]);
                 }
-                return ok;
+                __syncwarp();
+                return true;
             };
-            bool ok = true;
-            for (int j = 0; ok && j < n; j++) {
-                ok = wait(&sh.k_full[j % BUF], (j / BUF) & 1);
+            auto scores = [&](int rt, int j) {
+                // the weights that tile j - SB left where these scores go have been used
+                if (!wait(&sh.k_full[j % BUF], (j / BUF) & 1) ||
+                    (j >= SB && !wait(&sh.o_done[rt], (j - SB) & 1)))
+                    return false;
+                kp_fence_after();
                 const uint64_t k0 = dk + (uint32_t)(j % BUF) * (L::K_BYTES >> 4);
-                for (int rt = 0; ok && rt < tiles; rt++) {
-                    // the weights that tile j - 2 left where these scores go have been used
-                    if (j > 1) ok = wait(&sh.o_done[rt], j & 1);
-                    if (!ok) break;
-                    kp_fence_after();
-                    const uint32_t d = tmem + rt * 128 + (j & 1) * 64;
-                    const uint64_t q0 = dq + (uint32_t)rt * (L::Q_TILE >> 4);
-                    if (kp_elect()) {
+                const uint32_t d = tmem + rt * 128 + (j % SB) * NP;
+                const uint64_t q0 = dq + (uint32_t)rt * (L::Q_TILE >> 4);
+                if (kp_elect()) {
 #pragma unroll
-                        for (int q = 0; q < PARTS; q++)
+                    for (int q = 0; q < PARTS; q++)
 #pragma unroll
-                            for (int k = 0; k < HD / 16; k++)
-                                kp_mma_ss(d, q0 + ((q * L::Q_PART + (k >> 2) * (KP_ROWS * 128) + (k & 3) * 32) >> 4),
-                                          k0 + (((k >> 2) * (KP_POS * 128) + (k & 3) * 32) >> 4), idesc_s, q + k > 0);
-                        kp_commit(&sh.s_full[rt][j & 1]);
-                        if (rt == tiles - 1) kp_commit(&sh.k_empty[j % BUF]);
-                    }
-                    __syncwarp();
+                        for (int k = 0; k < HD / 16; k++)
+                            kp_mma_ss(d, q0 + ((q * L::Q_PART + (k >> 2) * (KP_ROWS * 128) + (k & 3) * 32) >> 4),
+                                      k0 + (((k >> 2) * L::K_PANEL + (k & 3) * 32) >> 4), idesc_s, q + k > 0);
+                    kp_commit(&sh.s_full[rt][j % SB]);
+                    if (rt == tiles - 1) kp_commit(&sh.k_empty[j % BUF]);
                 }
-                if (ok && j > 0) ok = outputs(j - 1);
-            }
-            if (ok) outputs(n - 1);
+                __syncwarp();
+                return true;
+            };
+            // SB scores ahead; with one tile of scores, a row tile's next scores follow its
+            // own outputs, while the other row tile's softmax runs
+            bool ok = true;
+            for (int j = 0; ok && j < SB && j < n; j++)
+                for (int rt = 0; ok && rt < tiles; rt++) ok = scores(rt, j);
+            for (int j = 0; ok && j < n; j++)
+                for (int rt = 0; ok && rt < tiles; rt++) {
+                    ok = outputs(rt, j);
+                    if (ok && j + SB < n) ok = scores(rt, j + SB);
+                }
             // products in flight end before tensor memory is given back
             int never = 0;
             if (kp_elect()) kp_commit(&sh.drain);
@@ -462,6 +484,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
                 uint32_t w[KN][NB], d[KN][NB < 2 ? 1 : NB / 2];
                 uint64_t ok;              // which of the positions there are
             };
+            static_assert(KN == 8 || KN == 4, "a warp's positions are 32 or 64 bits of the mask");
             int pg[(KN + 1) / 2];
             auto pages = [&](int j) {
 #pragma unroll
@@ -488,8 +511,8 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
                     return false;
                 uint8_t *dst = sm + L::OFF_K + (j % BUF) * L::K_BYTES;
                 if (lane == 0) {
-                    if (KN == 8) sh.valid[j & 3] = (uint64_t)ok1 << 32 | ok0;
-                    else reinterpret_cast<uint16_t *>(&sh.valid[j & 3])[warp - L::KEYS] = (uint16_t)ok0;
+                    if (KN == 8) sh.valid[j & 3][warp - L::KEYS] = (uint64_t)ok1 << 32 | ok0;
+                    else reinterpret_cast<uint32_t *>(sh.valid[j & 3])[warp - L::KEYS] = ok0;
                 }
 #pragma unroll
                 for (int i = 0; i < KN; i++) {
@@ -498,7 +521,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
                         const __half2 dd = bits_h2(__byte_perm(u.d[i][b / 2], 0, (b & 1) ? 0x3232 : 0x1010));
                         const uint32_t x = u.w[i][b], y = x >> 8;
                         const uint4 q = make_uint4(kp_low(x, dd), kp_high(x, dd), kp_low(y, dd), kp_high(y, dd));
-                        *reinterpret_cast<uint4 *>(dst + (b >> 1) * (KP_POS * 128) +
+                        *reinterpret_cast<uint4 *>(dst + (b >> 1) * L::K_PANEL +
                                                    kp_chunk(first + i * 8 + low, 4 * (b & 1) + t)) = q;
                     }
                 }
@@ -520,65 +543,71 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
                 if (!make(ub, j + 1)) break;
             }
         } else {
-            // thread: value words g of the 8 positions 8 c ..
+            // thread: value words g of the 8 positions 8 c .. of a half; item i is half
+            // i % H of tile i / H
             const int t64 = tid - 32 * L::VALS, c = t64 & 7, g = t64 >> 3;
             struct Packed { uint32_t w[4][NB], d[4][NB]; };
             int pg;
-            auto load = [&](Packed &u, int j) {
-                if (j >= n) return;
-                const int p0 = range.pos(j);
+            auto page = [&](int i) { pg = page_at(i / H, (i % H) * 64 + 8 * c); };
+            auto load = [&](Packed &u, int i) {
+                if (i >= n * H) return;
+                const int p0 = range.pos(i / H) + (i % H) * 64;
                 const uint8_t *gr = group(pg, p0 + 8 * c);
                 const bool is = (unsigned)pg < (unsigned)a.c.n_pages;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int pair = (c & 1) * 4 + i;
-                    lds_words<NB>(u.w[i], gr + 8 * HD + pair * HD + g * (4 * NB));
-                    lds_words<NB>(u.d[i], gr + 16 * HD + 32 * NB + pair * (4 * NB));
+                for (int e = 0; e < 4; e++) {
+                    const int pair = (c & 1) * 4 + e;
+                    lds_words<NB>(u.w[e], gr + 8 * HD + pair * HD + g * (4 * NB));
+                    lds_words<NB>(u.d[e], gr + 16 * HD + 32 * NB + pair * (4 * NB));
                 }
                 // positions behind the length may hold any bytes: their scales count as 0
-                if (!is || p0 + KP_POS > len) {
+                if (!is || p0 + 64 > len) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int left = is ? len - (p0 + 8 * c + 2 * i) : 0;
+                    for (int e = 0; e < 4; e++) {
+                        const int left = is ? len - (p0 + 8 * c + 2 * e) : 0;
                         const uint32_t keep = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0x0000FFFFu : 0u;
 #pragma unroll
-                        for (int b = 0; b < NB; b++) u.d[i][b] &= keep;
+                        for (int b = 0; b < NB; b++) u.d[e][b] &= keep;
                     }
                 }
             };
-            auto make = [&](const Packed &u, int j) {
-                if (!__all_sync(0xffffffffu, j < BUF || kp_wait(&sh.v_empty[j % BUF], ((j / BUF) + 1) & 1, abort)))
+            auto make = [&](const Packed &u, int i) {
+                const int j = i / H;
+                if (i % H == 0 &&
+                    !__all_sync(0xffffffffu, j < BUF || kp_wait(&sh.v_empty[j % BUF], ((j / BUF) + 1) & 1, abort)))
                     return false;
-                uint8_t *dst = sm + L::OFF_V + (j % BUF) * L::V_BYTES;
+                uint8_t *dst = sm + L::OFF_V + (j % BUF) * L::V_BYTES + (i % H) * L::V_PANEL;
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
                         uint32_t x[4];
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const uint32_t w = k < 2 ? u.w[i][b] : u.w[i][b] >> 8;
-                            x[i] = (k & 1) ? kp_high(w, bits_h2(u.d[i][b])) : kp_low(w, bits_h2(u.d[i][b]));
+                        for (int e = 0; e < 4; e++) {
+                            const uint32_t w = k < 2 ? u.w[e][b] : u.w[e][b] >> 8;
+                            x[e] = (k & 1) ? kp_high(w, bits_h2(u.d[e][b])) : kp_low(w, bits_h2(u.d[e][b]));
                         }
                         *reinterpret_cast<uint4 *>(dst + kp_chunk(b * 32 + 4 * g + k, c)) = make_uint4(x[0], x[1], x[2], x[3]);
                     }
                 }
-                kp_fence_smem();
-                mbar_arrive(&sh.v_full[j % BUF]);
+                if (i % H == H - 1) {
+                    kp_fence_smem();
+                    mbar_arrive(&sh.v_full[j % BUF]);
+                }
                 return true;
             };
             Packed ua, ub;
-            pg = page_at(0, 8 * c);
+            page(0);
             load(ua, 0);
-            pg = page_at(1, 8 * c);
-            for (int j = 0; j < n; j += 2) {
-                load(ub, j + 1);
-                pg = page_at(j + 2, 8 * c);
-                if (!make(ua, j)) break;
-                if (j + 1 >= n) break;
-                load(ua, j + 2);
-                pg = page_at(j + 3, 8 * c);
-                if (!make(ub, j + 1)) break;
+            page(1);
+            for (int i = 0; i < n * H; i += 2) {
+                load(ub, i + 1);
+                page(i + 2);
+                if (!make(ua, i)) break;
+                if (i + 1 >= n * H) break;
+                load(ua, i + 2);
+                page(i + 3);
+                if (!make(ub, i + 1)) break;
             }
         }
     }
