@@ -8,9 +8,10 @@
 //   4 per row tile   softmax: a thread owns a row; it reads the row's scores from tensor
 //        memory, raises the maximum if a score passes it by 2^8 (then O is rescaled in
 //        tensor memory, which is rare), and writes the weights over the scores
-//   1    issues the products: S = Q K^T and O += P V with P from tensor memory. Issuing
-//        was what all others waited for: a product of 64 positions costs this warp some
-//        100 cycles whatever its size, so larger tiles halved their number
+//   1 per row tile   issues its products: S = Q K^T and O += P V with P from tensor
+//        memory. One warp for both row tiles kept either waiting on the other's softmax,
+//        a warp that unpacks as well was waited for by all (6,900 and more cycles for what
+//        now takes XXXX)
 //   2 values, 4 (1) keys   packed codes from global memory, asked for a tile ahead, to
 //        exact fp16 numbers (code - 8) * d in shared memory, swizzled as the products read
 //        them; the values are transposed on the way, so both operands are K-major
@@ -40,7 +41,7 @@ struct KpLayout {
     static constexpr int SMEM = OFF_V + BUF * V_BYTES + 1024;   // + slack to align the base to 1024
     // tensor memory: S / P per row tile (SB tiles of NP columns: 128), then O per row tile
     static constexpr int COLS = RT * 256, COL_O = RT * 128;
-    static constexpr int SOFT = 4 * RT, ISSUE = SOFT, VALS = SOFT + 1, KEYS = SOFT + 3;   // first warps of the roles
+    static constexpr int SOFT = 4 * RT, ISSUE = SOFT, VALS = SOFT + RT, KEYS = VALS + 2;   // first warps of the roles
     static constexpr int KEY_WARPS = RT == 2 ? 4 : 1, WARPS = RT == 2 ? 16 : 8;
     static constexpr int KN = NP / 8 / KEY_WARPS;           // positions a key thread unpacks
     static_assert(SB * NP == 128, "scores take 128 columns");
@@ -49,7 +50,7 @@ struct KpLayout {
 
 template <int RT>
 struct KpShared {
-    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[RT][2], p_full[RT][2], o_done[RT], o_last[RT], drain;
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[RT][2], p_full[RT][2], o_done[RT], o_last[RT], q_full[RT], drain;
     uint32_t tmem;
     int abort;
     uint64_t valid[4][RT];      // which positions of a tile there are, by tile number mod 4
@@ -165,11 +166,11 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
     uint8_t *sm = kp_raw + ((1024u - (raw & 1023u)) & 1023u);
     const uint32_t sm32 = smem_u32(sm);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int seq = blockIdx.z, kv = blockIdx.y;
+    const int kv = blockIdx.x, seq = blockIdx.y;
     const Kv4Seq s = kv4_seq(a.b, seq);
     const int rows = min(s.rows, a.max_q) * a.group;
-    // the latest rows see the most positions: they go first
-    const int row_first = ((int)gridDim.x - 1 - (int)blockIdx.x) * (RT * KP_ROWS);
+    // the latest rows see the most positions: they go first, of all heads and sequences
+    const int row_first = ((int)gridDim.z - 1 - (int)blockIdx.z) * (RT * KP_ROWS);
     if (row_first >= rows) return;
     const int row_end = min(rows, row_first + RT * KP_ROWS);
     const int pos0 = s.len - s.rows, len = min(min(s.len, a.max_kv), a.b.cap);
@@ -180,13 +181,13 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
             mbar_init(&sh.k_full[i], 32 * L::KEY_WARPS);
-            mbar_init(&sh.k_empty[i], 1);
+            mbar_init(&sh.k_empty[i], tiles);
             mbar_init(&sh.v_full[i], 64);
-            mbar_init(&sh.v_empty[i], 1);
+            mbar_init(&sh.v_empty[i], tiles);
             for (int r = 0; r < RT; r++) { mbar_init(&sh.s_full[r][i], 1); mbar_init(&sh.p_full[r][i], KP_ROWS); }
         }
-        for (int r = 0; r < RT; r++) { mbar_init(&sh.o_done[r], 1); mbar_init(&sh.o_last[r], 1); }
-        mbar_init(&sh.drain, 1);
+        for (int r = 0; r < RT; r++) { mbar_init(&sh.o_done[r], 1); mbar_init(&sh.o_last[r], 1); mbar_init(&sh.q_full[r], KP_ROWS); }
+        mbar_init(&sh.drain, tiles);
         fence_mbar_init();
         sh.abort = 0;
     }
@@ -196,45 +197,6 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // queries: a warp takes 16 rows; within 8 dims the order is 0,4,1,5,2,6,3,7, as the
-    // keys come out of their words
-#pragma unroll 4
-    for (int i = 0; i < 16; i++) {
-        const int r = warp * 16 + i, rr = row_first + r;
-        float v[NB], m = 0.0f;
-        bool finite = true;
-        const int tok = rr / a.group, h = kv * a.group + rr - tok * a.group;
-        const T *src = (const T *)a.q + (int64_t)(s.row0 + tok) * a.q_tok + h * a.q_head + lane;
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            v[b] = rr < rows ? widen(src[b * 32]) : 0.0f;
-            finite = finite && fabsf(v[b]) < INFINITY;
-            m = fmaxf(m, fabsf(v[b]));
-        }
-        m = warp_max(m);
-        finite = __all_sync(0xffffffffu, finite);
-        // |q| * 2^e below 2^14; the sign of the scale goes into the queries, so that a
-        // row's largest product is its largest score
-        const int e = m > 0.0f ? 13 - ilogbf(m) : 0;
-        float f1 = __int_as_float((127 + e / 2) << 23);
-        const float f2 = __int_as_float((127 + e - e / 2) << 23);
-        // (never 0: a hidden score, -inf, must stay -inf)
-        if (lane == 0)
-            sh.rscale[r] = a.scale == 0.0f ? 1.0f : fmaxf(fabsf(a.scale) * KV4_LOG2E / f1 / f2, 1.2e-38f);
-        if (a.scale < 0.0f) f1 = -f1;
-        if (a.scale == 0.0f) f1 = 0.0f;
-        uint8_t *tile = sm + (r / KP_ROWS) * L::Q_TILE;
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            const float y = finite ? v[b] * f1 * f2 : __int_as_float(0x7fffffff);
-            const int d = b * 32 + lane, c = d >> 3, k = d & 7, p = k < 4 ? 2 * k : 2 * k - 7;
-            const uint32_t at = (c >> 3) * (KP_ROWS * 128) + kp_chunk(r & (KP_ROWS - 1), c & 7) + 2 * p;
-            const __half hi = __float2half_rn(y);
-            *reinterpret_cast<__half *>(tile + at) = hi;
-            if (PARTS == 2) *reinterpret_cast<__half *>(tile + L::Q_PART + at) = __float2half_rn(y - __half2float(hi));
-        }
-    }
-    kp_fence_smem();
     kp_fence_before();
     __syncthreads();
     kp_fence_after();
@@ -243,7 +205,57 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
 
     if (warp < L::SOFT) {
         // ---------------------------------------------------------- softmax ----
-        const int rt = warp >> 2, r = tid, rr = row_first + r;
+        const int rt = warp >> 2;
+        // the queries first: a warp takes 32 rows, 8 at a time; within 8 dims the order is
+        // 0,4,1,5,2,6,3,7, as the keys come out of their words
+        for (int i = 0; rt < tiles && i < 32; i += 8) {
+            float v[8][NB];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int rr = row_first + warp * 32 + i + e, tok = rr / a.group, h = kv * a.group + rr - tok * a.group;
+                const T *src = (const T *)a.q + (int64_t)(s.row0 + tok) * a.q_tok + h * a.q_head + lane;
+#pragma unroll
+                for (int b = 0; b < NB; b++) v[e][b] = rr < rows ? widen(src[b * 32]) : 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int r = warp * 32 + i + e;
+                float m = 0.0f;
+                bool finite = true;
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    finite = finite && fabsf(v[e][b]) < INFINITY;
+                    m = fmaxf(m, fabsf(v[e][b]));
+                }
+                m = warp_max(m);
+                finite = __all_sync(0xffffffffu, finite);
+                // |q| * 2^x below 2^14; the sign of the scale goes into the queries, so that
+                // a row's largest product is its largest score
+                const int x = m > 0.0f ? 13 - ilogbf(m) : 0;
+                float f1 = __int_as_float((127 + x / 2) << 23);
+                const float f2 = __int_as_float((127 + x - x / 2) << 23);
+                // (never 0: a hidden score, -inf, must stay -inf)
+                if (lane == 0)
+                    sh.rscale[r] = a.scale == 0.0f ? 1.0f : fmaxf(fabsf(a.scale) * KV4_LOG2E / f1 / f2, 1.2e-38f);
+                if (a.scale < 0.0f) f1 = -f1;
+                if (a.scale == 0.0f) f1 = 0.0f;
+                uint8_t *tile = sm + rt * L::Q_TILE;
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    const float y = finite ? v[e][b] * f1 * f2 : __int_as_float(0x7fffffff);
+                    const int d = b * 32 + lane, c = d >> 3, k = d & 7, p = k < 4 ? 2 * k : 2 * k - 7;
+                    const uint32_t at = (c >> 3) * (KP_ROWS * 128) + kp_chunk(r & (KP_ROWS - 1), c & 7) + 2 * p;
+                    const __half hi = __float2half_rn(y);
+                    *reinterpret_cast<__half *>(tile + at) = hi;
+                    if (PARTS == 2)
+                        *reinterpret_cast<__half *>(tile + L::Q_PART + at) = __float2half_rn(y - __half2float(hi));
+                }
+            }
+        }
+        kp_fence_smem();
+        mbar_arrive(&sh.q_full[rt]);
+        __syncwarp();
+        const int r = tid, rr = row_first + r;
         const int pos = pos0 + min(rr, rows - 1) / a.group;
         const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t col_o = mine + L::COL_O + rt * 128;
@@ -290,7 +302,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
                 }
             };
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
+#pragma unroll 1
             for (int h = 0; h < H; h++) {
                 read(h);
 #pragma unroll
@@ -321,11 +333,19 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
                     }
                 }
             }
+            if (RT == 2 && tiles == 2) {
+                // the row tiles take turns at the exponentials, so that one's run under the
+                // other's products
+                ok = rt == 0 ? j == 0 || kp_wait(&sh.p_full[RT - 1][0], (j - 1) & 1, abort)
+                             : kp_wait(&sh.p_full[0][0], j & 1, abort);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+            }
             const float base = m == -INFINITY ? 0.0f : m - 6.0f;
             float sum[2] = {0.0f, 0.0f};
             // the last half is still in registers; a half's weights take its scores' place,
             // first the roundings, then the rests
-#pragma unroll
+#pragma unroll 1
             for (int h = H - 1; h >= 0; h--) {
                 if (h < H - 1) read(h);
 #pragma unroll
@@ -346,11 +366,11 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
                     kp_st16(at + h * 64 + i * 16, hi);
                     if (PARTS == 2) kp_st16(at + h * 64 + 32 + i * 16, lo);
                 }
+                kp_wait_st();
+                kp_fence_before();
+                mbar_arrive(&sh.p_full[rt][H == 2 ? h : j % SB]);
             }
             l += sum[0] + sum[1];
-            kp_wait_st();
-            kp_fence_before();
-            mbar_arrive(&sh.p_full[rt][j % SB]);
         }
         if (todo > 0 && ok) {
             // (a barrier of its own: o_done may be one or two phases behind here)
@@ -388,10 +408,11 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
             __syncwarp();
         }
         kp_fence_before();
-    } else if (warp == L::ISSUE) {
+    } else if (warp < L::VALS) {
         // --------------------------------------------------------- products ----
         // the warp stays together and one elected lane issues
-        if (n > 0) {
+        const int rt = warp - L::ISSUE;
+        if (n > 0 && rt < tiles) {
             constexpr uint32_t kind = 1u << 4 | (uint32_t)(KP_ROWS >> 4) << 24;      // fp16 x fp16 -> fp32, M = 128
             constexpr uint32_t idesc_s = kind | (uint32_t)(NP >> 3) << 17, idesc_o = kind | (uint32_t)(HD >> 3) << 17;
             const uint64_t dq = kp_desc(sm32), dk = kp_desc(sm32 + L::OFF_K), dv = kp_desc(sm32 + L::OFF_V);
@@ -399,28 +420,32 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
                 return (bool)__all_sync(0xffffffffu, kp_wait(bar, parity, abort));
             };
             // (offsets inside shared memory are added to a descriptor's address field, in 16 bytes)
-            auto outputs = [&](int rt, int j) {
-                if (!wait(&sh.v_full[j % BUF], (j / BUF) & 1) || !wait(&sh.p_full[rt][j % SB], (j / SB) & 1)) return false;
-                kp_fence_after();
+            auto outputs = [&](int j) {
+                if (!wait(&sh.v_full[j % BUF], (j / BUF) & 1)) return false;
                 const uint64_t v = dv + (uint32_t)(j % BUF) * (L::V_BYTES >> 4);
                 const uint32_t p = tmem + rt * 128 + (j % SB) * NP, o = tmem + L::COL_O + rt * 128;
-                if (kp_elect()) {
 #pragma unroll
-                    for (int h = 0; h < H; h++)
+                for (int h = H - 1; h >= 0; h--) {
+                    if (!wait(&sh.p_full[rt][H == 2 ? h : j % SB], (j / SB) & 1)) return false;
+                    kp_fence_after();
+                    if (kp_elect()) {
 #pragma unroll
                         for (int q = 0; q < PARTS; q++)
 #pragma unroll
                             for (int k = 0; k < 4; k++)
                                 kp_mma_ts(o, p + h * 64 + q * 32 + k * 8, v + ((h * L::V_PANEL + k * 32) >> 4), idesc_o,
-                                          j > 0 || h + q + k > 0);
-                    kp_commit(&sh.o_done[rt]);
-                    if (rt == tiles - 1) kp_commit(&sh.v_empty[j % BUF]);
-                    if (j == n - 1) kp_commit(&sh.o_last[rt]);
+                                          j > 0 || h < H - 1 || q + k > 0);
+                        if (h == 0) {
+                            kp_commit(&sh.o_done[rt]);
+                            kp_commit(&sh.v_empty[j % BUF]);
+                            if (j == n - 1) kp_commit(&sh.o_last[rt]);
+                        }
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
                 return true;
             };
-            auto scores = [&](int rt, int j) {
+            auto scores = [&](int j) {
                 // the weights that tile j - SB left where these scores go have been used
                 if (!wait(&sh.k_full[j % BUF], (j / BUF) & 1) ||
                     (j >= SB && !wait(&sh.o_done[rt], (j - SB) & 1)))
@@ -437,21 +462,19 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
                             kp_mma_ss(d, q0 + ((q * L::Q_PART + (k >> 2) * (KP_ROWS * 128) + (k & 3) * 32) >> 4),
                                       k0 + (((k >> 2) * L::K_PANEL + (k & 3) * 32) >> 4), idesc_s, q + k > 0);
                     kp_commit(&sh.s_full[rt][j % SB]);
-                    if (rt == tiles - 1) kp_commit(&sh.k_empty[j % BUF]);
+                    kp_commit(&sh.k_empty[j % BUF]);
                 }
                 __syncwarp();
                 return true;
             };
-            // SB scores ahead; with one tile of scores, a row tile's next scores follow its
-            // own outputs, while the other row tile's softmax runs
-            bool ok = true;
-            for (int j = 0; ok && j < SB && j < n; j++)
-                for (int rt = 0; ok && rt < tiles; rt++) ok = scores(rt, j);
-            for (int j = 0; ok && j < n; j++)
-                for (int rt = 0; ok && rt < tiles; rt++) {
-                    ok = outputs(rt, j);
-                    if (ok && j + SB < n) ok = scores(rt, j + SB);
-                }
+            // SB scores ahead; with one tile of scores, the next follow the outputs, while the
+            // other row tile's softmax runs
+            bool ok = wait(&sh.q_full[rt], 0);
+            for (int j = 0; ok && j < SB && j < n; j++) ok = scores(j);
+            for (int j = 0; ok && j < n; j++) {
+                ok = outputs(j);
+                if (ok && j + SB < n) ok = scores(j + SB);
+            }
             // products in flight end before tensor memory is given back
             int never = 0;
             if (kp_elect()) kp_commit(&sh.drain);
@@ -631,8 +654,8 @@ static int kv4_prompt_launch(const Kv4AttnArgs &a, cudaStream_t st) {
         if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
     }
     const long long tiles = ((long long)a.max_q * a.group + RT * KP_ROWS - 1) / (RT * KP_ROWS);
-    if (tiles > 0x7FFFFFFF) return set_err("kv4 attention: max_q %d is too large", a.max_q);
-    const dim3 grid((unsigned)tiles, (unsigned)a.c.n_kv, (unsigned)a.b.n_seqs);
+    if (tiles > 65535) return set_err("kv4 attention: max_q %d is too large", a.max_q);
+    const dim3 grid((unsigned)a.c.n_kv, (unsigned)a.b.n_seqs, (unsigned)tiles);
     kv4_prompt_kernel<T, HD, RT><<<grid, 32 * L::WARPS, L::SMEM, st>>>(a);
     CK(cudaGetLastError());
     return 0;
