@@ -206,49 +206,89 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
     if (warp < L::SOFT) {
         // ---------------------------------------------------------- softmax ----
         const int rt = warp >> 2;
-        // the queries first: a warp takes 32 rows, 8 at a time; within 8 dims the order is
-        // 0,4,1,5,2,6,3,7, as the keys come out of their words
-        for (int i = 0; rt < tiles && i < 32; i += 8) {
-            float v[8][NB];
+        // The queries first: a warp takes 32 rows, HD / 4 lanes a row with 4 dims each.
+        // Within 8 dims the order is 0,4,1,5,2,6,3,7, as the keys come out of their words:
+        // neighbouring lanes exchange two numbers and store two pairs each.
+        if (rt < tiles) {
+            constexpr int LPR = HD / 4, RPI = 32 / LPR, BATCH = 8;
+            const int sub = lane / LPR, part = lane % LPR;
+            // row `lane` of the warp: where it is (there is none: the tile's first, counted as 0)
+            const int mine_rr = row_first + warp * 32 + lane, my_tok = mine_rr / a.group;
+            const int64_t my_off = mine_rr < rows ? (int64_t)(s.row0 + my_tok) * a.q_tok +
+                                                        (kv * a.group + mine_rr - my_tok * a.group) * a.q_head
+                                                  : (int64_t)s.row0 * a.q_tok + kv * a.group * a.q_head;
+            const int rows_here = rows - row_first - warp * 32;
+            const bool vec = !((uintptr_t)a.q % (4 * sizeof(T)) || a.q_tok % 4 || a.q_head % 4);
+#pragma unroll 1
+            for (int i0 = 0; i0 < 32; i0 += BATCH * RPI) {
+                // all loads first, nothing between them that needs one's data
+                uint32_t raw[BATCH][sizeof(T)];
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int rr = row_first + warp * 32 + i + e, tok = rr / a.group, h = kv * a.group + rr - tok * a.group;
-                const T *src = (const T *)a.q + (int64_t)(s.row0 + tok) * a.q_tok + h * a.q_head + lane;
+                for (int e = 0; e < BATCH; e++) {
+                    const int64_t off = __shfl_sync(0xffffffffu, my_off, (i0 + e * RPI + sub) & 31);
+                    const T *src = (const T *)a.q + off + part * 4;
+                    if (vec) {
+                        lds_words<sizeof(T)>(raw[e], reinterpret_cast<const uint8_t *>(src));
+                    } else if (sizeof(T) == 4) {
 #pragma unroll
-                for (int b = 0; b < NB; b++) v[e][b] = rr < rows ? widen(src[b * 32]) : 0.0f;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int r = warp * 32 + i + e;
-                float m = 0.0f;
-                bool finite = true;
-#pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    finite = finite && fabsf(v[e][b]) < INFINITY;
-                    m = fmaxf(m, fabsf(v[e][b]));
+                        for (int k = 0; k < 4; k++) raw[e][k % sizeof(T)] = __float_as_uint(widen(src[k]));
+                    } else {
+                        const uint16_t *u = reinterpret_cast<const uint16_t *>(src);
+                        raw[e][0] = u[0] | (uint32_t)u[1] << 16;
+                        raw[e][1] = u[2] | (uint32_t)u[3] << 16;
+                    }
                 }
-                m = warp_max(m);
-                finite = __all_sync(0xffffffffu, finite);
-                // |q| * 2^x below 2^14; the sign of the scale goes into the queries, so that
-                // a row's largest product is its largest score
-                const int x = m > 0.0f ? 13 - ilogbf(m) : 0;
-                float f1 = __int_as_float((127 + x / 2) << 23);
-                const float f2 = __int_as_float((127 + x - x / 2) << 23);
-                // (never 0: a hidden score, -inf, must stay -inf)
-                if (lane == 0)
-                    sh.rscale[r] = a.scale == 0.0f ? 1.0f : fmaxf(fabsf(a.scale) * KV4_LOG2E / f1 / f2, 1.2e-38f);
-                if (a.scale < 0.0f) f1 = -f1;
-                if (a.scale == 0.0f) f1 = 0.0f;
-                uint8_t *tile = sm + rt * L::Q_TILE;
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    const float y = finite ? v[e][b] * f1 * f2 : __int_as_float(0x7fffffff);
-                    const int d = b * 32 + lane, c = d >> 3, k = d & 7, p = k < 4 ? 2 * k : 2 * k - 7;
-                    const uint32_t at = (c >> 3) * (KP_ROWS * 128) + kp_chunk(r & (KP_ROWS - 1), c & 7) + 2 * p;
-                    const __half hi = __float2half_rn(y);
-                    *reinterpret_cast<__half *>(tile + at) = hi;
-                    if (PARTS == 2)
-                        *reinterpret_cast<__half *>(tile + L::Q_PART + at) = __float2half_rn(y - __half2float(hi));
+                for (int e = 0; e < BATCH; e++) {
+                    const int i = i0 + e * RPI + sub;
+                    float v[4];
+                    if (sizeof(T) == 4) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) v[k] = __uint_as_float(raw[e][k % sizeof(T)]);
+                    } else {
+                        const float2 lo = __half22float2(bits_h2(raw[e][0])), hi = __half22float2(bits_h2(raw[e][1]));
+                        v[0] = lo.x; v[1] = lo.y; v[2] = hi.x; v[3] = hi.y;
+                    }
+                    if (i >= rows_here) v[0] = v[1] = v[2] = v[3] = 0.0f;
+                    // the row's largest magnitude by its bits: infinities and NaNs are larger
+                    // than any number
+                    uint32_t m = 0;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) m = max(m, __float_as_uint(v[k]) & 0x7FFFFFFFu);
+#pragma unroll
+                    for (int o = LPR / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                    // |q| * 2^x below 2^14; the sign of the scale goes into the queries, so
+                    // that a row's largest product is its largest score
+                    const int x = m == 0 ? 0 : 13 - max((int)(m >> 23) - 127, -126);
+                    float f1 = __int_as_float((127 + x / 2) << 23);
+                    const float f2 = __int_as_float((127 + x - x / 2) << 23);
+                    // (never 0: a hidden score, -inf, must stay -inf)
+                    if (part == 0 && i < 32)
+                        sh.rscale[warp * 32 + i] =
+                            a.scale == 0.0f ? 1.0f : fmaxf(fabsf(a.scale) * KV4_LOG2E / f1 / f2, 1.2e-38f);
+                    if (a.scale < 0.0f) f1 = -f1;
+                    if (a.scale == 0.0f) f1 = 0.0f;
+                    if (m >= 0x7F800000u) f1 = __int_as_float(0x7fffffff);
+                    float y[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) y[k] = v[k] * f1 * f2;
+                    const bool odd = part & 1;
+                    const float r0 = __shfl_xor_sync(0xffffffffu, odd ? y[0] : y[2], 1);
+                    const float r1 = __shfl_xor_sync(0xffffffffu, odd ? y[1] : y[3], 1);
+                    // even lane: dims 0,4 and 1,5; odd lane: 2,6 and 3,7
+                    const float a0 = odd ? r0 : y[0], a1 = odd ? y[2] : r0, b0 = odd ? r1 : y[1], b1 = odd ? y[3] : r1;
+                    const uint32_t h0 = pack_half2(a0, a1), h1 = pack_half2(b0, b1);
+                    const int c = part >> 1;
+                    uint8_t *at = sm + rt * L::Q_TILE + (c >> 3) * (KP_ROWS * 128) +
+                                  kp_chunk(((warp & 3) * 32 + i) & (KP_ROWS - 1), c & 7) + (odd ? 8 : 0);
+                    if (i < 32) {
+                        *reinterpret_cast<uint2 *>(at) = make_uint2(h0, h1);
+                        if (PARTS == 2) {
+                            const float2 g0 = __half22float2(bits_h2(h0)), g1 = __half22float2(bits_h2(h1));
+                            *reinterpret_cast<uint2 *>(at + L::Q_PART) =
+                                make_uint2(pack_half2(a0 - g0.x, a1 - g0.y), pack_half2(b0 - g1.x, b1 - g1.y));
+                        }
+                    }
                 }
             }
         }
