@@ -478,6 +478,19 @@ def test_attention_neighbours_streams_and_graphs(ql):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("heads,kvh,hd", [(12, 12, 64), (40, 2, 128), (16, 8, 128)])
+def test_attention_prompts_again_and_again(dtype, heads, kvh, hd):
+    """many runs give the first one's bits: no wait that sometimes passes early"""
+    p = Paged([1, 130, 64, 300, 257, 5, 0, 129], [1, 130, 1, 100, 64, 2, 0, 129], 16, kvh, hd, seed=hd)
+    p.store_all()
+    q = torch.randn(sum(p.ql), heads, hd, generator=torch.Generator().manual_seed(4)).to(dtype).cuda()
+    first = check(p, q)
+    for _ in range(40):
+        assert torch.equal(p.attend(q), first)
+
+
+@pytest.mark.gpu
 def test_attention_large_offsets():
     """a cache of more than 2^32 bytes: pages behind 4 GiB"""
     page, kvh, hd = 128, 8, 128
