@@ -8,7 +8,7 @@
 // of them ask one question -- where does a running sum (of weights or of ones)
 // reach a target. It is answered without sorting: the distances max - logit are
 // binned, the bins' sums added up, and the bin in which the target lies is binned
-// again (by the bits of the distance, then by index) until its tokens fit a list;
+// again (by the bits of the logit, then by index) until its tokens fit a list;
 // there each token adds up the weights before it. The sums are integers: no order of
 // additions can change a token.
 //
@@ -88,12 +88,23 @@ EMB_DEV double sr_exp2_64(double y, const double *pow2) {
     return __longlong_as_double(__double_as_longlong(q) + ((long long)(k >> 6) << 52));
 }
 
+// Ascending keys are descending logits; -0 counts as +0. Key 0x80000000, that of -0,
+// is no token's.
+constexpr uint32_t SR_LAST_KEY = 0xFF800000u;   // -inf
+EMB_DEV uint32_t sr_key(float v) {
+    const uint32_t u = __float_as_uint(v + 0.0f);
+    return (u >> 31) ? u : 0x7FFFFFFFu - u;
+}
+EMB_DEV float sr_key_logit(uint32_t k) { return __uint_as_float((k >> 31) ? k : 0x7FFFFFFFu - k); }
+
 struct SrRow {
     float mx, limit;                      // distances above limit weigh nothing: w < 2^-45
     double slope;                         // -64 / (temperature * ln 2)
 };
-EMB_DEV double sr_weight(const SrRow &r, float dist, const double *pow2) {
-    return dist > r.limit ? 0.0 : sr_exp2_64((double)dist * r.slope, pow2);
+// The weight comes from the logits in double precision: their difference in fp32 is
+// rounded, which moved weights by 1e-7 and merged neighbouring logits.
+EMB_DEV double sr_weight(const SrRow &r, float l, const double *pow2) {
+    return r.mx - l > r.limit ? 0.0 : sr_exp2_64(((double)r.mx - (double)l) * r.slope, pow2);
 }
 // w is in [0, 1]: adding 2^52 to w * 2^44 leaves the integer in the mantissa
 EMB_DEV u64 sr_units(double w) {
@@ -113,25 +124,25 @@ EMB_DEV void sr_add(u64 *at, u64 v) {
 // order; the last bin holds what is farther than the scale's reach (also inf * 0).
 EMB_DEV int sr_bin(float scale, float d) { return (int)fminf(d * scale, (float)(SR_BINS - 1)); }
 
-// The bits of the smallest distance in bin `at` or a later one, by a whole warp: next
-// to at / scale, as rounding has it; by bisection should it not be there.
-EMB_DEV int sr_bin_start(float scale, int at, int lane) {
-    if (at == 0) return 0;
-    const int guess = max(0, __float_as_int(fminf((float)at / scale, 3.0e38f)) - 16) + lane;
-    const unsigned in = __ballot_sync(~0u, sr_bin(scale, __int_as_float(guess)) >= at);
-    if (in && !(in & 1)) return __shfl_sync(~0u, guess, __ffs(in) - 1);
-    int k0 = 0, k1 = 0x7F800000;          // k1 is in bin `at` or later: infinity is in the last one
+// The smallest key whose distance lies in bin `at` or a later one, by a whole warp:
+// 32 candidates at a time.
+EMB_DEV uint32_t sr_bin_start(float mx, float scale, int at, int lane) {
+    uint32_t k0 = sr_key(mx), k1 = SR_LAST_KEY;     // k0 before it (or it, at = 0); k1 in it or later
+    if (at == 0) return k0;
     while (k1 - k0 > 1) {
-        const int m = k0 + (k1 - k0) / 2;
-        if (sr_bin(scale, __int_as_float(m)) >= at) k1 = m;
-        else k0 = m;
+        const uint32_t step = (k1 - k0 + 32) / 33;
+        const uint32_t k = min((unsigned long long)k1, k0 + (unsigned long long)step * (lane + 1));
+        const unsigned in = __ballot_sync(~0u, sr_bin(scale, mx - sr_key_logit(k)) >= at);
+        const int first = in ? __ffs(in) - 1 : 32;
+        if (first < 32) k1 = __shfl_sync(~0u, k, first);
+        if (first > 0) k0 = __shfl_sync(~0u, k, first - 1);
     }
     return k1;
 }
 
 // where a running sum reaches its target
 struct SrFound {
-    u64 key;                              // (distance bits, index): ascending in the order
+    u64 key;                              // (logit's key, index): ascending in the order
     u64 w;                                // running weight there, inclusive
 };
 
@@ -139,7 +150,7 @@ template <typename T>
 __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleRows a, int slice, bool vec) {
     extern __shared__ __align__(16) uint8_t sr_raw[];
     SrShared &sh = *reinterpret_cast<SrShared *>(sr_raw);
-    float *val = reinterpret_cast<float *>(sr_raw + (sizeof(SrShared) + 15) / 16 * 16);   // distances max - logit
+    float *val = reinterpret_cast<float *>(sr_raw + (sizeof(SrShared) + 15) / 16 * 16);   // the slice's logits
     cg::cluster_group cl = cg::this_cluster();
     const int nc = (int)cl.num_blocks(), rank = (int)cl.block_rank();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.x / nc;
@@ -215,18 +226,16 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
         return;
     }
 
-    // ---- distances ----
-    R.mx = hi;
-    // (an infinite maximum: the other infinite logits are as far as it, 0)
-    auto dist_of = [&](float v) { return v == R.mx ? 0.0f : R.mx - v; };
+    // an infinite maximum: the infinite logits weigh 1, the others nothing, as 0 and -inf do
     const int n4 = n / 4;
     float4 *val4 = reinterpret_cast<float4 *>(val);
-    for (int i = tid; i < n4; i += SR_THREADS) {
-        const float4 v = val4[i];
-        val4[i] = make_float4(dist_of(v.x), dist_of(v.y), dist_of(v.z), dist_of(v.w));
+    if (hi == INFINITY) {
+        for (int i = tid; i < n; i += SR_THREADS) val[i] = val[i] == INFINITY ? 0.0f : -INFINITY;
+        hi = lo = 0.0f;
+        __syncthreads();
     }
-    for (int i = 4 * n4 + tid; i < n; i += SR_THREADS) val[i] = dist_of(val[i]);
-    // f(distance, index) for every token of the slice, four at a time
+    R.mx = hi;
+    // f(logit, index) for every token of the slice, four at a time
     auto each = [&](auto f) {
         for (int i = tid; i < n4; i += SR_THREADS) {
             const float4 v = val4[i];
@@ -238,7 +247,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
         if (nc > 1) cl.sync();
         else __syncthreads();
     };
-    const float far = lo == INFINITY ? 0.0f : dist_of(lo);           // of the finite logits (inf if they overflow)
+    const float far = lo == INFINITY ? 0.0f : R.mx - lo;    // of the finite logits (inf if that overflows)
 
     // ---- bins ----
     auto binning = [&](float to) { return fminf((float)(SR_BINS - 2) / fmaxf(to, 1e-30f), 3.0e38f); };
@@ -311,21 +320,25 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
         clean = false;
         in_min = 0;
         if (need_total) {
-            // every token has its weight, one beyond the limit the 0 units of the limit:
-            // no branch but those that all lanes take alike
-            each([&](float d, int) {
-                const double e = sr_exp2_64((double)fminf(d, R.limit) * R.slope, sh.pow2);
-                const u64 w = sr_units(e);
+            // every token has its weight, one beyond the limit 0: no branch but those that
+            // all lanes take alike
+            const double mx = (double)R.mx;
+            each([&](float l, int) {
+                const float d = R.mx - l;
+                const bool on = d <= R.limit;
+                const double e = sr_exp2_64((mx - (double)(on ? l : R.mx)) * R.slope, sh.pow2);
+                const u64 w = on ? sr_units(e) : 0;
                 const int b = sr_bin(top, d);
                 if (use_min && e >= (double)min_p) in_min += w;
                 if (use_k) atomicAdd(&sh.bin.c[b], 1u);
                 sr_add(&sh.bin.w[b], w);
             });
         } else {
-            each([&](float d, int) {
+            each([&](float l, int) {
+                const float d = R.mx - l;
                 u64 w = 0;
                 if (weights && d <= weigh_to) {
-                    const double e = sr_exp2_64((double)d * R.slope, sh.pow2);
+                    const double e = sr_weight(R, l, sh.pow2);
                     w = sr_units(e);
                     if (use_min && e >= (double)min_p) in_min += w;
                 }
@@ -336,8 +349,8 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
         top_valid = true;
     };
     // the bin in which the running sum, before_* at the first one's start, reaches the
-    // target (the last bin, should it reach it nowhere), and, for level 0, its distances
-    int k_first = 0, k_last = 0x7F800000;
+    // target (the last bin, should it reach it nowhere), and, for level 0, its keys
+    uint32_t k_first = 0, k_last = SR_LAST_KEY;
     auto bin_at = [&](u64 target, bool count, u64 before_w, u64 before_c, bool bounds) {
         if (tid == 0) sh.bin_at = SR_BINS - 1;
         __syncthreads();
@@ -350,26 +363,27 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
         __syncthreads();
         const int at = sh.bin_at;
         if (bounds) {
-            k_first = sr_bin_start(top, at, lane);
-            k_last = at < SR_BINS - 1 ? sr_bin_start(top, at + 1, lane) - 1 : 0x7F800000;
+            k_first = sr_bin_start(R.mx, top, at, lane);
+            k_last = at < SR_BINS - 1 ? sr_bin_start(R.mx, top, at + 1, lane) - 1 : SR_LAST_KEY;
         }
         return at;
     };
-    // tokens with a distance (its bits) in [k0, k1] and an index in [j0, j1] to the
+    // tokens with a key in [k0, k1] and an index in [j0, j1] to the
     // first CTA's list; their number, list_n, may be more than the list holds
     int turn = 0;
-    auto gather = [&](int k0, int k1, int j0, int j1) {
+    auto gather = [&](uint32_t k0, uint32_t k1, int j0, int j1) {
         // (the list's place was last read before a sync that all have passed; so was the
         // other counter, which is made ready for the next time)
         SrShared *first = cl.map_shared_rank(&sh, 0);
         if (rank == 0 && tid == 0) sh.list_n[turn ^ 1] = 0;
-        const float d0 = __int_as_float(k0), d1 = __int_as_float(k1);
-        auto push = [&](float d, int i) {
+        // (as numbers, -0 would let +0 in)
+        const float d1 = sr_key_logit(k0 == 0x80000000u ? 0x80000001u : k0), d0 = sr_key_logit(k1);
+        auto push = [&](float l, int i) {
             if (i < j0 || i > j1) return;
             const int e = atomicAdd(&first->list_n[turn], 1);
             if (e < SR_LIST) {
-                first->list.key[e] = ((u64)__float_as_uint(d) << 32) | (uint32_t)i;
-                first->list.w[e] = sr_units(sr_weight(R, d, sh.pow2));
+                first->list.key[e] = ((u64)sr_key(l) << 32) | (uint32_t)i;
+                first->list.w[e] = sr_units(sr_weight(R, l, sh.pow2));
             }
         };
         for (int i = tid; i < n4; i += SR_THREADS) {
@@ -388,17 +402,16 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
     };
     // in the first CTA: which of the list's tokens takes the running sum to target; all
     // CTAs learn its key and the running weight
-    auto resolve = [&](int tokens, u64 target, bool count, u64 before_w, u64 before_c, int k0, int k1) {
+    auto resolve = [&](int tokens, u64 target, bool count, u64 before_w, u64 before_c, uint32_t k0, uint32_t k1) {
         int m = tokens;
         if (tokens > SR_FEW) {
-            // finer bins, by the bits of the distance or, among equals, by index
+            // finer bins, by key or, among equal keys, by index
             const bool ties = k0 == k1;
-            int j0 = 0, width = k1 - k0;
-            if (ties) width = a.vocab - 1;
+            const uint32_t width = ties ? (uint32_t)a.vocab - 1 : k1 - k0;
             int shift = 0;
             while ((width >> shift) >= SR_SUB) shift++;
             auto sub_of = [&](u64 key) {
-                return (ties ? (int)(uint32_t)key - j0 : (int)(key >> 32) - k0) >> shift;
+                return (int)((ties ? (uint32_t)key : (uint32_t)(key >> 32) - k0) >> shift);
             };
             sh.sub_w[tid] = 0;
             sh.sub_c[tid] = 0;
@@ -458,10 +471,11 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
     // the first place in the order where the running sum reaches target
     auto find = [&](u64 target, bool count) {
         u64 before_w = 0, before_c = 0;
-        // the part of the row that is binned: level 0, all by distance; 1, distances in
-        // [k0, k1] by their bits; 2, one distance, by index. Each level's bin is a
-        // 1/1024 of its range, so there are at most 4 of bits and 2 of indices.
-        int level = 0, shift = 0, k0 = 0, k1 = 0x7F800000, j0 = 0, j1 = 0x7FFFFFFF;
+        // the part of the row that is binned: level 0, all by distance; 1, keys in
+        // [k0, k1]; 2, one key, by index. Each level's bin is a 1/512 of its range at most,
+        // so there are at most 4 of keys and 3 of indices.
+        uint32_t k0 = 0, k1 = SR_LAST_KEY;
+        int level = 0, shift = 0, j0 = 0, j1 = 0x7FFFFFFF;
         for (;;) {
             const int at = bin_at(target, count, before_w, before_c, level == 0);
             before_w += at ? sh.run_w[at - 1] : 0;
@@ -470,8 +484,8 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
                 k0 = k_first;
                 k1 = k_last;
             } else if (level == 1) {
-                k1 = min((long long)k1, k0 + ((at + 1ll) << shift) - 1);
-                k0 += at << shift;
+                k1 = (uint32_t)min((long long)k1, k0 + ((at + 1ll) << shift) - 1);
+                k0 += (uint32_t)at << shift;
             } else {
                 j1 = min((long long)j1, j0 + ((at + 1ll) << shift) - 1);
                 j0 += at << shift;
@@ -485,14 +499,14 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
             }
             if (k0 == k1 && level != 2) { j0 = 0; j1 = a.vocab - 1; }
             level = k0 == k1 ? 2 : 1;
-            const int width = level == 1 ? k1 - k0 : j1 - j0;
+            const uint32_t width = level == 1 ? k1 - k0 : (uint32_t)(j1 - j0);
             shift = 0;
             while ((width >> shift) >= SR_BINS) shift++;
             clear();
-            each([&](float d, int i) {
-                const int k = __float_as_int(d);
+            each([&](float l, int i) {
+                const uint32_t k = sr_key(l);
                 if (k >= k0 && k <= k1 && i >= j0 && i <= j1)
-                    add((level == 1 ? k - k0 : i - j0) >> shift, sr_units(sr_weight(R, d, sh.pow2)));
+                    add((int)((level == 1 ? k - k0 : (uint32_t)(i - j0)) >> shift), sr_units(sr_weight(R, l, sh.pow2)));
             });
             merge();
             top_valid = false;
@@ -512,7 +526,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
             const int tokens = (int)sh.run_c[at];
             if (tokens <= SR_LIST) {
                 // they and the rest of their bin fit the list: the first CTA does the rest
-                gather(0, k_last, 0, 0x7FFFFFFF);
+                gather(sr_key(R.mx), k_last, 0, 0x7FFFFFFF);
                 if (rank != 0) return;
                 constexpr int Q = (SR_LIST + SR_THREADS - 1) / SR_THREADS;
                 u64 mine[Q], sum = 0;
@@ -528,7 +542,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
                         if (sh.list.key[j] < key) { w += sh.list.w[j]; c++; }
                     if (c >= top_k) continue;
                     mine[q] = w;
-                    if (!use_min || sr_weight(R, __uint_as_float((uint32_t)(key >> 32)), sh.pow2) >= (double)min_p)
+                    if (!use_min || sr_weight(R, sr_key_logit((uint32_t)(key >> 32)), sh.pow2) >= (double)min_p)
                         sum += sh.list.w[i];
                 }
 #pragma unroll
@@ -570,7 +584,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
         }
         const SrFound f = find(target, stage == 0 || stage == 2);
         if (stage == 0) {
-            weigh_to = fminf(weigh_to, __uint_as_float((uint32_t)(f.key >> 32)));
+            weigh_to = fminf(weigh_to, R.mx - sr_key_logit((uint32_t)(f.key >> 32)));
             top = binning(weigh_to);
             top_valid = false;
         } else if (stage < 3) {

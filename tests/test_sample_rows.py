@@ -120,6 +120,24 @@ def test_mixed_rows_of_the_large_vocabulary():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(4))
+@pytest.mark.parametrize("scale", [0.3, 2.3])
+def test_full_batches_next_to_borders(seed, scale):
+    """thousands of untruncated draws: a weight that is off by 1e-8 of itself, or two
+    neighbouring logits taken for one, changes one of them"""
+    n, vocab = 256, 151936
+    x = logits(n, vocab, seed, scale=scale)
+    u, t = us(n, seed), np.random.default_rng(seed).uniform(0.5, 1.5, n).astype(np.float32)
+    out = torch.empty(n, dtype=torch.int32, device="cuda")
+    sample_rows(x, out, torch.tensor(u).cuda(), temperature=torch.tensor(t).cuda())
+    l, index = torch.sort(x, dim=-1, descending=True, stable=True)
+    w = torch.exp((l.double() - l[:, :1].double()) / torch.tensor(t).cuda()[:, None].double())
+    run = torch.cumsum(w, -1)
+    at = (run <= torch.tensor(u).cuda()[:, None].double() * run[:, -1:]).sum(-1, keepdim=True)
+    assert torch.equal(out.long(), torch.gather(index, -1, at)[:, 0])
+
+
+@pytest.mark.gpu
 def test_largest_vocabulary():
     draw(logits(2, 393216, 1), us(2), top_p=0.9)
     draw(logits(2, 393216, 1, torch.float16), us(2))
