@@ -13,13 +13,14 @@
 // with a handful of query rows per kv head its 64 rows and more have nothing to do
 // (prompts use it). Asynchronous copies keep a unit ahead in flight per warp without
 // holding registers for it.
-//   scores   A = keys (16 positions x 16 dims): a nibble of a word, masked in
-//            place, IS an fp16 subnormal (code * 2^-24, or code * 2^-20 for the
-//            upper nibbles, whose query elements carry 1/16), so 5 instructions
-//            make 8 operands; B = queries. Sums per 32-block, to which the block's
-//            scale and -8 * (sum of the queries) are applied in fp32.
+//   scores   A = keys (16 positions x 16 dims), the whole numbers code - 8 as fp16: a
+//        nibble or-ed into the mantissa of 1024 (or, in place, its sixteenfold), less 1032
+//        (1/16 of it less 72); B = queries. Sums per 32-block, to which the block's scale
+//        is applied in fp32. (A masked nibble is an fp16 subnormal already, code * 2^-24,
+//        and -8 * (sum of the queries) can be added afterwards: 8 instructions in 28 fewer,
+//        but the larger sums cost the result two bits, 3e-6 instead of 4e-7 of it.)
 //   outputs  A = values (16 dims x 16 positions), made exact fp16 numbers
-//            (code - 8) * d; B = the weights.
+//        (code - 8) * d; B = the weights.
 // Queries and weights take two columns of B each, the fp16 rounding and the
 // rounded rest: 22 bits for the price of idle columns. A query row is first scaled
 // by a power of two so that its largest element is below 2^14.
@@ -79,6 +80,14 @@ EMB_DEV uint32_t and_or(uint32_t v, uint32_t mask, uint32_t magic) {
     uint32_t r;
     asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(magic));
     return r;
+}
+
+// code - 8 of a word's lower (upper) nibbles of each byte 0 and 2, exact
+EMB_DEV uint32_t kd_low(uint32_t w) {
+    return h2bits(__hsub2(bits_h2(and_or(w, 0x000F000Fu, 0x64006400u)), bits_h2(0x64086408u)));
+}
+EMB_DEV uint32_t kd_high(uint32_t w) {
+    return h2bits(__hfma2(bits_h2(and_or(w, 0x00F000F0u, 0x64006400u)), bits_h2(0x2C002C00u), bits_h2(0xD480D480u)));
 }
 
 // W consecutive 32-bit words of shared memory (W = 0: one 16-bit piece)
@@ -161,7 +170,7 @@ __global__ void __launch_bounds__(KD_THREADS, KdLayout<HD, NT>::CTAS) kv4_decode
     float(*part)[R][PS] = reinterpret_cast<float(*)[R][PS]>(ring);      // [warp][row][PS]
     __shared__ __align__(16) uint4 qf[NT][NB][32];
     __shared__ __align__(16) float x[R][HD];  // scaled queries
-    __shared__ float xs8[R][NB], rscale[R];   // -8 * sum of a block's queries and the scores' factor, both in 2^-24
+    __shared__ float rscale[R];               // the scores' factor
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int seq = blockIdx.z, kv = blockIdx.y / a.chunks, chunk_row = (blockIdx.y - kv * a.chunks) * R;
     const KdItem it = kd_item(a, seq);
@@ -251,15 +260,9 @@ __global__ void __launch_bounds__(KD_THREADS, KdLayout<HD, NT>::CTAS) kv4_decode
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 const float y = finite ? qv[i][b] * f1 * f2 : __int_as_float(0x7fffffff);
-                const __half hi = __float2half_rn(y);
-                const __half lo = __float2half_rn(y - __half2float(hi));
-                float sum = __half2float(hi) + __half2float(lo);
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                 x[r][b * 32 + lane] = y;
-                if (lane == 0) xs8[r][b] = sum * (-8.0f / 16777216.0f);
             }
-            if (lane == 0) rscale[r] = a.scale * (16777216.0f * KV4_LOG2E) / f1 / f2;
+            if (lane == 0) rscale[r] = a.scale * KV4_LOG2E / f1 / f2;
         }
         __syncthreads();
         for (int f = warp; f < NT * NB; f += KD_WARPS) {
@@ -269,7 +272,6 @@ __global__ void __launch_bounds__(KD_THREADS, KdLayout<HD, NT>::CTAS) kv4_decode
             float y[8] = {xa.x, xa.y, xa.z, xa.w, xb.x, xb.y, xb.z, xb.w};
 #pragma unroll
             for (int n = 0; n < 8; n++) {
-                y[n] *= (n & 1) ? 0.0625f : 1.0f;
                 const float hi = __half2float(__float2half_rn(y[n]));
                 y[n] = (g & 1) ? y[n] - hi : hi;
             }
@@ -327,17 +329,16 @@ __global__ void __launch_bounds__(KD_THREADS, KdLayout<HD, NT>::CTAS) kv4_decode
             for (int b = 0; b < NB; b++) {
                 const uint32_t w0 = k[0][b], w1 = k[1][b];
                 const uint32_t h0 = w0 >> 8, h1 = w1 >> 8;
+                const uint32_t a0 = kd_low(w0), a1 = kd_low(w1), a2 = kd_high(w0), a3 = kd_high(w1);
+                const uint32_t e0 = kd_low(h0), e1 = kd_low(h1), e2 = kd_high(h0), e3 = kd_high(h1);
                 const float d0 = (b & 1) ? __high2float(bits_h2(ks[0][b / 2])) : __low2float(bits_h2(ks[0][b / 2]));
                 const float d1 = (b & 1) ? __high2float(bits_h2(ks[1][b / 2])) : __low2float(bits_h2(ks[1][b / 2]));
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     const uint4 f = qf[nt][b][lane];
-                    const float e8 = xs8[nt * 4 + t][b];
                     float c[4];
-                    mma_f16(c, w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, f.x, f.y, e8,
-                            0.0f, e8, 0.0f);
-                    mma_f16(c, h0 & 0x000F000Fu, h1 & 0x000F000Fu, h0 & 0x00F000F0u, h1 & 0x00F000F0u, f.z, f.w, c[0],
-                            c[1], c[2], c[3]);
+                    mma_f16(c, a0, a1, a2, a3, f.x, f.y, 0.0f, 0.0f, 0.0f, 0.0f);
+                    mma_f16(c, e0, e1, e2, e3, f.z, f.w, c[0], c[1], c[2], c[3]);
                     sc[nt][2 * h] = fmaf(d0, c[0] + c[1], sc[nt][2 * h]);
                     sc[nt][2 * h + 1] = fmaf(d1, c[2] + c[3], sc[nt][2 * h + 1]);
                 }

@@ -10,8 +10,8 @@
 //        tensor memory, which is rare), and writes the weights over the scores
 //   1 per row tile   issues its products: S = Q K^T and O += P V with P from tensor
 //        memory. One warp for both row tiles kept either waiting on the other's softmax,
-//        a warp that unpacks as well was waited for by all (6,900 and more cycles for what
-//        now takes XXXX)
+//        a warp that unpacks as well was waited for by all (6,900 and more cycles a tile for
+//        what now takes some 4,700)
 //   2 values, 4 (1) keys   packed codes from global memory, asked for a tile ahead, to
 //        exact fp16 numbers (code - 8) * d in shared memory, swizzled as the products read
 //        them; the values are transposed on the way, so both operands are K-major
