@@ -17,7 +17,8 @@
 //        them; the values are transposed on the way, so both operands are K-major
 // fp32 queries and weights enter as an fp16 rounding and its rest (two products into
 // the same sums, 22 bits); fp16 queries are exact as they are, and their weights are
-// rounded to 11 bits, which changes an output by less than its own rounding does.
+// rounded to 11 bits (measured: error 2.6e-4 of the outputs, 2.0e-4 by their own
+// rounding alone; fp32 outputs 1.5e-6, from the long chains of sums on the tensor cores).
 #pragma once
 
 #include "kv4_attn.cuh"
