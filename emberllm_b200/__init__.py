@@ -89,13 +89,21 @@ class Ember:
 class EmberBatch:
     """Independent sequences decoded together on one model (the library's
     ember_batch_* extension): per-stream prompts, then greedy steps of all
-    streams at once. Each stream's tokens equal its own single-sequence run."""
+    streams at once. Each stream's tokens equal its own single-sequence run.
 
-    def __init__(self, ember, n_streams, ctx=0, kv_fp16=False, max_steps=256):
+    ``kv4``: the caches are pages in 4 bits from one pool of ``pages`` (0: enough for
+    every stream's whole context), attended with ``window`` and ``sinks`` (0: all
+    positions); tokens may then differ from those over an exact cache."""
+
+    def __init__(self, ember, n_streams, ctx=0, kv_fp16=False, max_steps=256, kv4=False, pages=0, window=0, sinks=0):
         self.lib = ember.lib
         self.vocab = ember.vocab
         self.n = int(n_streams)
-        self.b = self.lib.ember_batch_new(ember.m, self.n, int(ctx), 1 if kv_fp16 else 0, int(max_steps))
+        if kv4:
+            self.b = self.lib.ember_batch_new_kv4(ember.m, self.n, int(ctx), int(pages), int(window), int(sinks),
+                                                  int(max_steps))
+        else:
+            self.b = self.lib.ember_batch_new(ember.m, self.n, int(ctx), 1 if kv_fp16 else 0, int(max_steps))
 
     def prefill(self, stream, ids):
         """Prompt of one stream; returns the index of its greedy next token."""
@@ -118,6 +126,22 @@ class EmberBatch:
                                     ctypes.cast(lg, ctypes.POINTER(ctypes.c_float)) if logits else None)
         toks_out = [[out[s * self.n + i] for i in range(self.n)] for s in range(n_steps)]
         return (toks_out, lg) if logits else toks_out
+
+    def sample(self, toks, pos, n_steps, samplers, u):
+        """n_steps steps of every stream with drawn tokens: stream i with the settings
+        of ``samplers[i]`` (a Sampler without penalties) and, at step t, the random
+        number ``u[t][i]`` in [0, 1). Returns tokens [n_steps][n]."""
+        t = (ctypes.c_int * self.n)(*[int(x) for x in toks])
+        p = (ctypes.c_int * self.n)(*[int(x) for x in pos])
+        s = (_libmod.EmberSampleParams * self.n)(*[x.params() for x in samplers])
+        r = (ctypes.c_float * (n_steps * self.n))(*[float(x) for row in u for x in row])
+        out = (ctypes.c_int * (n_steps * self.n))()
+        self.lib.ember_batch_sample(self.b, t, p, int(n_steps), s, r, out, None)
+        return [[out[k * self.n + i] for i in range(self.n)] for k in range(n_steps)]
+
+    def release(self, stream):
+        """give a stream's pages back (kv4 batches); its next prompt starts anew"""
+        self.lib.ember_batch_release(self.b, int(stream))
 
     def close(self):
         if getattr(self, "b", None):

@@ -82,6 +82,8 @@ CUDA_SYMBOLS = [
 KV4_SYMBOLS = [
     "ember_cuda_kv4_bytes", "ember_cuda_kv4_store", "ember_cuda_kv4_read", "ember_cuda_kv4_attention_workspace",
     "ember_cuda_kv4_attention", "ember_cuda_sample_rows",
+    "ember_cuda_batch_new_kv4", "ember_cuda_batch_release", "ember_cuda_batch_sample", "ember_batch_new_kv4",
+    "ember_batch_release", "ember_batch_sample",
 ]
 
 _lib = None
@@ -172,6 +174,13 @@ def load(path=None):
     lib.ember_cuda_kv4_attention_workspace.restype = ctypes.c_size_t
     lib.ember_cuda_kv4_attention_workspace.argtypes = [_P] + [ctypes.c_int32] * 4
     lib.ember_cuda_sample_rows.argtypes = [_P, _P]
+    lib.ember_batch_new_kv4.restype = _P
+    lib.ember_batch_new_kv4.argtypes = [_P] + [ctypes.c_int] * 6
+    lib.ember_batch_release.argtypes = [_P, ctypes.c_int]
+    lib.ember_batch_sample.argtypes = [_P, _IP, _IP, ctypes.c_int, ctypes.POINTER(EmberSampleParams), _FP, _IP, _FP]
+    lib.ember_cuda_batch_sample.argtypes = lib.ember_batch_sample.argtypes
+    lib.ember_cuda_batch_greedy.argtypes = [_P, _IP, _IP, ctypes.c_int, _IP, _FP]
+    lib.ember_cuda_batch_prefill.argtypes = [_P, ctypes.c_int, _IP, ctypes.c_int, _FP]
     lib.ember_host_rope_table.argtypes = [_P, ctypes.c_int, ctypes.c_int, ctypes.c_float]
     _lib = lib
     return lib

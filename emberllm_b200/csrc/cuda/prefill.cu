@@ -18,6 +18,7 @@
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 
+#include <math.h>
 #include <stdio.h>
 #include <stdlib.h>
 #include <string.h>
@@ -25,6 +26,7 @@
 #include <mutex>
 #include <vector>
 
+#include "ember_kv4.h"
 #include "ember_ops.h"
 #include "prefill_kernels.cuh"
 #include "runtime_internal.cuh"
@@ -506,7 +508,15 @@ struct PfSeq {
     int dec_attn, dec_chunk;
     size_t dec_smem;
     int *ctl;                        // error word
+    // a paged 4-bit cache instead (kv4.data set: layer 0's, kv4_layer bytes apart)
+    EmberKv4Cache kv4;
+    size_t kv4_layer;
+    EmberKv4Batch kv4_rows;
+    EmberKv4Attention kv4_att;
+    float *kr, *vr, *ao;             // keys, values and attention outputs as plain rows
 };
+
+__global__ void pf_quant_kernel(const PfTokArgs a);
 
 // the attention instantiation for (cache type, register rows, output rows)
 template <typename T, int RS>
@@ -562,10 +572,22 @@ static int pf_layers(EmberCudaModel *m, PfState *ps, const PfSeq &q, const int *
         qa.nh = m->n_heads; qa.nkv = m->n_kv; qa.hd = hd; qa.ctx = q.ctx; qa.kstride = q.kstride;
         qa.neox = m->rope_neox; qa.start = q.start; qa.pos = q.pos; qa.cache_stride = q.cache_stride; qa.eps = m->eps;
         qa.n = nc;
+        qa.kr = q.kr; qa.vr = q.vr;
         const unsigned qgrid = (unsigned)((nc * (m->n_heads + m->n_kv) + PF_QKV_WARPS - 1) / PF_QKV_WARPS);
         if (q.kv_fp16) pf_qkv_post_kernel<__half><<<qgrid, 32 * PF_QKV_WARPS, 0, st>>>(qa);
         else pf_qkv_post_kernel<float><<<qgrid, 32 * PF_QKV_WARPS, 0, st>>>(qa);
         CK(cudaGetLastError());
+        if (q.kv4.data) {
+            EmberKv4Cache c = q.kv4;
+            c.data = (char *)c.data + (size_t)l * q.kv4_layer;
+            const EmberKv4Rows rows = { q.kr, q.vr, EMBER_DT_F32, (int64_t)m->n_kv * hd, hd, (int64_t)m->n_kv * hd, hd };
+            if (ember_cuda_kv4_store(&c, &q.kv4_rows, &rows, st) ||
+                ember_cuda_kv4_attention(&c, &q.kv4_rows, &q.kv4_att, st))
+                return 1;
+            ta.x = q.ao; ta.ld_x = m->n_heads * hd; ta.cols = m->n_heads * hd; ta.k_pad = ps->k_pad[PF_K_QD];
+            pf_quant_kernel<<<nc, 256, (size_t)ta.cols * 4, st>>>(ta);
+            CK(cudaGetLastError());
+        } else {
         PfAttnArgs aa;
         aa.qr = ps->QR; aa.kc = qa.kc; aa.vc = qa.vc; aa.xq = ps->XQ; aa.k_pad = ps->k_pad[PF_K_QD];
         aa.xs = ps->XS; aa.n_pad = ps->n_pad; aa.nh = m->n_heads; aa.nkv = m->n_kv; aa.hd = hd;
@@ -604,6 +626,7 @@ static int pf_layers(EmberCudaModel *m, PfState *ps, const PfSeq &q, const int *
             if (launch_pf_attn(q.kv_fp16 != 0, q.rs, pf_attn_rows_per_group(q.rs, hd), agrid, asmem, st, aa)) return 1;
         }
         CK(cudaGetLastError());
+        }
         if (launch_gemm(P.wo, ps->mapB[PF_K_QD], ps->XQ, ps->XS, ps->n_pad, nc, ps->X, m->dim, true, err, m->n_sm, st))
             return 1;
         // feed-forward block
@@ -775,6 +798,45 @@ __global__ void batch_advance_kernel(int *nout) {
     if (threadIdx.x == 0) *nout += 1;
 }
 
+// a drawn step: this step's random numbers, and after the draw each stream's next
+// token and position; out[step][S]
+__global__ void batch_u_kernel(const float *u, const int *nout, float *now, int S) {
+    const int s = blockIdx.x * blockDim.x + threadIdx.x;
+    if (s < S) now[s] = u[(size_t)(*nout) * S + s];
+}
+__global__ void batch_take_kernel(const int *drawn, int *tok, int *pos, int *out, const int *nout, int S) {
+    const int s = blockIdx.x * blockDim.x + threadIdx.x;
+    if (s >= S) return;
+    tok[s] = drawn[s];
+    pos[s] += 1;
+    out[(size_t)(*nout) * S + s] = drawn[s];
+}
+// a step's cache lengths: the token at pos is the last position
+__global__ void batch_len_kernel(const int *pos, int *len, int S) {
+    const int s = blockIdx.x * blockDim.x + threadIdx.x;
+    if (s < S) len[s] = pos[s] + 1;
+}
+
+// The caches of a batch over pages: one pool of pages per layer, shared by the
+// streams; a stream gets its next page when a call needs it and keeps it until it
+// is released. The same page number serves every layer.
+constexpr int KV4_BATCH_PAGE = 64;
+struct Kv4Streams {
+    cudaStream_t st = nullptr;
+    int *ctl = nullptr, *ids = nullptr;
+    float2 *rope = nullptr;
+    EmberKv4Cache cache = {};         // layer 0
+    size_t layer = 0;                 // bytes per layer
+    int width = 0;                    // pages of a stream, at most
+    int32_t *table = nullptr, *len = nullptr, *one = nullptr;   // [S][width]; [S]; a prompt's {0, rows, length}
+    float *kr = nullptr, *vr = nullptr, *ao = nullptr;
+    void *ws = nullptr;
+    size_t ws_bytes = 0;
+    int window = 0, sinks = 0;
+    std::vector<int32_t> h_table, free;
+    std::vector<int> held;
+};
+
 }  // namespace emb
 
 using namespace emb;
@@ -796,6 +858,12 @@ struct EmberCudaBatch {
     // overlap better than a GEMM of a handful of rows)
     std::vector<EmberCudaState *> reps;
     int *htok = nullptr;                  // pinned [S][max_steps] chosen tokens
+    // a batch over a paged 4-bit cache (ember_cuda_batch_new_kv4) has no worker state
+    Kv4Streams *kv4 = nullptr;
+    // drawn steps (ember_cuda_batch_sample)
+    cudaGraphExec_t g_draw = nullptr;
+    float *d_u = nullptr, *d_set = nullptr;   // [max_steps][S] random numbers; [4][S] settings, then this step's u
+    int *d_top_k = nullptr, *d_drawn = nullptr;
 };
 
 // streams up to which a batch keeps one single-stream state per stream (the
@@ -809,10 +877,167 @@ static void batch_release(EmberCudaBatch *b) {
     for (void *p : b->allocs) cudaFree(p);
     b->allocs.clear();
     if (b->worker) ember_cuda_state_free(b->worker);
+    if (b->g_draw) cudaGraphExecDestroy(b->g_draw);
+    if (b->kv4) {
+        if (b->kv4->st) cudaStreamDestroy(b->kv4->st);
+        delete b->kv4;
+    }
     for (EmberCudaState *r : b->reps) ember_cuda_state_free(r);
     b->reps.clear();
     if (b->htok) cudaFreeHost(b->htok);
     b->htok = nullptr;
+}
+
+static cudaStream_t batch_stream(EmberCudaBatch *b) { return b->kv4 ? b->kv4->st : b->worker->stream; }
+static int *batch_ctl(EmberCudaBatch *b) { return b->kv4 ? b->kv4->ctl : b->worker->ctl; }
+
+// final norm + lm_head over the first `rows` rows of the activations
+static int batch_head(EmberCudaBatch *b, int rows, int *err, cudaStream_t st) {
+    EmberCudaModel *m = b->m;
+    PfState *ps = b->ps;
+    PfTokArgs ta;
+    memset(&ta, 0, sizeof(ta));
+    ta.xq = ps->XQ; ta.xs = ps->XS; ta.n_pad = ps->n_pad; ta.ex = m->ex; ta.eps = m->eps;
+    ta.x = ps->X; ta.ld_x = m->dim; ta.norm_w = m->final_norm; ta.cols = m->dim; ta.k_pad = ps->k_pad[PF_K_DIM];
+    pf_norm_quant_kernel<<<rows, 256, (size_t)m->dim * 8, st>>>(ta);
+    CK(cudaGetLastError());
+    return launch_gemm(m->pf->head, ps->mapB[PF_K_DIM], ps->XQ, ps->XS, ps->n_pad, rows, b->logits, b->ld_log, false, err,
+                       m->n_sm, st);
+}
+
+// ---- a batch over a paged 4-bit cache ----
+
+// what every pass over the layers shares (the caller adds which rows they are)
+static void kv4_seq_args(EmberCudaBatch *b, PfSeq &q) {
+    Kv4Streams *k = b->kv4;
+    const int hd = b->m->head_dim, nh = b->m->n_heads;
+    q.rope = k->rope; q.ctx = b->ctx; q.ctl = k->ctl; q.tq = 1;
+    q.kv4 = k->cache; q.kv4_layer = k->layer;
+    q.kr = k->kr; q.vr = k->vr; q.ao = k->ao;
+    q.kv4_rows.table_stride = k->width;
+    EmberKv4Attention &a = q.kv4_att;
+    a.q = b->ps->QR; a.out = k->ao; a.dtype = EMBER_DT_F32; a.n_heads = nh;
+    a.q_tok = a.out_tok = (int64_t)nh * hd;
+    a.q_head = a.out_head = hd;
+    a.scale = 1.0f / sqrtf((float)hd);
+    a.max_kv = b->ctx; a.window = k->window; a.sinks = k->sinks;
+    a.workspace = k->ws; a.workspace_bytes = k->ws_bytes;
+}
+
+// pages for a stream's first `positions` positions, its row of the table on the device
+static int kv4_reserve(EmberCudaBatch *b, int stream, int positions) {
+    Kv4Streams *k = b->kv4;
+    const int need = (positions + KV4_BATCH_PAGE - 1) / KV4_BATCH_PAGE, have = k->held[stream];
+    if (need <= have) return 0;
+    if ((size_t)(need - have) > k->free.size())
+        return set_err("batch: stream %d needs %d more pages, %zu are free", stream, need - have, k->free.size());
+    int32_t *row = k->h_table.data() + (size_t)stream * k->width;
+    for (int i = have; i < need; i++) {
+        row[i] = k->free.back();
+        k->free.pop_back();
+    }
+    k->held[stream] = need;
+    CK(cudaMemcpyAsync(k->table + (size_t)stream * k->width + have, row + have, (size_t)(need - have) * 4,
+                       cudaMemcpyHostToDevice, k->st));
+    return 0;
+}
+
+static int kv4_prefill(EmberCudaBatch *b, int stream, const int *ids, int n, float *host_logits) {
+    EmberCudaModel *m = b->m;
+    Kv4Streams *k = b->kv4;
+    if (kv4_reserve(b, stream, n)) return 1;
+    CK(cudaMemsetAsync(k->ctl + CTL_ERR, 0, 4, k->st));
+    int nc = 0;
+    for (int c0 = 0; c0 < n; c0 += nc) {
+        nc = n - c0 < PF_CHUNK ? n - c0 : PF_CHUNK;
+        const int32_t one[3] = { 0, nc, c0 + nc };
+        // (pageable host memory: the copies have been staged when the calls return)
+        CK(cudaMemcpyAsync(k->one, one, sizeof(one), cudaMemcpyHostToDevice, k->st));
+        CK(cudaMemcpyAsync(k->ids, ids + c0, (size_t)nc * 4, cudaMemcpyHostToDevice, k->st));
+        PfSeq q;
+        memset(&q, 0, sizeof(q));
+        q.n = nc; q.start = c0;
+        kv4_seq_args(b, q);
+        q.kv4_rows.q_start = k->one;
+        q.kv4_rows.kv_len = k->one + 2;
+        q.kv4_rows.block_table = k->table + (size_t)stream * k->width;
+        q.kv4_rows.n_seqs = 1;
+        q.kv4_rows.n_tokens = q.kv4_rows.max_q = nc;
+        if (pf_layers(m, b->ps, q, k->ids, k->ctl + CTL_ERR, k->st)) return 1;
+    }
+    if (nc > 1)
+        CK(cudaMemcpyAsync(b->ps->X, b->ps->X + (size_t)(nc - 1) * m->dim, (size_t)m->dim * 4, cudaMemcpyDeviceToDevice,
+                           k->st));
+    if (batch_head(b, 1, k->ctl + CTL_ERR, k->st)) return 1;
+    int herr = 0;
+    if (host_logits)
+        CK(cudaMemcpyAsync(host_logits, b->logits, (size_t)m->vocab * 4, cudaMemcpyDeviceToHost, k->st));
+    CK(cudaMemcpyAsync(&herr, k->ctl + CTL_ERR, 4, cudaMemcpyDeviceToHost, k->st));
+    CK(cudaStreamSynchronize(k->st));
+    return herr ? set_err("batch: device wait timed out (code %d)", herr) : 0;
+}
+
+extern "C" int ember_cuda_batch_new_kv4(EmberCudaModel *m, int n_streams, int ctx, int n_pages, int window, int sinks,
+                                        const float *rope_cs, int max_steps, EmberCudaBatch **out) {
+    *out = nullptr;
+    CK(cudaSetDevice(m->device));
+    if (n_streams < 1 || n_streams > PF_CHUNK) return set_err("batch: n_streams must be in [1, %d]", PF_CHUNK);
+    if (max_steps < 1) return set_err("batch: max_steps must be positive");
+    if (window < 0 || sinks < 0) return set_err("batch: window and sinks must not be negative");
+    if (!pf_supported(m)) return set_err("batch: the model's layer weights are not all Q8_0 / Q4_0");
+    const int width = (ctx + KV4_BATCH_PAGE - 1) / KV4_BATCH_PAGE;
+    if (n_pages == 0) n_pages = (long long)width * n_streams > 0x7FFFFFFF ? -1 : width * n_streams;
+    const size_t layer = ember_cuda_kv4_bytes(n_pages, KV4_BATCH_PAGE, m->n_kv, m->head_dim);
+    if (!layer)
+        return set_err("batch: a 4-bit cache of %d pages, %d kv heads of %d is not supported", n_pages, m->n_kv, m->head_dim);
+    EmberCudaBatch *b = new EmberCudaBatch();
+    Kv4Streams *k = b->kv4 = new Kv4Streams();
+    b->m = m; b->S = n_streams; b->ctx = ctx; b->max_steps = max_steps;
+    k->width = width; k->window = window; k->sinks = sinks; k->layer = layer;
+    k->h_table.assign((size_t)n_streams * width, -1);
+    k->held.assign(n_streams, 0);
+    for (int i = n_pages - 1; i >= 0; i--) k->free.push_back(i);
+    const int hd = m->head_dim, rows = PF_CHUNK;
+    const size_t n_rope = (size_t)ctx * (hd / 2) * sizeof(float2);
+    int rc = pf_prepare_model(m) || pf_init(m->device) || pf_prepare_head(m) || pf_state_new(m, rows, &b->ps);
+    if (!rc && cudaStreamCreateWithFlags(&k->st, cudaStreamNonBlocking) != cudaSuccess)
+        rc = set_err("batch: stream creation failed");
+    if (!rc) {
+        k->cache.n_pages = n_pages; k->cache.page_size = KV4_BATCH_PAGE;
+        k->cache.n_kv_heads = m->n_kv; k->cache.head_dim = hd;
+        k->ws_bytes = ember_cuda_kv4_attention_workspace(&k->cache, m->n_heads, n_streams, rows, ctx);
+        b->ld_log = m->pf->head.rows_pad;
+        auto get = [&](void **p, size_t n) { return pf_alloc(b->allocs, p, n); };
+        rc = get(&k->cache.data, layer * m->n_layers) || get((void **)&k->rope, n_rope) ||
+             get((void **)&k->ctl, CTL_WORDS * 4) || get((void **)&k->ids, (size_t)rows * 4) ||
+             get((void **)&k->table, k->h_table.size() * 4) || get((void **)&k->len, (size_t)n_streams * 4) ||
+             get((void **)&k->one, 16) || get((void **)&k->kr, (size_t)rows * m->n_kv * hd * 4) ||
+             get((void **)&k->vr, (size_t)rows * m->n_kv * hd * 4) || get((void **)&k->ao, (size_t)rows * m->n_heads * hd * 4) ||
+             get(&k->ws, k->ws_bytes ? k->ws_bytes : 16) || get((void **)&b->tok, (size_t)n_streams * 4) ||
+             get((void **)&b->pos, (size_t)n_streams * 4) || get((void **)&b->out, (size_t)max_steps * n_streams * 4) ||
+             get((void **)&b->nout, 16) || get((void **)&b->logits, (size_t)n_streams * b->ld_log * 4);
+    }
+    if (!rc && (cudaMemcpy(k->rope, rope_cs, n_rope, cudaMemcpyHostToDevice) != cudaSuccess ||
+                cudaMemset(k->ctl, 0, CTL_WORDS * 4) != cudaSuccess ||
+                cudaMemcpy(k->table, k->h_table.data(), k->h_table.size() * 4, cudaMemcpyHostToDevice) != cudaSuccess))
+        rc = set_err("batch: cache initialisation failed");
+    if (rc) {
+        batch_release(b);
+        delete b;
+        return 1;
+    }
+    *out = b;
+    return 0;
+}
+
+extern "C" int ember_cuda_batch_release(EmberCudaBatch *b, int stream) {
+    if (!b->kv4) return set_err("batch: only a batch over a 4-bit cache has pages to give back");
+    if (stream < 0 || stream >= b->S) return set_err("batch: stream %d out of range", stream);
+    Kv4Streams *k = b->kv4;
+    const int32_t *row = k->h_table.data() + (size_t)stream * k->width;
+    for (int i = k->held[stream] - 1; i >= 0; i--) k->free.push_back(row[i]);
+    k->held[stream] = 0;
+    return 0;
 }
 
 extern "C" int ember_cuda_batch_new(EmberCudaModel *m, int n_streams, int ctx, int kv_fp16, const float *rope_cs,
@@ -885,13 +1110,14 @@ extern "C" void ember_cuda_batch_free(EmberCudaBatch *b) {
     if (!b) return;
     cudaSetDevice(b->m->device);
     if (b->worker) cudaStreamSynchronize(b->worker->stream);
+    if (b->kv4 && b->kv4->st) cudaStreamSynchronize(b->kv4->st);
     for (EmberCudaState *r : b->reps) cudaStreamSynchronize(r->stream);
     batch_release(b);
     delete b;
 }
 
 extern "C" void *ember_cuda_batch_stream(EmberCudaBatch *b) {
-    return (void *)(b->worker ? b->worker->stream : b->reps[0]->stream);
+    return (void *)(b->kv4 ? b->kv4->st : b->worker ? b->worker->stream : b->reps[0]->stream);
 }
 
 // the worker state's cache pointers aimed at stream i's cache
@@ -906,6 +1132,7 @@ extern "C" int ember_cuda_batch_prefill(EmberCudaBatch *b, int stream, const int
     if (stream < 0 || stream >= b->S) return set_err("batch: stream %d out of range", stream);
     if (n < 1 || n > b->ctx) return set_err("batch: prompt of %d tokens does not fit the context", n);
     if (!b->reps.empty()) return ember_cuda_prefill(b->reps[stream], ids, n, 0, host_logits);
+    if (b->kv4) return kv4_prefill(b, stream, ids, n, host_logits);
     EmberCudaState *w = b->worker;
     aim_worker(b, stream);
     // the batched prefill (also for one token: the decode graphs of the worker
@@ -913,68 +1140,128 @@ extern "C" int ember_cuda_batch_prefill(EmberCudaBatch *b, int stream, const int
     return ember_cuda_prefill_batched(w, ids, n, 0, host_logits);
 }
 
-// one greedy step of every stream, recorded once into a graph
-static int batch_record(EmberCudaBatch *b) {
+// one step of every stream (greedy, or drawn with the batch's settings), recorded once
+// into a graph
+static int batch_record(EmberCudaBatch *b, bool draw) {
     EmberCudaModel *m = b->m;
     EmberCudaState *w = b->worker;
-    cudaStream_t st = w->stream;
-    int *err = w->ctl + CTL_ERR;
+    cudaStream_t st = batch_stream(b);
+    int *err = batch_ctl(b) + CTL_ERR;
     PfSeq q;
     memset(&q, 0, sizeof(q));
     q.n = b->S; q.start = 0; q.pos = b->pos;
-    q.kc = b->kc; q.vc = b->vc; q.cache_stride = b->stride;
-    q.k_layer = w->k_layer_elems; q.v_layer = w->v_layer_elems;
-    q.ctx = b->ctx; q.kstride = w->kstride; q.kv_fp16 = b->kv_fp16; q.rope = w->rope;
-    q.p_cap = (int)round_up((size_t)b->ctx, 4);
-    q.tq = 1;
-    q.rs = (m->n_heads / m->n_kv + 3) / 4 * 4;
-    // attention per (kv head, stream) (attn_batch_kernel) where the kv head's query
-    // heads fit one CTA, else per (query head, stream) (attn_decode_kernel, BATCH);
-    // EMBER_BATCH_ATTN=head forces the latter, =tile the prefill's token-tile
-    // kernel (for comparisons)
-    const char *ba = getenv("EMBER_BATCH_ATTN");
-    q.dec_attn = !(w->att_in_smem && w->m->head_dim <= ATTN_THREADS) || (ba && strcmp(ba, "tile") == 0)
-                     ? 0
-                     : ((ba && strcmp(ba, "head") == 0) ? 2 : 1);
-    // chunks of 48 positions (fp32, head_dim 128: 48 KB of buffers), so several
-    // (head, stream) CTAs share an SM; EMBER_BATCH_ATTN_CHUNK overrides (tuning)
-    {
-        const size_t es = b->kv_fp16 ? 2 : 4, hd = (size_t)m->head_dim;
-        const char *ce = getenv("EMBER_BATCH_ATTN_CHUNK");
-        int ch = ce && atoi(ce) >= 8 ? atoi(ce) / 8 * 8 : (int)((48 * 1024) / (2 * hd * es)) / 8 * 8;
-        if (ch < 8) ch = 8;
-        if (ch > w->attn_chunk) ch = w->attn_chunk;
-        q.dec_chunk = ch;
-        q.dec_smem = 2 * (size_t)ch * hd * es + ((size_t)b->ctx * 4 + 15) / 16 * 16;
+    if (b->kv4) {
+        Kv4Streams *k = b->kv4;
+        batch_len_kernel<<<(b->S + 255) / 256, 256, 0, st>>>(b->pos, k->len, b->S);
+        CK(cudaGetLastError());
+        kv4_seq_args(b, q);
+        q.kv4_rows.kv_len = k->len;
+        q.kv4_rows.block_table = k->table;
+        q.kv4_rows.n_seqs = q.kv4_rows.n_tokens = b->S;
+        q.kv4_rows.max_q = 1;
+    } else {
+        q.kc = b->kc; q.vc = b->vc; q.cache_stride = b->stride;
+        q.k_layer = w->k_layer_elems; q.v_layer = w->v_layer_elems;
+        q.ctx = b->ctx; q.kstride = w->kstride; q.kv_fp16 = b->kv_fp16; q.rope = w->rope;
+        q.p_cap = (int)round_up((size_t)b->ctx, 4);
+        q.tq = 1;
+        q.rs = (m->n_heads / m->n_kv + 3) / 4 * 4;
+        // attention per (kv head, stream) (attn_batch_kernel) where the kv head's query
+        // heads fit one CTA, else per (query head, stream) (attn_decode_kernel, BATCH);
+        // EMBER_BATCH_ATTN=head forces the latter, =tile the prefill's token-tile
+        // kernel (for comparisons)
+        const char *ba = getenv("EMBER_BATCH_ATTN");
+        q.dec_attn = !(w->att_in_smem && w->m->head_dim <= ATTN_THREADS) || (ba && strcmp(ba, "tile") == 0)
+                         ? 0
+                         : ((ba && strcmp(ba, "head") == 0) ? 2 : 1);
+        // chunks of 48 positions (fp32, head_dim 128: 48 KB of buffers), so several
+        // (head, stream) CTAs share an SM; EMBER_BATCH_ATTN_CHUNK overrides (tuning)
+        {
+            const size_t es = b->kv_fp16 ? 2 : 4, hd = (size_t)m->head_dim;
+            const char *ce = getenv("EMBER_BATCH_ATTN_CHUNK");
+            int ch = ce && atoi(ce) >= 8 ? atoi(ce) / 8 * 8 : (int)((48 * 1024) / (2 * hd * es)) / 8 * 8;
+            if (ch < 8) ch = 8;
+            if (ch > w->attn_chunk) ch = w->attn_chunk;
+            q.dec_chunk = ch;
+            q.dec_smem = 2 * (size_t)ch * hd * es + ((size_t)b->ctx * 4 + 15) / 16 * 16;
+        }
+        q.ctl = w->ctl;
     }
-    q.ctl = w->ctl;
-    if (pf_layers(m, b->ps, q, b->tok, err, st)) return 1;
-    // final norm + lm_head over the S rows, then each stream's argmax
-    PfState *ps = b->ps;
-    PfTokArgs ta;
-    memset(&ta, 0, sizeof(ta));
-    ta.xq = ps->XQ; ta.xs = ps->XS; ta.n_pad = ps->n_pad; ta.ex = m->ex; ta.eps = m->eps;
-    ta.x = ps->X; ta.ld_x = m->dim; ta.norm_w = m->final_norm; ta.cols = m->dim; ta.k_pad = ps->k_pad[PF_K_DIM];
-    pf_norm_quant_kernel<<<b->S, 256, (size_t)m->dim * 8, st>>>(ta);
-    CK(cudaGetLastError());
-    if (launch_gemm(m->pf->head, ps->mapB[PF_K_DIM], ps->XQ, ps->XS, ps->n_pad, b->S, b->logits, b->ld_log, false, err,
-                    m->n_sm, st))
-        return 1;
-    batch_argmax_kernel<<<b->S, 256, 0, st>>>(b->logits, b->ld_log, m->vocab, b->tok, b->pos, b->out, b->nout, b->S);
+    if (pf_layers(m, b->ps, q, b->tok, err, st) || batch_head(b, b->S, err, st)) return 1;
+    if (draw) {
+        const int grid = (b->S + 255) / 256;
+        float *now = b->d_set + 3 * (size_t)b->S;
+        batch_u_kernel<<<grid, 256, 0, st>>>(b->d_u, b->nout, now, b->S);
+        CK(cudaGetLastError());
+        EmberSampleRows r;
+        memset(&r, 0, sizeof(r));
+        r.logits = b->logits; r.dtype = EMBER_DT_F32; r.n_rows = b->S; r.vocab = m->vocab; r.stride = b->ld_log;
+        r.temperature = b->d_set; r.top_p = b->d_set + b->S; r.min_p = b->d_set + 2 * (size_t)b->S; r.u = now;
+        r.top_k = b->d_top_k; r.out = b->d_drawn;
+        if (ember_cuda_sample_rows(&r, st)) return 1;
+        batch_take_kernel<<<grid, 256, 0, st>>>(b->d_drawn, b->tok, b->pos, b->out, b->nout, b->S);
+    } else {
+        batch_argmax_kernel<<<b->S, 256, 0, st>>>(b->logits, b->ld_log, m->vocab, b->tok, b->pos, b->out, b->nout, b->S);
+    }
     CK(cudaGetLastError());
     batch_advance_kernel<<<1, 32, 0, st>>>(b->nout);
     CK(cudaGetLastError());
     return 0;
 }
 
-extern "C" int ember_cuda_batch_greedy(EmberCudaBatch *b, const int *toks, const int *pos, int n_steps,
-                                       int *host_tokens, float *host_logits) {
-    CK(cudaSetDevice(b->m->device));
+// n_steps recorded steps from toks / pos; the results to the host
+static int batch_run(EmberCudaBatch *b, bool draw, const int *toks, const int *pos, int n_steps, int *host_tokens,
+                     float *host_logits) {
+    cudaStream_t st = batch_stream(b);
+    int *ctl = batch_ctl(b);
+    if (b->kv4)
+        for (int i = 0; i < b->S; i++)
+            if (kv4_reserve(b, i, pos[i] + n_steps)) return 1;
+    cudaGraphExec_t &exec = draw ? b->g_draw : b->g_step;
+    if (!exec) {
+        cudaGraph_t g = nullptr;
+        CK(cudaStreamBeginCapture(st, cudaStreamCaptureModeThreadLocal));
+        int rc = batch_record(b, draw);
+        cudaError_t e = cudaStreamEndCapture(st, &g);
+        if (rc) {
+            if (g) cudaGraphDestroy(g);
+            return 1;
+        }
+        if (e != cudaSuccess) return set_err("batch graph capture failed: %s", cudaGetErrorString(e));
+        e = cudaGraphInstantiate(&exec, g, 0);
+        cudaGraphDestroy(g);
+        if (e != cudaSuccess) return set_err("batch graph instantiate failed: %s", cudaGetErrorString(e));
+    }
+    CK(cudaMemcpyAsync(b->tok, toks, (size_t)b->S * 4, cudaMemcpyHostToDevice, st));
+    CK(cudaMemcpyAsync(b->pos, pos, (size_t)b->S * 4, cudaMemcpyHostToDevice, st));
+    CK(cudaMemsetAsync(b->nout, 0, 4, st));
+    CK(cudaMemsetAsync(ctl + CTL_ERR, 0, 4, st));
+    for (int i = 0; i < n_steps; i++) CK(cudaGraphLaunch(exec, st));
+    if (host_tokens)
+        CK(cudaMemcpyAsync(host_tokens, b->out, (size_t)n_steps * b->S * 4, cudaMemcpyDeviceToHost, st));
+    if (host_logits)
+        CK(cudaMemcpy2DAsync(host_logits, (size_t)b->m->vocab * 4, b->logits, (size_t)b->ld_log * 4,
+                             (size_t)b->m->vocab * 4, (size_t)b->S, cudaMemcpyDeviceToHost, st));
+    int herr = 0;
+    CK(cudaMemcpyAsync(&herr, ctl + CTL_ERR, 4, cudaMemcpyDeviceToHost, st));
+    CK(cudaStreamSynchronize(st));
+    if (herr) return set_err("batch: device wait timed out (code %d)", herr);
+    return 0;
+}
+
+static int batch_check_steps(EmberCudaBatch *b, const int *toks, const int *pos, int n_steps) {
     if (n_steps < 1 || n_steps > b->max_steps) return set_err("batch: n_steps must be in [1, %d]", b->max_steps);
     for (int i = 0; i < b->S; i++) {
         if (toks[i] < 0 || toks[i] >= b->m->vocab) return set_err("batch: token id %d out of range", toks[i]);
-        if (pos[i] < 0 || pos[i] + n_steps > b->ctx) return set_err("batch: stream %d does not fit the context", i);
+        if (pos[i] < 0 || pos[i] > b->ctx - n_steps) return set_err("batch: stream %d does not fit the context", i);
     }
+    return 0;
+}
+
+extern "C" int ember_cuda_batch_greedy(EmberCudaBatch *b, const int *toks, const int *pos, int n_steps,
+                                       int *host_tokens, float *host_logits) {
+    CK(cudaSetDevice(b->m->device));
+    if (batch_check_steps(b, toks, pos, n_steps)) return 1;
     if (!b->reps.empty()) {
         // every stream's steps enqueued before any wait, so that they run at once
         for (int i = 0; i < b->S; i++)
@@ -996,36 +1283,42 @@ extern "C" int ember_cuda_batch_greedy(EmberCudaBatch *b, const int *toks, const
                               cudaMemcpyDeviceToHost));
         return 0;
     }
-    cudaStream_t st = b->worker->stream;
-    if (!b->g_step) {
-        cudaGraph_t g = nullptr;
-        CK(cudaStreamBeginCapture(st, cudaStreamCaptureModeThreadLocal));
-        int rc = batch_record(b);
-        cudaError_t e = cudaStreamEndCapture(st, &g);
-        if (rc) {
-            if (g) cudaGraphDestroy(g);
-            return 1;
-        }
-        if (e != cudaSuccess) return set_err("batch graph capture failed: %s", cudaGetErrorString(e));
-        e = cudaGraphInstantiate(&b->g_step, g, 0);
-        cudaGraphDestroy(g);
-        if (e != cudaSuccess) return set_err("batch graph instantiate failed: %s", cudaGetErrorString(e));
+    return batch_run(b, false, toks, pos, n_steps, host_tokens, host_logits);
+}
+
+extern "C" int ember_cuda_batch_sample(EmberCudaBatch *b, const int *toks, const int *pos, int n_steps,
+                                       const EmberSampleParams *params, const float *u, int *host_tokens,
+                                       float *host_logits) {
+    CK(cudaSetDevice(b->m->device));
+    if (!params || !u) return set_err("batch: null settings or random numbers");
+    if (!b->reps.empty())
+        return set_err("batch: drawn steps need a batch of more than %d streams or one over a 4-bit cache", BATCH_REPLICA_MAX);
+    if (batch_check_steps(b, toks, pos, n_steps)) return 1;
+    if (b->m->vocab > EMBER_SAMPLE_MAX_VOCAB) return set_err("batch: a vocabulary of %d is too large to draw from", b->m->vocab);
+    std::vector<float> set((size_t)3 * b->S);
+    std::vector<int> top_k(b->S);
+    for (int i = 0; i < b->S; i++) {
+        const EmberSampleParams &p = params[i];
+        if (p.repeat_penalty != 1.0f || p.presence_penalty != 0.0f || p.frequency_penalty != 0.0f)
+            return set_err("batch: stream %d: penalties are not supported by drawn steps", i);
+        if (p.temperature != p.temperature) return set_err("batch: stream %d: temperature is NaN", i);
+        set[i] = p.temperature;
+        set[(size_t)b->S + i] = p.top_p;
+        set[(size_t)2 * b->S + i] = p.min_p;
+        top_k[i] = p.top_k;
     }
-    CK(cudaMemcpyAsync(b->tok, toks, (size_t)b->S * 4, cudaMemcpyHostToDevice, st));
-    CK(cudaMemcpyAsync(b->pos, pos, (size_t)b->S * 4, cudaMemcpyHostToDevice, st));
-    CK(cudaMemsetAsync(b->nout, 0, 4, st));
-    CK(cudaMemsetAsync(b->worker->ctl + CTL_ERR, 0, 4, st));
-    for (int i = 0; i < n_steps; i++) CK(cudaGraphLaunch(b->g_step, st));
-    if (host_tokens)
-        CK(cudaMemcpyAsync(host_tokens, b->out, (size_t)n_steps * b->S * 4, cudaMemcpyDeviceToHost, st));
-    if (host_logits)
-        CK(cudaMemcpy2DAsync(host_logits, (size_t)b->m->vocab * 4, b->logits, (size_t)b->ld_log * 4,
-                             (size_t)b->m->vocab * 4, (size_t)b->S, cudaMemcpyDeviceToHost, st));
-    int herr = 0;
-    CK(cudaMemcpyAsync(&herr, b->worker->ctl + CTL_ERR, 4, cudaMemcpyDeviceToHost, st));
-    CK(cudaStreamSynchronize(st));
-    if (herr) return set_err("batch: device wait timed out (code %d)", herr);
-    return 0;
+    if (!b->d_u) {
+        if (pf_alloc(b->allocs, (void **)&b->d_set, (size_t)4 * b->S * 4) ||
+            pf_alloc(b->allocs, (void **)&b->d_top_k, (size_t)b->S * 4) ||
+            pf_alloc(b->allocs, (void **)&b->d_drawn, (size_t)b->S * 4) ||
+            pf_alloc(b->allocs, (void **)&b->d_u, (size_t)b->max_steps * b->S * 4))
+            return 1;
+    }
+    cudaStream_t st = batch_stream(b);
+    CK(cudaMemcpyAsync(b->d_set, set.data(), set.size() * 4, cudaMemcpyHostToDevice, st));
+    CK(cudaMemcpyAsync(b->d_top_k, top_k.data(), top_k.size() * 4, cudaMemcpyHostToDevice, st));
+    CK(cudaMemcpyAsync(b->d_u, u, (size_t)n_steps * b->S * 4, cudaMemcpyHostToDevice, st));
+    return batch_run(b, true, toks, pos, n_steps, host_tokens, host_logits);
 }
 
 #ifdef EMBER_PROBES

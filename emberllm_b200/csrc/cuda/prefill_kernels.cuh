@@ -730,6 +730,7 @@ struct PfQkvArgs {
     const int *pos;        // batched decode: token t's position pos[t] (device) and
     size_t cache_stride;   //   its own cache at kc/vc + t * cache_stride elements
     float eps;
+    float *kr, *vr;        // when set: keys and values as plain rows [n][n_kv][hd] instead of the cache
 };
 
 // One warp per (token, head) for the nh query heads and nkv key heads, eight
@@ -779,6 +780,11 @@ __global__ void __launch_bounds__(32 * PF_QKV_WARPS) pf_qkv_post_kernel(const Pf
     for (int i = lane; i < hd; i += 32) {
         if (is_q) {
             a.qr[(size_t)t * qd + head * hd + i] = vals[i];
+        } else if (a.kr) {
+            float v = row[qd + kvd + head * hd + i];
+            if (a.bv) v = fadd(v, a.bv[head * hd + i]);
+            a.kr[((size_t)t * a.nkv + head) * hd + i] = vals[i];
+            a.vr[((size_t)t * a.nkv + head) * hd + i] = v;
         } else {
             T *kt = reinterpret_cast<T *>(a.kc) + coff + (size_t)head * hd * a.kstride;
             T *vt = reinterpret_cast<T *>(a.vc) + coff + (size_t)head * a.ctx * hd;

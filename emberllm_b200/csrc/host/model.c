@@ -10,6 +10,7 @@
  * that the device reproduces the reference's results bit for bit.
  */
 #include "model_internal.h"
+#include "ember_kv4.h"
 
 #include <stdio.h>
 #include <stdlib.h>
@@ -247,7 +248,9 @@ struct EmberBatch {
     float *logits;            /* [vocab]: the last prompt's logits */
 };
 
-EmberBatch *ember_batch_new(EmberModel *m, int n_streams, int ctx_len, int kv_fp16, int max_steps) {
+/* pages >= 0: a paged 4-bit cache */
+static EmberBatch *batch_new(EmberModel *m, int n_streams, int ctx_len, int kv_fp16, int pages, int window, int sinks,
+                             int max_steps) {
     const EmberHeader *h = ember_model_header(m);
     if (h->n_heads <= 0 || h->n_kv_heads <= 0 || h->n_heads % h->n_kv_heads != 0)
         ember_die("n_heads (%d) must be a positive multiple of n_kv_heads (%d)", h->n_heads, h->n_kv_heads);
@@ -261,11 +264,27 @@ EmberBatch *ember_batch_new(EmberModel *m, int n_streams, int ctx_len, int kv_fp
     size_t n_rope = (size_t)b->ctx * (size_t)(h->head_dim / 2) * 2;
     float *rope = ember_xmalloc(n_rope * sizeof(float), "rope table");
     ember_host_rope_table(rope, b->ctx, h->head_dim, h->rope_theta);
-    cuda_check(ember_cuda_batch_new(m->dev, n_streams, b->ctx, kv_fp16 ? 1 : 0, rope, max_steps, &b->dev),
+    cuda_check(pages >= 0 ? ember_cuda_batch_new_kv4(m->dev, n_streams, b->ctx, pages, window, sinks, rope, max_steps,
+                                                     &b->dev)
+                          : ember_cuda_batch_new(m->dev, n_streams, b->ctx, kv_fp16 ? 1 : 0, rope, max_steps, &b->dev),
                "batch");
     free(rope);
     b->logits = ember_xmalloc((size_t)b->vocab * sizeof(float), "batch logits");
     return b;
+}
+
+EmberBatch *ember_batch_new(EmberModel *m, int n_streams, int ctx_len, int kv_fp16, int max_steps) {
+    return batch_new(m, n_streams, ctx_len, kv_fp16, -1, 0, 0, max_steps);
+}
+
+EmberBatch *ember_batch_new_kv4(EmberModel *m, int n_streams, int ctx_len, int n_pages, int window, int sinks,
+                                int max_steps) {
+    if (n_pages < 0) ember_die("a cache of %d pages is not supported", n_pages);
+    return batch_new(m, n_streams, ctx_len, 0, n_pages, window, sinks, max_steps);
+}
+
+void ember_batch_release(EmberBatch *b, int stream) {
+    cuda_check(ember_cuda_batch_release(b->dev, stream), "batch release");
 }
 
 void ember_batch_free(EmberBatch *b) {
@@ -295,4 +314,9 @@ void ember_batch_greedy(EmberBatch *b, const int *toks, const int *pos, int n_st
                       b->ctx);
     }
     cuda_check(ember_cuda_batch_greedy(b->dev, toks, pos, n_steps, out_tokens, out_logits), "batch greedy");
+}
+
+void ember_batch_sample(EmberBatch *b, const int *toks, const int *pos, int n_steps, const EmberSampleParams *params,
+                        const float *u, int *out_tokens, float *out_logits) {
+    cuda_check(ember_cuda_batch_sample(b->dev, toks, pos, n_steps, params, u, out_tokens, out_logits), "batch sample");
 }

@@ -149,6 +149,33 @@ typedef struct {
 } EmberSampleRows;
 int ember_cuda_sample_rows(const EmberSampleRows *args, void *stream);
 
+/* ---- streams over a paged 4-bit cache, and drawn steps ----
+ * A batch of independent streams (ember_cuda_batch_*, ember_batch_*) whose caches are
+ * pages of 64 positions in 4 bits, taken from one pool of n_pages (0: enough for every
+ * stream's whole context) when a prompt or a step needs them. Keys and values are
+ * quantized, so tokens may differ from those over an fp32 or fp16 cache; attention is
+ * ember_cuda_kv4_attention's, with `window` and `sinks`. Any n_streams in [1, 512];
+ * head_dim 32, 64 or 128. prefill, greedy, sample and free take such a batch as any
+ * other. A call that finds no free page fails and leaves the streams as they were
+ * (pages handed out before it found out stay with their streams). release gives a
+ * stream's pages back: its next prompt starts anew. */
+int ember_cuda_batch_new_kv4(EmberCudaModel *m, int n_streams, int ctx, int n_pages, int window, int sinks,
+                             const float *rope_cs, int max_steps, EmberCudaBatch **out);
+int ember_cuda_batch_release(EmberCudaBatch *b, int stream);
+/* As ember_cuda_batch_greedy, but every step's tokens are drawn by
+ * ember_cuda_sample_rows: stream i with params[i] (no penalties) and, at step t, the
+ * random number u[t * n_streams + i]. Not for a batch that holds one state per stream
+ * (up to 8 streams over an fp32 or fp16 cache). */
+int ember_cuda_batch_sample(EmberCudaBatch *b, const int *toks, const int *pos, int n_steps,
+                            const EmberSampleParams *params, const float *u, int *host_tokens, float *host_logits);
+
+/* the same on the public batch; fatal errors follow the library's convention */
+EmberBatch *ember_batch_new_kv4(EmberModel *m, int n_streams, int ctx_len, int n_pages, int window, int sinks,
+                                int max_steps);
+void ember_batch_release(EmberBatch *b, int stream);
+void ember_batch_sample(EmberBatch *b, const int *toks, const int *pos, int n_steps, const EmberSampleParams *params,
+                        const float *u, int *out_tokens, float *out_logits);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif
