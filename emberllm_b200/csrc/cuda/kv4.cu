@@ -16,38 +16,48 @@ struct Kv4Io {
     int64_t k_tok, k_head, v_tok, v_head;
 };
 
-EMB_DEV void load4(const float *p, bool vec, float (&x)[4]) {
+EMB_DEV void load8(const float *p, bool vec, float (&x)[8]) {
     if (vec) {
-        const float4 f = *reinterpret_cast<const float4 *>(p);
+        const float4 f = reinterpret_cast<const float4 *>(p)[0], g = reinterpret_cast<const float4 *>(p)[1];
         x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
+        x[4] = g.x; x[5] = g.y; x[6] = g.z; x[7] = g.w;
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; j++) x[j] = p[j];
+        for (int j = 0; j < 8; j++) x[j] = p[j];
     }
 }
-EMB_DEV void load4(const __half *p, bool vec, float (&x)[4]) {
+EMB_DEV void load8(const __half *p, bool vec, float (&x)[8]) {
     if (vec) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(p);
-        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&w.x));
-        const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
-        x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+        const uint4 w = *reinterpret_cast<const uint4 *>(p);
+        const __half2 *h = reinterpret_cast<const __half2 *>(&w);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float2 f = __half22float2(h[j]);
+            x[2 * j] = f.x; x[2 * j + 1] = f.y;
+        }
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; j++) x[j] = __half2float(p[j]);
+        for (int j = 0; j < 8; j++) x[j] = __half2float(p[j]);
     }
 }
 
-// code of x for scale d: floor(x / d + 8.5) in exact arithmetic. The division and
-// the addition round, so the result can be one off where x / d lies next to a
-// border (c - 8.5); a border times d has 13 significant bits, exact in fp32, so
-// comparing x with the borders around the first guess settles it.
-EMB_DEV uint32_t kv4_code(float x, float d) {
-    const float ax = d < 0.0f ? -x : x, ad = fabsf(d);
-    float c = floorf(__fadd_rn(__fdiv_rn(ax, ad), 8.5f));
-    c = fminf(fmaxf(c, 0.0f), 15.0f);
-    if (ax < __fmul_rn(c - 8.5f, ad)) c -= 1.0f;
-    else if (ax >= __fmul_rn(c - 7.5f, ad)) c += 1.0f;
-    return (uint32_t)fminf(fmaxf(c, 0.0f), 15.0f);
+// code of x for scale d: floor(x / d + 8.5) in exact arithmetic, clamped; y = x * inv,
+// inv = 1 / d, is off by less than 2e-6. Adding 1.5 * 2^23 + 8 rounds y + 8 to the nearest
+// whole number, in the lower bits. Within 1e-4 of a border (c - 8.5) that may be the
+// wrong side: a border times d has 13 significant bits, exact in fp32, so comparing x
+// with it settles it. (No conversion instructions: their pipe takes 16 lanes a cycle.)
+EMB_DEV uint32_t kv4_code(float x, float d, float inv) {
+    const float y = fminf(fmaxf(__fmul_rn(x, inv), -9.0f), 9.0f);
+    const float r = __fadd_rn(y, 12582920.0f);
+    int c = (int)(__float_as_uint(r) & 0xFFu);                   // -1 (0xFF) .. 17
+    c = c == 0xFF ? -1 : c;
+    const float whole = __fadd_rn(r, -12582912.0f);
+    if (fabsf(__fadd_rn(y, 8.0f) - whole) > 0.4999f) {
+        const float ax = d < 0.0f ? -x : x, ad = fabsf(d);
+        if (ax < __fmul_rn(whole - 8.5f, ad)) c -= 1;
+        else if (ax >= __fmul_rn(whole - 7.5f, ad)) c += 1;
+    }
+    return (uint32_t)min(max(c, 0), 15);
 }
 
 // The scale of a block whose value of largest magnitude (the first one) is v.
@@ -58,90 +68,133 @@ EMB_DEV __half kv4_scale(float v) {
     return __float2half_rn(__uint_as_float(u));
 }
 
-// Store and read, one kernel per direction. Eight lanes hold a block, each four
-// consecutive elements and so one 16-bit piece of a key word or of a value row;
-// head_dim / 4 lanes hold a row of one head. Bound by memory: each row is read
-// (written) once, 16 bytes a lane for fp32 rows.
-// x: items (row, kv head, keys or values); y: sequences.
-constexpr int KV4_IO_THREADS = 256;
+// Store and read, one kernel per direction. Four lanes hold a block, each eight
+// consecutive elements: one 32-bit key word, or one 16-bit piece of each of two value
+// words; head_dim / 8 lanes hold a row of one head. A thread takes KV4_IO_ROWS rows
+// in a row, so that their loads are under way together. Bound by memory: each
+// row is read (written) once, 16 bytes a lane and load.
+// x: items (row, kv head, keys or values) of a row group; y: sequences.
+constexpr int KV4_IO_THREADS = 256, KV4_IO_ROWS = 4;
 
 template <typename T, int HD, bool STORE>
 __global__ void __launch_bounds__(KV4_IO_THREADS) kv4_io_kernel(Kv4View c, Kv4Rows b, Kv4Io io, bool vec) {
-    constexpr int LANES = HD / 4, NB = HD / 32;
+    constexpr int LANES = HD / 8, NB = HD / 32, N = KV4_IO_ROWS;
     const Kv4Seq s = kv4_seq(b, blockIdx.y);
-    const int lane = threadIdx.x % LANES;
-    const long long item = ((long long)blockIdx.x * KV4_IO_THREADS + threadIdx.x) / LANES;
-    const int per_row = 2 * c.n_kv;
-    const long long row = item / per_row;
-    // no lane leaves before the shuffles: lanes of other items share the warp
-    bool live = row < s.rows;
-    const int which = (int)(item % per_row), head = which >> 1;
+    const int lane = threadIdx.x % LANES, per_row = 2 * c.n_kv;
+    const unsigned item = (blockIdx.x * KV4_IO_THREADS + threadIdx.x) / LANES;
+    const int group_row = (int)(item / per_row), which = (int)(item - (unsigned)group_row * per_row), head = which >> 1;
     const bool is_v = which & 1;
-    const long long pos = (long long)s.len - s.rows + row;
-    live = live && pos >= 0 && pos < b.cap;
-    const int page = live ? kv4_page(c, b, blockIdx.y, (int)pos) : -1;
-    live = page >= 0;
-    const int slot = (int)(pos & ((1 << c.page_shift) - 1)), in = slot & 15;
-    uint8_t *chunk = live ? kv4_chunk_ptr(c, page, head) : nullptr;
-    const int blk = lane >> 3, g = lane & 7;
-    uint16_t *code = nullptr;
-    __half *scale = nullptr;
-    if (live) {
-        uint8_t *group = chunk + (slot >> 4) * kv4_group(HD);
-        const int pair = in >> 1, odd = in & 1;
-        code = reinterpret_cast<uint16_t *>(
-            group + (is_v ? 8 * HD + pair * HD + g * (4 * NB) + 4 * blk + 2 * odd
-                          : in * (HD / 2) + (g >> 1) * (4 * NB) + 4 * blk + 2 * (g & 1)));
-        scale = reinterpret_cast<__half *>(group + 16 * HD) + (is_v ? 16 * NB + (pair * NB + blk) * 2 + odd : in * NB + blk);
+    const int ps = 1 << c.page_shift, blk = lane >> 2, w4 = lane & 3;
+    uint8_t *group[N];               // the position's group of 16, or null
+    T *mem[N];
+    int in[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int row = group_row * N + i;
+        const long long pos = (long long)s.len - s.rows + row;
+        const bool live = row < s.rows && pos >= 0 && pos < b.cap;
+        const int page = live ? kv4_page(c, b, blockIdx.y, (int)pos) : -1;
+        const int slot = (int)(pos & (ps - 1));
+        in[i] = slot & 15;
+        group[i] = page >= 0 ? kv4_chunk_ptr(c, page, head) + (slot >> 4) * kv4_group(HD) : nullptr;
+        const long long tok = s.row0 + row;
+        mem[i] = is_v ? (T *)io.v + tok * io.v_tok + head * io.v_head + lane * 8
+                      : (T *)io.k + tok * io.k_tok + head * io.k_head + lane * 8;
     }
-    const long long tok = s.row0 + row;
-    T *mem = nullptr;
-    if (live)
-        mem = is_v ? (T *)io.v + tok * io.v_tok + head * io.v_head + lane * 4
-                   : (T *)io.k + tok * io.k_tok + head * io.k_head + lane * 4;
+    // where a position's codes and scale are: keys one word, values the halves of the
+    // words g = 2 w4 and 2 w4 + 1
+    auto codes = [&](int i) {
+        return is_v ? group[i] + 8 * HD + (in[i] >> 1) * HD + (2 * w4) * (4 * NB) + 4 * blk + 2 * (in[i] & 1)
+                    : group[i] + in[i] * (HD / 2) + w4 * (4 * NB) + 4 * blk;
+    };
+    auto scale = [&](int i) {
+        return reinterpret_cast<__half *>(group[i] + 16 * HD) +
+               (is_v ? 16 * NB + ((in[i] >> 1) * NB + blk) * 2 + (in[i] & 1) : in[i] * NB + blk);
+    };
+    float x[N][8];
     if (STORE) {
-        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (live) load4(mem, vec, x);
-        float m = 0.0f, first = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            x[j] = x[j] != x[j] ? 0.0f : fminf(fmaxf(x[j], -3.402823466e38f), 3.402823466e38f);
-            if (fabsf(x[j]) > m) { m = fabsf(x[j]); first = x[j]; }
+        for (int i = 0; i < N; i++) {
+            if (group[i]) load8(mem[i], vec, x[i]);
+            else
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[i][j] = 0.0f;
         }
-        float bm = m;
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, o));
-        const unsigned mask = __ballot_sync(0xffffffffu, m == bm);
-        const int base = (threadIdx.x & 31) & ~7;
-        const int src = base + __ffs((mask >> base) & 0xffu) - 1;
-        const __half d = kv4_scale(__shfl_sync(0xffffffffu, first, src));
-        const float df = __half2float(d);
-        if (!live) return;
-        uint32_t w = 0;
+        for (int i = 0; i < N; i++) {
+            float m = 0.0f, first = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; j++) w |= (df != 0.0f ? kv4_code(x[j], df) : 8u) << (4 * j);
-        *code = (uint16_t)w;
-        if (g == 0) *scale = d;
+            for (int j = 0; j < 8; j++) {
+                float &v = x[i][j];
+                v = v != v ? 0.0f : fminf(fmaxf(v, -3.402823466e38f), 3.402823466e38f);
+                if (fabsf(v) > m) { m = fabsf(v); first = v; }
+            }
+            float bm = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
+            // the first lane of the block that has it
+            const unsigned mask = __ballot_sync(0xffffffffu, m == bm);
+            const int base = (threadIdx.x & 31) & ~3;
+            const __half d = kv4_scale(__shfl_sync(0xffffffffu, first, base + __ffs((mask >> base) & 0xfu) - 1));
+            const float df = __half2float(d), inv = df != 0.0f ? __fdiv_rn(1.0f, df) : 0.0f;
+            uint32_t w = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) w |= (df != 0.0f ? kv4_code(x[i][j], df, inv) : 8u) << (4 * j);
+            if (!group[i]) continue;
+            uint8_t *p = codes(i);
+            if (is_v) {
+                *reinterpret_cast<uint16_t *>(p) = (uint16_t)w;
+                *reinterpret_cast<uint16_t *>(p + 4 * NB) = (uint16_t)(w >> 16);
+            } else {
+                *reinterpret_cast<uint32_t *>(p) = w;
+            }
+            if (w4 == 0) *scale(i) = d;
+        }
     } else {
-        if (!live) return;
-        const uint32_t w = *code;
-        const float d = __half2float(*scale);
-        float x[4];
+        uint32_t w[N];
+        __half d[N];
 #pragma unroll
-        for (int j = 0; j < 4; j++) x[j] = (float)((int)((w >> (4 * j)) & 15u) - 8) * d;
-        if (sizeof(T) == 4) {
-            float *o = reinterpret_cast<float *>(mem);
-            if (vec) *reinterpret_cast<float4 *>(o) = make_float4(x[0], x[1], x[2], x[3]);
-            else
+        for (int i = 0; i < N; i++) {
+            w[i] = 0;
+            d[i] = __float2half_rn(0.0f);
+            if (!group[i]) continue;
+            const uint8_t *p = codes(i);
+            w[i] = is_v ? *reinterpret_cast<const uint16_t *>(p) |
+                              (uint32_t)*reinterpret_cast<const uint16_t *>(p + 4 * NB) << 16
+                        : *reinterpret_cast<const uint32_t *>(p);
+            d[i] = *scale(i);
+        }
 #pragma unroll
-                for (int j = 0; j < 4; j++) o[j] = x[j];
-        } else {
-            __half *o = reinterpret_cast<__half *>(mem);
-            __half2 h[2] = {__floats2half2_rn(x[0], x[1]), __floats2half2_rn(x[2], x[3])};   // exact
-            if (vec) *reinterpret_cast<uint2 *>(o) = *reinterpret_cast<uint2 *>(h);
-            else
+        for (int i = 0; i < N; i++) {
+            if (!group[i]) continue;
+            // (code - 8) * d, exact in fp16: dims 0,4 / 1,5 / 2,6 / 3,7
+            const __half2 dd = __half2half2(d[i]);
+            const uint32_t h0 = kp_low(w[i], dd), h1 = kp_high(w[i], dd), h2 = kp_low(w[i] >> 8, dd),
+                           h3 = kp_high(w[i] >> 8, dd);
+            const uint4 q = make_uint4(__byte_perm(h0, h1, 0x5410), __byte_perm(h2, h3, 0x5410),
+                                       __byte_perm(h0, h1, 0x7632), __byte_perm(h2, h3, 0x7632));
+            const __half2 *qh = reinterpret_cast<const __half2 *>(&q);
 #pragma unroll
-                for (int j = 0; j < 4; j++) o[j] = __float2half_rn(x[j]);
+            for (int j = 0; j < 4; j++) {
+                const float2 f = __half22float2(qh[j]);
+                x[i][2 * j] = f.x;
+                x[i][2 * j + 1] = f.y;
+            }
+            if (sizeof(T) == 4) {
+                float *o = reinterpret_cast<float *>(mem[i]);
+                if (vec) {
+                    reinterpret_cast<float4 *>(o)[0] = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
+                    reinterpret_cast<float4 *>(o)[1] = make_float4(x[i][4], x[i][5], x[i][6], x[i][7]);
+                } else
+#pragma unroll
+                    for (int j = 0; j < 8; j++) o[j] = x[i][j];
+            } else {
+                __half *o = reinterpret_cast<__half *>(mem[i]);
+                if (vec) {
+                    *reinterpret_cast<uint4 *>(o) = q;
+                } else
+#pragma unroll
+                    for (int j = 0; j < 8; j++) o[j] = __float2half_rn(x[i][j]);
+            }
         }
     }
 }
@@ -234,9 +287,9 @@ static int kv4_views(const char *who, const EmberKv4Cache *cache, const EmberKv4
 template <typename T, bool STORE>
 static int kv4_io_launch(const Kv4View &c, const Kv4Rows &b, const Kv4Io &io, bool vec, int hd, int max_q,
                          cudaStream_t st) {
-    const long long items = (long long)max_q * 2 * c.n_kv * (hd / 4);
+    const long long items = ((long long)max_q + KV4_IO_ROWS - 1) / KV4_IO_ROWS * 2 * c.n_kv * (hd / 8);
     const long long gx = (items + KV4_IO_THREADS - 1) / KV4_IO_THREADS;
-    if (gx > 0x7FFFFFFFll) return set_err("kv4: max_q %d is too large", max_q);
+    if (items > 0x7FFFFFFFll - KV4_IO_THREADS) return set_err("kv4: max_q %d is too large", max_q);
     const dim3 grid((unsigned)gx, (unsigned)b.n_seqs);
     switch (hd) {
     case 32: kv4_io_kernel<T, 32, STORE><<<grid, KV4_IO_THREADS, 0, st>>>(c, b, io, vec); break;
@@ -266,9 +319,10 @@ static int kv4_io(const char *who, const EmberKv4Cache *cache, const EmberKv4Bat
         return set_err("%s: k and v must be memory of the cache's device", who);
     if (rows->k_tok < 0 || rows->k_head < 0 || rows->v_tok < 0 || rows->v_head < 0)
         return set_err("%s: negative strides are not supported", who);
-    const size_t w = 4 * es;      // a lane's four elements as one access
-    const bool vec = !((uintptr_t)rows->k % w || (uintptr_t)rows->v % w || rows->k_tok % 4 || rows->k_head % 4 ||
-                       rows->v_tok % 4 || rows->v_head % 4);
+    // a lane's eight elements as 16-byte accesses
+    const int64_t per = 16 / (int64_t)es;
+    const bool vec = !((uintptr_t)rows->k % 16 || (uintptr_t)rows->v % 16 || rows->k_tok % per || rows->k_head % per ||
+                       rows->v_tok % per || rows->v_head % per);
     Kv4Io io;
     io.k = const_cast<void *>(rows->k); io.v = const_cast<void *>(rows->v);
     io.k_tok = rows->k_tok; io.k_head = rows->k_head; io.v_tok = rows->v_tok; io.v_head = rows->v_head;
