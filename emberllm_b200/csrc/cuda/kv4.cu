@@ -68,6 +68,63 @@ EMB_DEV __half kv4_scale(float v) {
     return __float2half_rn(__uint_as_float(u));
 }
 
+// Eight elements of a block held by four neighbouring lanes: their codes as a word, and
+// the block's scale. Called by whole warps.
+EMB_DEV void kv4_block(float (&x)[8], uint32_t *word, __half *scale) {
+    const int base = (threadIdx.x & 31) & ~3;
+    // the largest and the smallest decide the scale unless they tie; z is NaN when some
+    // element is no finite number
+    float hi = x[0], lo = x[0], z = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        hi = fmaxf(hi, x[j]);
+        lo = fminf(lo, x[j]);
+        z = fmaf(x[j], 0.0f, z);
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    }
+    const float m = fmaxf(hi, -lo);
+    __half d = kv4_scale(hi > -lo ? hi : lo);
+    float df = __half2float(d), inv = __fdividef(1.0f, df);
+    // ordinary blocks: |x / d| <= 8.04, so 1.5 * 2^23 + 8 + x / d has the code in its lower
+    // bits, rounded to nearest; how far that was from x / d tells of borders
+    uint32_t w = 0;
+    float off = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float r = fmaf(x[j], inv, 12582920.0f);
+        off = fmaxf(off, fabsf(fmaf(x[j], inv, 12582920.0f - r)));
+        w += __float_as_uint(fminf(r, 12582927.0f)) << (4 * j);
+    }
+    w -= 0x4B400000u * 0x11111111u;
+    // the others: no finite numbers, two largest of opposite signs, scales that saturate
+    // or are no normal fp16 number, an element within 1e-5 of a border (x / d is 4e-6 off)
+    const bool rare = z != z || hi == -lo || m > 65000.0f || m < 0.0005f || off > 0.49999f;
+    if (__any_sync(0xffffffffu, rare)) {
+        float am = 0.0f, first = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            x[j] = x[j] != x[j] ? 0.0f : fminf(fmaxf(x[j], -3.402823466e38f), 3.402823466e38f);
+            if (fabsf(x[j]) > am) { am = fabsf(x[j]); first = x[j]; }
+        }
+        float bm = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
+        bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
+        // the first lane of the block that has it
+        const unsigned mask = __ballot_sync(0xffffffffu, am == bm);
+        d = kv4_scale(__shfl_sync(0xffffffffu, first, base + __ffs((mask >> base) & 0xfu) - 1));
+        df = __half2float(d);
+        inv = df != 0.0f ? __fdiv_rn(1.0f, df) : 0.0f;
+        w = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) w |= (df != 0.0f ? kv4_code(x[j], df, inv) : 8u) << (4 * j);
+    }
+    *word = w;
+    *scale = d;
+}
+
 // Store and read, one kernel per direction. Four lanes hold a block, each eight
 // consecutive elements: one 32-bit key word, or one 16-bit piece of each of two value
 // words; head_dim / 8 lanes hold a row of one head. A thread takes KV4_IO_ROWS rows
@@ -82,25 +139,32 @@ __global__ void __launch_bounds__(KV4_IO_THREADS) kv4_io_kernel(Kv4View c, Kv4Ro
     const Kv4Seq s = kv4_seq(b, blockIdx.y);
     const int lane = threadIdx.x % LANES, per_row = 2 * c.n_kv;
     const unsigned item = (blockIdx.x * KV4_IO_THREADS + threadIdx.x) / LANES;
-    const int group_row = (int)(item / per_row), which = (int)(item - (unsigned)group_row * per_row), head = which >> 1;
-    const bool is_v = which & 1;
+    const int group_row = (int)(item / per_row), which = (int)(item - (unsigned)group_row * per_row);
+    const bool is_v = which >= c.n_kv;           // neighbouring lanes: heads of the same tensor
+    const int head = is_v ? which - c.n_kv : which;
     const int ps = 1 << c.page_shift, blk = lane >> 2, w4 = lane & 3;
+    const int row0 = group_row * N, pos0 = s.len - s.rows + row0;
+    const int64_t stride = is_v ? io.v_tok : io.k_tok;
+    T *const mem0 = (T *)(is_v ? io.v : io.k) + (int64_t)(s.row0 + row0) * stride + head * (is_v ? io.v_head : io.k_head) +
+                    lane * 8;
+    uint8_t *const base = c.data + (size_t)head * c.chunk;
+    const uint64_t page_bytes = (uint64_t)c.n_kv * c.chunk;
+    const int32_t *table = b.table + (size_t)blockIdx.y * b.table_stride;
     uint8_t *group[N];               // the position's group of 16, or null
     T *mem[N];
     int in[N];
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        const int row = group_row * N + i;
-        const long long pos = (long long)s.len - s.rows + row;
-        const bool live = row < s.rows && pos >= 0 && pos < b.cap;
-        const int page = live ? kv4_page(c, b, blockIdx.y, (int)pos) : -1;
-        const int slot = (int)(pos & (ps - 1));
-        in[i] = slot & 15;
-        group[i] = page >= 0 ? kv4_chunk_ptr(c, page, head) + (slot >> 4) * kv4_group(HD) : nullptr;
-        const long long tok = s.row0 + row;
-        mem[i] = is_v ? (T *)io.v + tok * io.v_tok + head * io.v_head + lane * 8
-                      : (T *)io.k + tok * io.k_tok + head * io.k_head + lane * 8;
+        const int pos = pos0 + i;
+        const bool live = row0 + i < s.rows && pos >= 0 && pos < b.cap;
+        const int page = live ? __ldg(table + (pos >> c.page_shift)) : -1;
+        in[i] = pos & 15;
+        group[i] = (unsigned)page < (unsigned)c.n_pages
+                       ? base + (uint64_t)(uint32_t)page * page_bytes + ((pos & (ps - 1)) >> 4) * kv4_group(HD)
+                       : nullptr;
+        mem[i] = mem0 + i * stride;
     }
+    if (!__any_sync(0xffffffffu, row0 < s.rows)) return;
     // where a position's codes and scale are: keys one word, values the halves of the
     // words g = 2 w4 and 2 w4 + 1
     auto codes = [&](int i) {
@@ -118,27 +182,13 @@ __global__ void __launch_bounds__(KV4_IO_THREADS) kv4_io_kernel(Kv4View c, Kv4Ro
             if (group[i]) load8(mem[i], vec, x[i]);
             else
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[i][j] = 0.0f;
+                for (int j = 0; j < 8; j++) x[i][j] = j == 0 ? 1.0f : 0.0f;      // an ordinary block
         }
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            float m = 0.0f, first = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                float &v = x[i][j];
-                v = v != v ? 0.0f : fminf(fmaxf(v, -3.402823466e38f), 3.402823466e38f);
-                if (fabsf(v) > m) { m = fabsf(v); first = v; }
-            }
-            float bm = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
-            // the first lane of the block that has it
-            const unsigned mask = __ballot_sync(0xffffffffu, m == bm);
-            const int base = (threadIdx.x & 31) & ~3;
-            const __half d = kv4_scale(__shfl_sync(0xffffffffu, first, base + __ffs((mask >> base) & 0xfu) - 1));
-            const float df = __half2float(d), inv = df != 0.0f ? __fdiv_rn(1.0f, df) : 0.0f;
-            uint32_t w = 0;
-#pragma unroll
-            for (int j = 0; j < 8; j++) w |= (df != 0.0f ? kv4_code(x[i][j], df, inv) : 8u) << (4 * j);
+            uint32_t w;
+            __half d;
+            kv4_block(x[i], &w, &d);
             if (!group[i]) continue;
             uint8_t *p = codes(i);
             if (is_v) {
