@@ -9,43 +9,29 @@ its work on ``stream`` (a cudaStream_t as an integer; 0 is the default stream).
 Arguments that do not fit raise ValueError; what the library refuses raises
 RuntimeError with its message.
 """
-import ctypes
+import struct
 
 from . import _lib as _libmod
 
-_DTYPES = {"torch.float32": 0, "torch.float16": 3}
+# the structures of include/ember_kv4.h in native layout, packed per call: a ctypes
+# Structure of 14 fields costs a call a microsecond more
+_CACHE = struct.Struct("@Piiii")                # EmberKv4Cache
+_BATCH = struct.Struct("@PPPiiii")              # EmberKv4Batch
+_ROWS = struct.Struct("@PPi4xqqqq")             # EmberKv4Rows
+_ATT = struct.Struct("@PPiiqqqqfiiiPN")       # EmberKv4Attention
+_SAMPLE = struct.Struct("@PiiiqPPPPPP")         # EmberSampleRows
 
 
-class _Cache(ctypes.Structure):
-    _fields_ = [("data", ctypes.c_void_p), ("n_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
-                ("n_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+class _Dtypes(dict):
+    """the library's code of a dtype object, by its name"""
+
+    def __missing__(self, dtype):
+        self[dtype] = code = {"torch.float32": 0, "torch.float16": 3, "torch.int32": -32}.get(str(dtype))
+        return code
 
 
-class _Batch(ctypes.Structure):
-    _fields_ = [("q_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p), ("block_table", ctypes.c_void_p),
-                ("n_seqs", ctypes.c_int32), ("table_stride", ctypes.c_int32), ("n_tokens", ctypes.c_int32),
-                ("max_q", ctypes.c_int32)]
-
-
-class _Rows(ctypes.Structure):
-    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("dtype", ctypes.c_int32),
-                ("k_tok", ctypes.c_int64), ("k_head", ctypes.c_int64), ("v_tok", ctypes.c_int64),
-                ("v_head", ctypes.c_int64)]
-
-
-class _Attention(ctypes.Structure):
-    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("dtype", ctypes.c_int32),
-                ("n_heads", ctypes.c_int32), ("q_tok", ctypes.c_int64), ("q_head", ctypes.c_int64),
-                ("out_tok", ctypes.c_int64), ("out_head", ctypes.c_int64), ("scale", ctypes.c_float),
-                ("max_kv", ctypes.c_int32), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32),
-                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
-
-
-class _SampleRows(ctypes.Structure):
-    _fields_ = [("logits", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("n_rows", ctypes.c_int32),
-                ("vocab", ctypes.c_int32), ("stride", ctypes.c_int64), ("temperature", ctypes.c_void_p),
-                ("top_p", ctypes.c_void_p), ("min_p", ctypes.c_void_p), ("u", ctypes.c_void_p),
-                ("top_k", ctypes.c_void_p), ("out", ctypes.c_void_p)]
+_DT = _Dtypes()
+_F32, _I32 = 0, -32
 
 
 def _fail():
@@ -53,16 +39,16 @@ def _fail():
 
 
 def _dtype(t, name):
-    d = _DTYPES.get(str(t.dtype))
-    if d is None:
+    d = _DT[t.dtype]
+    if d is None or d < 0:
         raise ValueError(f"{name} must be float32 or float16, not {t.dtype}")
     return d
 
 
 def _array(t, name, dtype, n):
     """pointer of a contiguous array of n elements of `dtype`"""
-    if str(t.dtype) != dtype or t.ndim != 1 or t.shape[0] != n or (n > 1 and t.stride()[0] != 1):
-        raise ValueError(f"{name} must be a contiguous {dtype} array of {n}")
+    if _DT[t.dtype] != dtype or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name} must be a contiguous {'float32' if dtype == _F32 else 'int32'} array of {n}")
     return t.data_ptr()
 
 
@@ -96,28 +82,25 @@ class Kv4Cache:
         self.lib = _libmod.load()
         self.buffer = buffer            # kept alive
         self.page_size, self.n_kv_heads, self.head_dim = int(page_size), int(n_kv_heads), int(head_dim)
-        self._c = _Cache(buffer.data_ptr(), n_pages, page_size, n_kv_heads, head_dim)
-        self._p = ctypes.byref(self._c)
+        self._p = _CACHE.pack(buffer.data_ptr(), n_pages, page_size, n_kv_heads, head_dim)
 
     def _batch(self, tokens, q_start, kv_len, block_table, max_q):
         n = kv_len.shape[0]
-        if block_table.ndim != 2 or block_table.shape[0] != n or str(block_table.dtype) != "torch.int32" or \
-                (n and block_table.stride()[1] != 1 and block_table.shape[1] > 1):
-            raise ValueError(f"block_table must be an int32 [{n}][pages] array with consecutive pages")
-        stride = block_table.stride()[0] if n > 1 else block_table.shape[1]
-        if stride != block_table.shape[1]:
+        ts = block_table.shape
+        if len(ts) != 2 or ts[0] != n or _DT[block_table.dtype] != _I32:
+            raise ValueError(f"block_table must be an int32 [{n}][pages] array")
+        if not block_table.is_contiguous():
             raise ValueError("block_table must be contiguous")
-        return _Batch(None if q_start is None else _array(q_start, "q_start", "torch.int32", n + 1),
-                      _array(kv_len, "kv_len", "torch.int32", n), block_table.data_ptr(), n, stride, tokens, int(max_q))
+        return _BATCH.pack(0 if q_start is None else _array(q_start, "q_start", _I32, n + 1),
+                           _array(kv_len, "kv_len", _I32, n), block_table.data_ptr(), n, ts[1], tokens, max_q)
 
     def _io(self, fn, k, v, q_start, kv_len, block_table, max_q, stream):
         k_tok, k_head = _rows(k, "k", self.n_kv_heads, self.head_dim)
         v_tok, v_head = _rows(v, "v", self.n_kv_heads, self.head_dim)
         if k.shape[0] != v.shape[0] or k.dtype != v.dtype:
             raise ValueError("k and v must have the same rows and type")
-        b = self._batch(k.shape[0], q_start, kv_len, block_table, max_q)
-        r = _Rows(k.data_ptr(), v.data_ptr(), _dtype(k, "k"), k_tok, k_head, v_tok, v_head)
-        if fn(self._p, ctypes.byref(b), ctypes.byref(r), stream):
+        if fn(self._p, self._batch(k.shape[0], q_start, kv_len, block_table, max_q),
+              _ROWS.pack(k.data_ptr(), v.data_ptr(), _dtype(k, "k"), k_tok, k_head, v_tok, v_head), stream):
             _fail()
 
     def store(self, k, v, q_start, kv_len, block_table, max_q=1, stream=0):
@@ -150,11 +133,11 @@ class Kv4Cache:
         b = self._batch(q.shape[0], q_start, kv_len, block_table, max_q)
         if max_kv is None:
             max_kv = min(block_table.shape[1] * self.page_size, 2 ** 31 - 1)
-        ws, nws = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None \
-            else (None, 0)
-        a = _Attention(q.data_ptr(), out.data_ptr(), _dtype(q, "q"), heads, q_tok, q_head, out_tok, out_head,
-                       self.head_dim ** -0.5 if scale is None else scale, max_kv, window, sinks, ws, nws)
-        if self.lib.ember_cuda_kv4_attention(self._p, ctypes.byref(b), ctypes.byref(a), stream):
+        ws, nws = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
+        if self.lib.ember_cuda_kv4_attention(
+                self._p, b,
+                _ATT.pack(q.data_ptr(), out.data_ptr(), _dtype(q, "q"), heads, q_tok, q_head, out_tok, out_head,
+                          self.head_dim ** -0.5 if scale is None else scale, max_kv, window, sinks, ws, nws), stream):
             _fail()
 
 
@@ -168,11 +151,10 @@ def sample_rows(logits, out, u, temperature=None, top_k=None, top_p=None, min_p=
         raise ValueError("logits must be [rows][vocab] with consecutive elements")
     n = logits.shape[0]
 
-    def opt(t, name, dtype="torch.float32"):
-        return None if t is None else _array(t, name, dtype, n)
-    a = _SampleRows(logits.data_ptr(), _dtype(logits, "logits"), n, logits.shape[1], logits.stride()[0],
-                    opt(temperature, "temperature"), opt(top_p, "top_p"), opt(min_p, "min_p"),
-                    _array(u, "u", "torch.float32", n), opt(top_k, "top_k", "torch.int32"),
-                    _array(out, "out", "torch.int32", n))
-    if lib.ember_cuda_sample_rows(ctypes.byref(a), stream):
+    def opt(t, name, dtype=_F32):
+        return 0 if t is None else _array(t, name, dtype, n)
+    if lib.ember_cuda_sample_rows(
+            _SAMPLE.pack(logits.data_ptr(), _dtype(logits, "logits"), n, logits.shape[1], logits.stride(0),
+                         opt(temperature, "temperature"), opt(top_p, "top_p"), opt(min_p, "min_p"),
+                         _array(u, "u", _F32, n), opt(top_k, "top_k", _I32), _array(out, "out", _I32, n)), stream):
         _fail()

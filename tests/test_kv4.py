@@ -7,7 +7,7 @@ import re
 import numpy as np
 import pytest
 
-from emberllm_b200 import Kv4Cache, _lib
+from emberllm_b200 import Kv4Cache, _lib, kv4
 
 from . import helpers as H
 
@@ -143,6 +143,23 @@ def test_declared_functions_are_exported_and_listed():
     assert all(hasattr(lib, n) for n in names)
 
 
+def test_packed_structures_are_the_headers(tmp_path):
+    """the Python face packs the header's structures itself: sizes and last fields"""
+    import subprocess
+    src, exe = tmp_path / "s.c", tmp_path / "s"
+    src.write_text("""#include "ember_kv4.h"
+#include <stddef.h>
+#include <stdio.h>
+int main(void) { printf("%zu %zu %zu %zu %zu %zu %zu\\n", sizeof(EmberKv4Cache), sizeof(EmberKv4Batch),
+    sizeof(EmberKv4Rows), sizeof(EmberKv4Attention), sizeof(EmberSampleRows), offsetof(EmberKv4Attention, workspace),
+    offsetof(EmberSampleRows, stride)); }
+""")
+    subprocess.run(["gcc", "-I" + os.path.join(H.ROOT, "include"), "-o", str(exe), str(src)], check=True)
+    got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True).stdout.split()]
+    assert got == [s.size for s in (kv4._CACHE, kv4._BATCH, kv4._ROWS, kv4._ATT, kv4._SAMPLE)] + [72, 24]
+    assert kv4._ATT.unpack(kv4._ATT.pack(1, 2, 3, 4, 5, 6, 7, 8, 0.5, 9, 10, 11, 12, 13))[-2:] == (12, 13)
+
+
 @pytest.mark.parametrize("args", [(0, 16, 1, 64), (4, 24, 1, 64), (4, 8, 1, 64), (4, 256, 1, 64), (4, 16, 0, 64),
                                   (4, 16, 1, 96), (4, 16, 1, 256), (1 << 28, 16, 1, 64), (-1, 16, 1, 64)])
 def test_cache_sizes_refused(args):
@@ -165,8 +182,10 @@ def cpu_call(**change):
     p = Paged.__new__(Paged)
     buf = torch.zeros(Kv4Cache.nbytes(4, 16, 2, 64) + 16, dtype=torch.uint8)
     cache = Kv4Cache(buf, 4, 16, 2, 64)
-    for k, v in change.pop("cache", {}).items():
-        setattr(cache._c, k, v)
+    if "cache" in change:
+        c = dict(page_size=16, head_dim=64)
+        c.update(change.pop("cache"))
+        cache._p = kv4._CACHE.pack(buf.data_ptr(), 4, c["page_size"], 2, c["head_dim"])
     q = change.pop("q", torch.zeros(3, 4, 64))
     out = change.pop("out", torch.zeros_like(q))
     kw = dict(max_q=1, max_kv=16, window=0, sinks=0)
