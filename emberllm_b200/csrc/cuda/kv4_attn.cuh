@@ -262,7 +262,9 @@ __global__ void __launch_bounds__(KD_THREADS, KdLayout<HD, NT>::CTAS) kv4_decode
                 const float y = finite ? qv[i][b] * f1 * f2 : __int_as_float(0x7fffffff);
                 x[r][b * 32 + lane] = y;
             }
-            if (lane == 0) rscale[r] = a.scale * KV4_LOG2E / f1 / f2;
+            if (lane == 0)
+                rscale[r] = a.scale * KV4_LOG2E * __int_as_float((127 - e / 2) << 23) *
+                            __int_as_float((127 - e + e / 2) << 23);
         }
         __syncthreads();
         for (int f = warp; f < NT * NB; f += KD_WARPS) {

@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
         // Within 8 dims the order is 0,4,1,5,2,6,3,7, as the keys come out of their words:
         // neighbouring lanes exchange two numbers and store two pairs each.
         if (rt < tiles) {
-            constexpr int LPR = HD / 4, RPI = 32 / LPR, BATCH = 8;
+            constexpr int LPR = HD / 4, RPI = 32 / LPR, BATCH = HD == 128 && sizeof(T) == 2 ? 16 : 8;
             const int sub = lane / LPR, part = lane % LPR;
             // row `lane` of the warp: where it is (there is none: the tile's first, counted as 0)
             const int mine_rr = row_first + warp * 32 + lane, my_tok = mine_rr / a.group;
@@ -256,8 +256,10 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
                     uint32_t m = 0;
 #pragma unroll
                     for (int k = 0; k < 4; k++) m = max(m, __float_as_uint(v[k]) & 0x7FFFFFFFu);
+                    if (LPR == 32) m = __reduce_max_sync(0xffffffffu, m);
+                    else
 #pragma unroll
-                    for (int o = LPR / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                        for (int o = LPR / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
                     // |q| * 2^x below 2^14; the sign of the scale goes into the queries, so
                     // that a row's largest product is its largest score
                     const int x = m == 0 ? 0 : 13 - max((int)(m >> 23) - 127, -126);
@@ -266,7 +268,10 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
                     // (never 0: a hidden score, -inf, must stay -inf)
                     if (part == 0 && i < 32)
                         sh.rscale[warp * 32 + i] =
-                            a.scale == 0.0f ? 1.0f : fmaxf(fabsf(a.scale) * KV4_LOG2E / f1 / f2, 1.2e-38f);
+                            a.scale == 0.0f ? 1.0f
+                                            : fmaxf(fabsf(a.scale) * KV4_LOG2E * __int_as_float((127 - x / 2) << 23) *
+                                                        __int_as_float((127 - x + x / 2) << 23),
+                                                    1.2e-38f);
                     if (a.scale < 0.0f) f1 = -f1;
                     if (a.scale == 0.0f) f1 = 0.0f;
                     if (m >= 0x7F800000u) f1 = __int_as_float(0x7fffffff);
