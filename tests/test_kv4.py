@@ -510,6 +510,26 @@ def test_attention_prompts_again_and_again(dtype, heads, kvh, hd):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("seqs,ql,heads,kvh,hd", [(1, 40, 16, 8, 128), (40, 40, 16, 8, 128), (40, 33, 9, 3, 64),
+                                                  (2, 700, 4, 2, 64), (3, 600, 8, 1, 32), (70, 9, 16, 8, 128)])
+def test_attention_between_few_and_many_rows(dtype, seqs, ql, heads, kvh, hd):
+    """both kernels, in contiguous tensors and in odd strides and offsets"""
+    kv = [ql + (37 * i) % 300 for i in range(seqs)]
+    p = Paged(kv, [ql - i % min(ql, 7) for i in range(seqs)], 32, kvh, hd, seed=ql)
+    p.store_all()
+    n = sum(p.ql)
+    q = torch.randn(n, heads, hd, generator=torch.Generator().manual_seed(ql)).to(dtype).cuda()
+    got = check(p, q)
+    wide = torch.zeros(n, heads + 1, hd + 3, dtype=dtype, device="cuda")
+    q2 = wide[:, 1:, 3:]
+    q2.copy_(q)
+    out = torch.zeros(heads, n, hd + 1, dtype=dtype, device="cuda")[:, :, 1:].transpose(0, 1)
+    assert torch.equal(p.attend(q2, out=out, max_q=ql), got)
+    assert (wide[:, 0] == 0).all() and (wide[:, :, :3] == 0).all()
+
+
+@pytest.mark.gpu
 def test_attention_large_offsets():
     """a cache of more than 2^32 bytes: pages behind 4 GiB"""
     page, kvh, hd = 128, 8, 128
