@@ -34,7 +34,7 @@ constexpr int SR_THREADS = 512, SR_WARPS = SR_THREADS / 32;
 constexpr int SR_BINS = 1024;
 constexpr int SR_LIST = 768;              // tokens of a bin that are compared one by one
 constexpr int SR_MAX_CLUSTER = 8;
-static_assert(SR_BINS == 2 * SR_THREADS, "two bins a thread");
+static_assert(SR_BINS == 32 * 32, "32 groups of 32 bins");
 
 typedef unsigned long long u64;
 
@@ -43,17 +43,19 @@ constexpr int SR_FEW = 64;                // listed tokens compared with each ot
 
 // One CTA's shared memory; the row's slice of logits follows.
 struct SrShared {
-    union {
-        struct {
-            u64 w[SR_BINS];               // this CTA's bins: weights ...
-            uint32_t c[SR_BINS];          // ... and, where top_k needs them, tokens
-        } bin;
-        struct {
-            u64 key[SR_LIST], w[SR_LIST]; // the first CTA: tokens of the bin that is looked through
-        } list;
-    };
-    u64 run_w[SR_BINS];                   // running sums over the row's bins
-    uint32_t run_c[SR_BINS];
+    struct {
+        u64 w[SR_BINS];                   // this CTA's bins: weights ...
+        uint32_t c[SR_BINS];              // ... and, where top_k needs them, tokens
+    } bin;
+    struct {
+        u64 w[32];
+        uint32_t c[32];
+    } group;                              // sums of 32 bins each
+    struct {
+        u64 key[SR_LIST], w[SR_LIST];     // the first CTA: tokens of the bin that is looked through
+    } list;
+    u64 run_w[32];                        // running sums over the row's groups
+    uint32_t run_c[32];
     u64 sub_w[SR_SUB];                    // the first CTA: sums of the finer bins
     uint32_t sub_c[SR_SUB];
     int few[SR_LIST];                     // tokens of one of them
@@ -64,6 +66,7 @@ struct SrShared {
     int part_i[SR_WARPS], hi_i;
     int list_n[2], few_n;
     u64 at_w, at_c;                       // running sums before a bin that is looked through
+    uint32_t to_c;                        // tokens up to its end
     u64 res_key, res_w;                   // a search's result
     int bin_at;
 };
@@ -138,6 +141,15 @@ EMB_DEV uint32_t sr_bin_start(float mx, float scale, int at, int lane) {
         if (first > 0) k0 = __shfl_sync(~0u, k, first - 1);
     }
     return k1;
+}
+
+// The smallest distance in bin `at` or a later one, by a whole warp: d * scale is rounded
+// once, so it is next to at / scale.
+EMB_DEV float sr_bin_distance(float scale, int at, int lane) {
+    if (at == 0) return 0.0f;
+    const float d = __uint_as_float(__float_as_uint((float)at / scale) - 16 + lane);
+    const unsigned in = __ballot_sync(~0u, sr_bin(scale, d) >= at);
+    return __shfl_sync(~0u, d, in ? __ffs(in) - 1 : 31);
 }
 
 // where a running sum reaches its target
@@ -260,6 +272,15 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
         if (use_k) atomicAdd(&sh.bin.c[b], 1u);
         if (w) sr_add(&sh.bin.w[b], w);
     };
+    // running sums over a warp's lanes
+    auto warp_run = [&](u64 &w, uint32_t &c) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 vw = __shfl_up_sync(~0u, w, o);
+            const uint32_t vc = __shfl_up_sync(~0u, c, o);
+            if (lane >= o) { w += vw; c += vc; }
+        }
+    };
     // adds the sums of the earlier warps (part_*)
     auto before = [&](u64 &w, uint32_t &c) {
         u64 pw = lane < warp ? sh.part_w[lane] : 0;
@@ -272,42 +293,34 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
         w += __shfl_sync(~0u, pw, 0);
         c += __shfl_sync(~0u, pc, 0);
     };
-    // the row's running sums over the bins, the same in every CTA
+    // the bins' groups of 32 and the row's running sums over them, the same in every CTA
     auto merge = [&]() {
-        sync();
-        // this CTA adds up its share of the bins and tells all; nc lanes a bin, each with
-        // one CTA's, so that the remote reads are under way together
-        const int per = SR_THREADS / nc, q = tid & (nc - 1);
-        SrShared *o = cl.map_shared_rank(&sh, q);
-        for (int j = tid / nc; j < SR_BINS / nc; j += per) {
-            const int b = rank * (SR_BINS / nc) + j;
-            u64 w = o->bin.w[b];
-            uint32_t c = use_k ? o->bin.c[b] : 0;
-            for (int d = nc / 2; d; d /= 2) {
-                w += __shfl_xor_sync(~0u, w, d);
-                c += __shfl_xor_sync(~0u, c, d);
-            }
-            o->run_w[b] = w;
-            o->run_c[b] = c;
-        }
-        sync();
-        u64 w0 = sh.run_w[2 * tid], w1 = sh.run_w[2 * tid + 1], w = w0 + w1;
-        uint32_t c0 = sh.run_c[2 * tid], c1 = sh.run_c[2 * tid + 1], c = c0 + c1;
-        const u64 mw = w;
-        const uint32_t mc = c;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const u64 vw = __shfl_up_sync(~0u, w, o);
-            const uint32_t vc = __shfl_up_sync(~0u, c, o);
-            if (lane >= o) { w += vw; c += vc; }
-        }
-        if (lane == 31) { sh.part_w[warp] = w; sh.part_c[warp] = c; }
         __syncthreads();
-        before(w, c);
-        sh.run_w[2 * tid] = w - mw + w0;
-        sh.run_c[2 * tid] = c - mc + c0;
-        sh.run_w[2 * tid + 1] = w;
-        sh.run_c[2 * tid + 1] = c;
+        for (int g = warp; g < 32; g += SR_WARPS) {
+            u64 w = sh.bin.w[32 * g + lane];
+            uint32_t c = use_k ? sh.bin.c[32 * g + lane] : 0;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
+                w += __shfl_xor_sync(~0u, w, o);
+                c += __shfl_xor_sync(~0u, c, o);
+            }
+            if (lane == 0) { sh.group.w[g] = w; sh.group.c[g] = c; }
+        }
+        sync();
+        if (warp == 0) {
+            u64 w = 0;
+            uint32_t c = 0;
+#pragma unroll
+            for (int q = 0; q < SR_MAX_CLUSTER; q++)
+                if (q < nc) {
+                    const SrShared *o = cl.map_shared_rank(&sh, q);
+                    w += o->group.w[lane];
+                    c += o->group.c[lane];
+                }
+            warp_run(w, c);
+            sh.run_w[lane] = w;
+            sh.run_c[lane] = c;
+        }
         __syncthreads();
     };
 
@@ -349,35 +362,52 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
         top_valid = true;
     };
     // the bin in which the running sum, before_* at the first one's start, reaches the
-    // target (the last bin, should it reach it nowhere), and, for level 0, its keys
-    uint32_t k_first = 0, k_last = SR_LAST_KEY;
-    auto bin_at = [&](u64 target, bool count, u64 before_w, u64 before_c, bool bounds) {
-        if (tid == 0) sh.bin_at = SR_BINS - 1;
-        __syncthreads();
-        for (int j = tid; j < SR_BINS; j += SR_THREADS) {
-            const u64 s = count ? before_c + sh.run_c[j] : before_w + sh.run_w[j];
-            const u64 s0 = j == 0 ? (count ? before_c : before_w)
-                                  : (count ? before_c + sh.run_c[j - 1] : before_w + sh.run_w[j - 1]);
-            if (s >= target && s0 < target) sh.bin_at = j;
+    // target (the last bin, should it reach it nowhere): its group, then the bin in it;
+    // before_* become the sums at its start
+    auto bin_at = [&](u64 target, bool count, u64 &before_w, u64 &before_c) {
+        if (warp == 0) {
+            unsigned in = __ballot_sync(~0u, (count ? before_c + sh.run_c[lane] : before_w + sh.run_w[lane]) >= target);
+            const int g = in ? __ffs(in) - 1 : 31;
+            u64 w0 = 0, w;
+            uint32_t c0 = 0, c;
+#pragma unroll
+            for (int q = 0; q < SR_MAX_CLUSTER; q++)
+                if (q < nc) {
+                    const SrShared *o = cl.map_shared_rank(&sh, q);
+                    w0 += o->bin.w[32 * g + lane];
+                    c0 += use_k ? o->bin.c[32 * g + lane] : 0;
+                }
+            w = w0;
+            c = c0;
+            warp_run(w, c);
+            const u64 bw = before_w + (g ? sh.run_w[g - 1] : 0) + w, bc = before_c + (g ? sh.run_c[g - 1] : 0) + c;
+            in = __ballot_sync(~0u, (count ? bc : bw) >= target);
+            if (lane == (in ? __ffs(in) - 1 : 31)) {
+                sh.bin_at = 32 * g + lane;
+                sh.at_w = bw - w0;
+                sh.at_c = bc - c0;
+                sh.to_c = (uint32_t)bc;
+            }
         }
         __syncthreads();
-        const int at = sh.bin_at;
-        if (bounds) {
-            k_first = sr_bin_start(R.mx, top, at, lane);
-            k_last = at < SR_BINS - 1 ? sr_bin_start(R.mx, top, at + 1, lane) - 1 : SR_LAST_KEY;
-        }
-        return at;
+        before_w = sh.at_w;
+        before_c = sh.at_c;
+        return sh.bin_at;
     };
-    // tokens with a key in [k0, k1] and an index in [j0, j1] to the
+    // the distances in a bin of level 0
+    auto bin_distances = [&](int at, float &d0, float &d1) {
+        d0 = sr_bin_distance(top, at, lane);
+        d1 = INFINITY;
+        if (at < SR_BINS - 1) d1 = __uint_as_float(__float_as_uint(sr_bin_distance(top, at + 1, lane)) - 1);
+    };
+    // tokens with base - logit in [d0, d1] and an index in [j0, j1] to the
     // first CTA's list; their number, list_n, may be more than the list holds
     int turn = 0;
-    auto gather = [&](uint32_t k0, uint32_t k1, int j0, int j1) {
+    auto gather = [&](float base, float d0, float d1, int j0, int j1) {
         // (the list's place was last read before a sync that all have passed; so was the
         // other counter, which is made ready for the next time)
         SrShared *first = cl.map_shared_rank(&sh, 0);
         if (rank == 0 && tid == 0) sh.list_n[turn ^ 1] = 0;
-        // (as numbers, -0 would let +0 in)
-        const float d1 = sr_key_logit(k0 == 0x80000000u ? 0x80000001u : k0), d0 = sr_key_logit(k1);
         auto push = [&](float l, int i) {
             if (i < j0 || i > j1) return;
             const int e = atomicAdd(&first->list_n[turn], 1);
@@ -387,31 +417,34 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
             }
         };
         for (int i = tid; i < n4; i += SR_THREADS) {
-            const float4 v = val4[i];
+            float4 v = val4[i];
+            v.x = base - v.x; v.y = base - v.y; v.z = base - v.z; v.w = base - v.w;
             int in = (v.x >= d0 && v.x <= d1) | (v.y >= d0 && v.y <= d1) << 1 | (v.z >= d0 && v.z <= d1) << 2 |
                      (v.w >= d0 && v.w <= d1) << 3;
             for (; in; in &= in - 1) {    // mostly none
                 const int e = __ffs(in) - 1;
-                push(e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w, i0 + 4 * i + e);
+                push(val[4 * i + e], i0 + 4 * i + e);
             }
         }
         for (int i = 4 * n4 + tid; i < n; i += SR_THREADS)
-            if (val[i] >= d0 && val[i] <= d1) push(val[i], i0 + i);
+            if (base - val[i] >= d0 && base - val[i] <= d1) push(val[i], i0 + i);
         sync();
         turn ^= 1;
     };
     // in the first CTA: which of the list's tokens takes the running sum to target; all
     // CTAs learn its key and the running weight
-    auto resolve = [&](int tokens, u64 target, bool count, u64 before_w, u64 before_c, uint32_t k0, uint32_t k1) {
+    auto resolve = [&](int tokens, u64 target, bool count, u64 before_w, u64 before_c, float base, float d0, float d1,
+                       bool ties, bool last) {
         int m = tokens;
         if (tokens > SR_FEW) {
-            // finer bins, by key or, among equal keys, by index
-            const bool ties = k0 == k1;
-            const uint32_t width = ties ? (uint32_t)a.vocab - 1 : k1 - k0;
+            // finer bins, by distance or, among equal logits, by index (a product of zero and
+            // infinity, d1's, goes to the last bin)
+            const float sub = (float)SR_SUB / (d1 - d0);
             int shift = 0;
-            while ((width >> shift) >= SR_SUB) shift++;
+            while (((uint32_t)(a.vocab - 1) >> shift) >= SR_SUB) shift++;
             auto sub_of = [&](u64 key) {
-                return (int)((ties ? (uint32_t)key : (uint32_t)(key >> 32) - k0) >> shift);
+                const float d = base - sr_key_logit((uint32_t)(key >> 32));
+                return ties ? (int)((uint32_t)key >> shift) : (int)fminf((d - d0) * sub, (float)(SR_SUB - 1));
             };
             sh.sub_w[tid] = 0;
             sh.sub_c[tid] = 0;
@@ -427,12 +460,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
             const uint32_t mc = sh.sub_c[tid];
             u64 w = mw;
             uint32_t c = mc;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const u64 vw = __shfl_up_sync(~0u, w, o);
-                const uint32_t vc = __shfl_up_sync(~0u, c, o);
-                if (lane >= o) { w += vw; c += vc; }
-            }
+            warp_run(w, c);
             if (lane == 31) { sh.part_w[warp] = w; sh.part_c[warp] = c; }
             __syncthreads();
             before(w, c);
@@ -461,15 +489,16 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
                 if (sh.list.key[sh.few[j]] < key) { w += sh.list.w[sh.few[j]]; c++; }
             const u64 s0 = count ? c : w, s = count ? c + 1 : w + sh.list.w[i];
             if (s0 < target && s >= target)
-                for (int q = 0; q < nc; q++) {
+                for (int q = 0; q < (last ? 1 : nc); q++) {
                     SrShared *o = cl.map_shared_rank(&sh, q);
                     o->res_key = key;
                     o->res_w = w + sh.list.w[i];
                 }
         }
     };
-    // the first place in the order where the running sum reaches target
-    auto find = [&](u64 target, bool count) {
+    // the first place in the order where the running sum reaches target; the last search's
+    // result is the first CTA's alone, the others are done
+    auto find = [&](u64 target, bool count, bool last) {
         u64 before_w = 0, before_c = 0;
         // the part of the row that is binned: level 0, all by distance; 1, keys in
         // [k0, k1]; 2, one key, by index. Each level's bin is a 1/512 of its range at most,
@@ -477,25 +506,35 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
         uint32_t k0 = 0, k1 = SR_LAST_KEY;
         int level = 0, shift = 0, j0 = 0, j1 = 0x7FFFFFFF;
         for (;;) {
-            const int at = bin_at(target, count, before_w, before_c, level == 0);
-            before_w += at ? sh.run_w[at - 1] : 0;
-            before_c += at ? sh.run_c[at - 1] : 0;
+            const int at = bin_at(target, count, before_w, before_c);
+            float base = 0.0f, d0, d1;
             if (level == 0) {
-                k0 = k_first;
-                k1 = k_last;
-            } else if (level == 1) {
-                k1 = (uint32_t)min((long long)k1, k0 + ((at + 1ll) << shift) - 1);
-                k0 += (uint32_t)at << shift;
+                base = R.mx;
+                bin_distances(at, d0, d1);
             } else {
-                j1 = min((long long)j1, j0 + ((at + 1ll) << shift) - 1);
-                j0 += at << shift;
+                if (level == 1) {
+                    k1 = (uint32_t)min((long long)k1, k0 + ((at + 1ll) << shift) - 1);
+                    k0 += (uint32_t)at << shift;
+                } else {
+                    j1 = min((long long)j1, j0 + ((at + 1ll) << shift) - 1);
+                    j0 += at << shift;
+                }
+                // (as numbers, -0 would let +0 in)
+                d0 = 0.0f - sr_key_logit(k0 == 0x80000000u ? 0x80000001u : k0);
+                d1 = 0.0f - sr_key_logit(k1);
             }
-            gather(k0, k1, j0, j1);
+            gather(base, d0, d1, j0, j1);
             const int tokens = cl.map_shared_rank(&sh, 0)->list_n[turn ^ 1];
             if (tokens <= SR_LIST) {
-                if (rank == 0) resolve(tokens, target, count, before_w, before_c, k0, k1);
-                sync();
+                if (last) sync();         // all have read the number: they may leave
+                if (rank == 0) resolve(tokens, target, count, before_w, before_c, base, d0, d1, level && k0 == k1, last);
+                if (!last) sync();
+                else __syncthreads();
                 return SrFound{sh.res_key, sh.res_w};
+            }
+            if (level == 0) {
+                k0 = sr_bin_start(R.mx, top, at, lane);
+                k1 = at < SR_BINS - 1 ? sr_bin_start(R.mx, top, at + 1, lane) - 1 : SR_LAST_KEY;
             }
             if (k0 == k1 && level != 2) { j0 = 0; j1 = a.vocab - 1; }
             level = k0 == k1 ? 2 : 1;
@@ -522,11 +561,13 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
         u64 target = (u64)top_k;
         if (stage == 0) {
             // no weights beyond the last of the k: binned by tokens alone
-            const int at = bin_at(target, true, 0, 0, true);
-            const int tokens = (int)sh.run_c[at];
+            u64 w = 0, c = 0;
+            float d0, d1;
+            bin_distances(bin_at(target, true, w, c), d0, d1);
+            const int tokens = (int)sh.to_c;
             if (tokens <= SR_LIST) {
                 // they and the rest of their bin fit the list: the first CTA does the rest
-                gather(sr_key(R.mx), k_last, 0, 0x7FFFFFFF);
+                gather(R.mx, 0.0f, d1, 0, 0x7FFFFFFF);
                 if (rank != 0) return;
                 constexpr int Q = (SR_LIST + SR_THREADS - 1) / SR_THREADS;
                 u64 mine[Q], sum = 0;
@@ -560,10 +601,10 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
                 return;
             }
         } else if (stage == 1) {
-            const u64 total = sh.run_w[SR_BINS - 1];
+            const u64 total = sh.run_w[31];
             target = max(1ull, min((u64)ceil((double)top_p * (double)total), total));
         } else if (stage == 3) {
-            kept = min(kept, sh.run_w[SR_BINS - 1]);
+            kept = min(kept, sh.run_w[31]);
             if (use_min) {
                 // the weight of what min_p keeps, over the cluster
 #pragma unroll
@@ -582,7 +623,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
             }
             target = min((u64)((u > 0.0f ? (double)fminf(u, 1.0f) : 0.0) * (double)kept), kept - 1) + 1;
         }
-        const SrFound f = find(target, stage == 0 || stage == 2);
+        const SrFound f = find(target, stage == 0 || stage == 2, stage == 3);
         if (stage == 0) {
             weigh_to = fminf(weigh_to, R.mx - sr_key_logit((uint32_t)(f.key >> 32)));
             top = binning(weigh_to);
