@@ -334,18 +334,41 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
         in_min = 0;
         if (need_total) {
             // every token has its weight, one beyond the limit 0: no branch but those that
-            // all lanes take alike
+            // all lanes take alike. The additions of four tokens come after their weights:
+            // an atomic between them would hold back the next one's table entry, and the
+            // upper words need what the lower ones returned.
             const double mx = (double)R.mx;
-            each([&](float l, int) {
+            auto weigh = [&](float l, int &b) {
                 const float d = R.mx - l;
                 const bool on = d <= R.limit;
                 const double e = sr_exp2_64((mx - (double)(on ? l : R.mx)) * R.slope, sh.pow2);
                 const u64 w = on ? sr_units(e) : 0;
-                const int b = sr_bin(top, d);
+                b = sr_bin(top, d);
                 if (use_min && e >= (double)min_p) in_min += w;
+                return w;
+            };
+            for (int i = tid; i < n4; i += SR_THREADS) {
+                const float4 v = val4[i];
+                int b[4];
+                const u64 w[4] = {weigh(v.x, b[0]), weigh(v.y, b[1]), weigh(v.z, b[2]), weigh(v.w, b[3])};
+                uint32_t old[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    if (use_k) atomicAdd(&sh.bin.c[b[k]], 1u);
+                    old[k] = atomicAdd(reinterpret_cast<uint32_t *>(&sh.bin.w[b[k]]), (uint32_t)w[k]);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t up = (uint32_t)(w[k] >> 32) + (old[k] + (uint32_t)w[k] < old[k] ? 1u : 0u);
+                    if (up) atomicAdd(reinterpret_cast<uint32_t *>(&sh.bin.w[b[k]]) + 1, up);
+                }
+            }
+            for (int i = 4 * n4 + tid; i < n; i += SR_THREADS) {
+                int b;
+                const u64 w = weigh(val[i], b);
                 if (use_k) atomicAdd(&sh.bin.c[b], 1u);
                 sr_add(&sh.bin.w[b], w);
-            });
+            }
         } else {
             each([&](float l, int) {
                 const float d = R.mx - l;
