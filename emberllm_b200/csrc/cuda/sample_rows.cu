@@ -13,10 +13,14 @@
 // additions can change a token.
 //
 // A cluster of CTAs holds the row in shared memory, so the logits are read once;
-// they exchange maxima, bins and lists through distributed shared memory. Bound by
-// the exponentials (11 double-precision operations a token: the draw compares sums
-// of up to 393,216 weights, and a token next to a border must not change) and the
-// shared-memory atomics, not by memory.
+// they exchange maxima, bins and lists through distributed shared memory: each adds up
+// its own bins by groups of 32, and who looks for a target reads the groups, then the
+// bins of one group, of all. Bound by instructions, 97 a token and lane at half of the
+// issue slots: the weight (11 double-precision operations: the draw compares sums of
+// up to 393,216 weights, and a token next to a border must not change), its bin and
+// the atomic additions; memory would take 48 us of the 413 us for 512 rows of 151,936
+// (64 rows with truncations 76 us, one of 32,000 12 us with the call). With the running
+// sums over all bins in every CTA it took 454 us.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
