@@ -15,19 +15,20 @@
 //   2 values, 4 (1) keys   packed codes from global memory, asked for a tile ahead, to
 //        exact fp16 numbers (code - 8) * d in shared memory, swizzled as the products read
 //        them; the values are transposed on the way, so both operands are K-major
-// fp32 queries and weights enter as an fp16 rounding and its rest (two products into
-// the same sums, 22 bits); fp16 queries are exact as they are, and their weights are
-// rounded to 11 bits (measured: error 2.6e-4 of the outputs, 2.0e-4 by their own
-// rounding alone). Each product cuts the sum it adds to toward zero at 24 bits, two for 16
-// positions in fp32: outputs are off by 2.3e-9 of themselves a position (measured 3e-7 at
-// 100, 2.9e-6 at 1200, 9.4e-6 at 4000). Sums taken out of tensor memory every 2048
-// positions halve that at 4000 and bound it behind, but cost 13 to 16 % there and 4 % at
+// Weights and fp32 queries enter as an fp16 number and the rest (two products into
+// the same sums, 22 bits); fp16 queries are exact as they are. (Weights of 11 bits for fp16
+// outputs took 201 us instead of 247 for two prompts of 4k, but moved 40 % of the outputs to a
+// neighbouring number: error 2.6e-4, where the outputs' own rounding is 2.0e-4.) Each
+// product cuts the sum it adds to toward zero at 24 bits, two for 16 positions: outputs
+// are off by 2.3e-9 of themselves a position (measured 3e-7 at 100, 2.9e-6 at 1200, 9.4e-6 at
+// 4000). Sums taken out of tensor memory every 2048 positions halve that at 4000 and
+// bound it behind, but cost 13 to 16 % there and 4 % at
 // 1200.
 //
 // Bound by the chain scores - maximum - exponentials - weights - outputs of a row tile: tensor
 // pipe, exponentials and conversions are each busy a third of the time. Two prompts of 3.9-4.1k,
-// 16 / 8 heads of 128, fp16: 201 us, 674 TFLOP/s; six of up to 512 rows on up to 1200
-// positions, fp32: 60 us.
+// 16 / 8 heads of 128, fp16: 247 us, 549 TFLOP/s; six of up to 512 rows on up to 1200
+// positions, fp32: 55 us.
 #pragma once
 
 #include "kv4_attn.cuh"
@@ -39,7 +40,7 @@ constexpr unsigned long long KP_WAIT_NS = 1000000000ull;
 
 template <typename T, int HD, int RT>
 struct KpLayout {
-    static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;    // fp16 parts of a query and of a weight
+    static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;    // fp16 parts of a query (a weight has two)
     static constexpr int NP = 64 * RT, H = NP / 64;         // positions of a tile, and its halves of 64
     static constexpr int SB = 3 - RT;                       // tiles of scores per row tile in tensor memory
     static constexpr int BUF = PARTS == 2 ? 1 : 2;          // tiles of keys and of values in shared memory
@@ -139,6 +140,11 @@ EMB_DEV void kp_st16(uint32_t ta, const uint32_t (&u)[16]) {
         : "memory");
 }
 EMB_DEV void kp_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// a weight's first 11 bits: an fp16 number, as long as that is a normal one (the weights that
+// matter are: a row's largest is 2^6 or more). Cheaper than the rounding, which has to be widened
+// again to get the rest: no spills, 281 -> 247 us for two prompts of 4k in fp16
+EMB_DEV float kp_cut(float e) { return __uint_as_float(__float_as_uint(e) & 0xFFFFE000u); }
 
 // the lower (1024 + c) and upper (1024 + 16 c) nibbles' exact (code - 8) * d
 EMB_DEV uint32_t kp_low(uint32_t w, __half2 d) {
@@ -399,7 +405,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
             const float base = m == -INFINITY ? 0.0f : m - 6.0f;
             float sum[2] = {0.0f, 0.0f};
             // the last half is still in registers; a half's weights take its scores' place,
-            // first the roundings, then the rests
+            // first the 11 bits, then the rests
 #pragma unroll 1
             for (int h = H - 1; h >= 0; h--) {
                 if (h < H - 1) read(h);
@@ -412,14 +418,12 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
                         const float e1 = kv4_exp2(fmaf(v[i * 32 + 2 * k + 1], rs, -base));
                         sum[0] += e0;
                         sum[1] += e1;
-                        hi[k] = pack_half2(e0, e1);
-                        if (PARTS == 2) {
-                            const float2 q = __half22float2(bits_h2(hi[k]));
-                            lo[k] = pack_half2(e0 - q.x, e1 - q.y);
-                        }
+                        const float h0 = kp_cut(e0), h1 = kp_cut(e1);
+                        hi[k] = pack_half2(h0, h1);
+                        lo[k] = pack_half2(e0 - h0, e1 - h1);
                     }
                     kp_st16(at + h * 64 + i * 16, hi);
-                    if (PARTS == 2) kp_st16(at + h * 64 + 32 + i * 16, lo);
+                    kp_st16(at + h * 64 + 32 + i * 16, lo);
                 }
                 kp_wait_st();
                 kp_fence_before();
@@ -485,7 +489,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
                     kp_fence_after();
                     if (kp_elect()) {
 #pragma unroll
-                        for (int q = 0; q < PARTS; q++)
+                        for (int q = 0; q < 2; q++)
 #pragma unroll
                             for (int k = 0; k < 4; k++)
                                 kp_mma_ts(o, p + h * 64 + q * 32 + k * 8, v + ((h * L::V_PANEL + k * 32) >> 4), idesc_o,

@@ -94,9 +94,8 @@ int ember_cuda_kv4_read(const EmberKv4Cache *cache, const EmberKv4Batch *batch, 
  * makes that (row, head)'s output NaN and no other.
  *
  * Arithmetic: the queries enter the products in 22 significant bits relative to
- * the row's largest element, the softmax weights in 22 bits (fp16 outputs of
- * many-row calls: 11 bits); scores, maxima, sums and outputs accumulate in fp32.
- * Many-row calls (prompts) add on the
+ * the row's largest element, the softmax weights in 22 bits; scores, maxima, sums
+ * and outputs accumulate in fp32. Many-row calls (prompts) add on the
  * tensor cores, which cut toward zero: about 2.3e-9 of an output a position in fp32.
  * The same call gives the same bits. A row's result does not depend on its
  * neighbours in the batch; in the last bits it depends on how the cache is cut into

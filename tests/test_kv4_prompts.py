@@ -1,0 +1,34 @@
+"""Attention of many rows over the paged 4-bit cache: how exact its sums are, beyond
+the worst-case bounds of test_kv4.py."""
+import pytest
+
+from .test_kv4 import Paged
+
+torch = pytest.importorskip("torch")
+
+
+def queries(n, heads, hd, seed=1, scale=1.2, dtype=torch.float32):
+    return (torch.randn(n, heads, hd, generator=torch.Generator().manual_seed(seed)) * scale).to(dtype).cuda()
+
+
+def relative(got, want):
+    return ((got.double() - want).norm() / want.norm()).item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kvh,hd,seqs", [(16, 8, 128, 2), (16, 8, 128, 1), (12, 12, 64, 2), (9, 3, 64, 1), (8, 1, 32, 3)])
+def test_half_precision_outputs_are_rounded_once(heads, kvh, hd, seqs):
+    """fp16 outputs are the exact ones rounded, but for those next to a border of two
+    numbers. Before that rounding an output is off by r of itself: the scores' products
+    (at most 8 cuts at 24 bits of sums of a few units: 2e-6), the weights in 22 bits
+    (2.4e-7), their sums over 900 positions (2.3e-9 each: 2e-6), which is less than
+    r = 2e-5. An output moves across a border of numbers 2^-11 apart with the chance
+    r / 2^-11, three times that for the small ones among them: 3 %. (Weights of 11 bits
+    move 40 % of the outputs.)"""
+    p = Paged([900 - 7 * i for i in range(seqs)], [900 - 7 * i for i in range(seqs)], 64, kvh, hd, seed=hd)
+    p.store_all()
+    q = queries(sum(p.ql), heads, hd, dtype=torch.float16)
+    got, want = p.attend(q), p.want(q)
+    once = want.half()
+    assert (got != once).double().mean().item() < 0.03
+    assert relative(got, want) < 1.01 * relative(once, want)
