@@ -372,7 +372,8 @@ __global__ void __launch_bounds__(KD_THREADS, KdLayout<HD, NT>::CTAS) kv4_decode
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                const float mn = fmaxf(m[nt], mx);
+                // (a row that did not pass its own stays as it is: its bits are its own affair)
+                const float mn = mx > m[nt] + 8.0f ? mx : m[nt];
                 const float f = mn == m[nt] ? 1.0f : kv4_exp2(m[nt] - mn);
                 m[nt] = mn;
                 l[nt] *= f;

@@ -371,7 +371,8 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
             }
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * rs;
             if (__any_sync(0xffffffffu, top > m + 8.0f)) {
-                const float mn = fmaxf(m, top);
+                // (a row that did not pass its own stays as it is: its bits are its own affair)
+                const float mn = top > m + 8.0f ? top : m;
                 const float f = mn == m ? 1.0f : kv4_exp2(m - mn);
                 m = mn;
                 l *= f;
