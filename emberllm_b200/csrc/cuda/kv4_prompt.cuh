@@ -17,18 +17,21 @@
 //        them; the values are transposed on the way, so both operands are K-major
 // Weights and fp32 queries enter as an fp16 number and the rest (two products into
 // the same sums, 22 bits); fp16 queries are exact as they are. (Weights of 11 bits for fp16
-// outputs took 201 us instead of 247 for two prompts of 4k, but moved 40 % of the outputs to a
+// outputs took 201 us instead of 246 for two prompts of 4k, but moved 40 % of the outputs to a
 // neighbouring number: error 2.6e-4, where the outputs' own rounding is 2.0e-4.) Each
-// product cuts the sum it adds to toward zero at 24 bits, two for 16 positions: outputs
-// are off by 2.3e-9 of themselves a position (measured 3e-7 at 100, 2.9e-6 at 1200, 9.4e-6 at
-// 4000). Sums taken out of tensor memory every 2048 positions halve that at 4000 and
-// bound it behind, but cost 13 to 16 % there and 4 % at
-// 1200.
+// product cuts the sum it adds to toward zero at 24 bits, two for 16 positions: sums
+// are off by 2.5e-9 of themselves a position. So those of fp32 outputs leave tensor memory
+// every 512 positions and are added up by rounding additions: 1.6e-6 of the outputs at any length.
+// Us and error, staying / every 2048 / 1024 / 512 / 256 positions: two prompts of 4k 276, 9.9e-6 /
+// 287, 5.2e-6 / 304, 2.8e-6 / 321, 1.6e-6 / 356, 1.0e-6; 512 rows of 40,000 1170, 9.4e-5 / 1184,
+// 5.2e-6 / 1210, 2.8e-6 / 1262, 1.6e-6 / 1369, 1.1e-6; six ragged prompts 54, 1.3e-6 / 54 / 60 / 63,
+// 9e-7 / 68, 6.5e-7 (in plain fp32 operations 4.5e-7). Those of fp16 outputs stay: 9.4e-5 of an
+// output at 40,000 positions, half a step is 2.4e-4 and more.
 //
 // Bound by the chain scores - maximum - exponentials - weights - outputs of a row tile: tensor
 // pipe, exponentials and conversions are each busy a third of the time. Two prompts of 3.9-4.1k,
-// 16 / 8 heads of 128, fp16: 247 us, 549 TFLOP/s; six of up to 512 rows on up to 1200
-// positions, fp32: 55 us.
+// 16 / 8 heads of 128, fp16: 246 us, 552 TFLOP/s; six of up to 512 rows on up to 1200
+// positions, fp32: 63 us.
 #pragma once
 
 #include "kv4_attn.cuh"
@@ -36,6 +39,7 @@
 namespace emb {
 
 constexpr int KP_ROWS = 128;
+constexpr int KP_DRAIN = 512;             // positions whose sums stay in tensor memory (fp32)
 constexpr unsigned long long KP_WAIT_NS = 1000000000ull;
 
 template <typename T, int HD, int RT>
@@ -54,6 +58,8 @@ struct KpLayout {
     static constexpr int COLS = RT * 256, COL_O = RT * 128;
     static constexpr int SOFT = 4 * RT, ISSUE = SOFT, VALS = SOFT + RT, KEYS = VALS + 2;   // first warps of the roles
     static constexpr int KEY_WARPS = RT == 2 ? 4 : 1, WARPS = RT == 2 ? 16 : 8;
+    // tiles after which the sums leave tensor memory
+    static constexpr int DRAIN = KP_DRAIN / NP;
     static constexpr int KN = NP / 8 / KEY_WARPS;           // positions a key thread unpacks
     static_assert(SB * NP == 128, "scores take 128 columns");
     static_assert(SMEM <= (RT == 2 ? 227 : 113) * 1024, "shared memory");
@@ -143,7 +149,7 @@ EMB_DEV void kp_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "m
 
 // a weight's first 11 bits: an fp16 number, as long as that is a normal one (the weights that
 // matter are: a row's largest is 2^6 or more). Cheaper than the rounding, which has to be widened
-// again to get the rest: no spills, 281 -> 247 us for two prompts of 4k in fp16
+// again to get the rest: no spills, 281 -> 246 us for two prompts of 4k in fp16
 EMB_DEV float kp_cut(float e) { return __uint_as_float(__float_as_uint(e) & 0xFFFFE000u); }
 
 // the lower (1024 + c) and upper (1024 + 16 c) nibbles' exact (code - 8) * d
@@ -326,10 +332,84 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
         const int first_pos = pos0 + min(row_first + rt * KP_ROWS, rows - 1) / a.group;
         const int last_pos = pos0 + (min(rows, row_first + (rt + 1) * KP_ROWS) - 1) / a.group;
         const long long all_from = a.window > 0 ? (long long)last_pos - a.window + 1 : 0;
-        float m = -INFINITY, l = 0.0f;
+        float m = -INFINITY, l = 0.0f, m_out = -INFINITY;
         bool ok = true;
         const int todo = rt < tiles ? n : 0;
+        // The sums in tensor memory added to those of earlier tiles, which are kept in the warp's
+        // own 32 rows of `out`, scaled by 2^-m_out; `last`: all of them back to tensor memory.
+        // Lane r keeps its four numbers number k at place 32 k + r of the rows' numbers in a
+        // row, so that the lanes' places are neighbours (in its own row, a warp's access touched 32 rows:
+        // 4.9 us a time); a warp with fewer rows keeps them in its own.
+        constexpr bool TAKE = sizeof(T) == 4;
+        auto drain = [&](bool more, bool last) {
+            constexpr int Q = HD / 4;
+            const bool whole = row_first + (warp + 1) * 32 <= rows, mine_too = whole || rr < rows;
+            const int row = min(rr, rows - 1), tok = row / a.group;
+            const int64_t my_off = (int64_t)(s.row0 + tok) * a.out_tok + (kv * a.group + row - tok * a.group) * a.out_head;
+            const bool vec = !((uintptr_t)a.out % 16 || a.out_tok % 4 || a.out_head % 4);
+            // (m == m_out: nothing to scale, the addition can be left to the memory)
+            const float f = m == m_out ? 1.0f : kv4_exp2(m_out - m);
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+                float o[32], w[32];
+                float *at[8];
+#pragma unroll
+                for (int k = 0; k < 32; k += 4) {
+                    const int place = ((c + k) / 4) * 32 + lane;
+                    const int64_t off = __shfl_sync(0xffffffffu, my_off, whole ? place / Q : lane);
+                    at[k / 4] = reinterpret_cast<float *>(a.out) + off + (whole ? place % Q * 4 : c + k);
+                    w[k] = w[k + 1] = w[k + 2] = w[k + 3] = 0.0f;
+                    if (!mine_too || !more || (f == 1.0f && !last)) continue;
+                    if (vec) {
+                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(at[k / 4]));
+                        w[k] = x.x; w[k + 1] = x.y; w[k + 2] = x.z; w[k + 3] = x.w;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) w[k + e] = __ldcg(at[k / 4] + e);
+                    }
+                }
+                kp_ld32<0>(o, col_o + c);
+#pragma unroll
+                for (int k = 0; k < 32; k++) o[k] = fmaf(w[k], f, o[k]);
+                if (last) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t u[16];
+#pragma unroll
+                        for (int k = 0; k < 16; k++) u[k] = __float_as_uint(o[16 * h + k]);
+                        kp_st16(col_o + c + 16 * h, u);
+                    }
+                } else if (mine_too) {
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4) {
+                        float *p = at[k / 4];
+                        if (vec && more && f == 1.0f)
+                            asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(o[k]),
+                                         "f"(o[k + 1]), "f"(o[k + 2]), "f"(o[k + 3])
+                                         : "memory");
+                        else if (vec) *reinterpret_cast<float4 *>(p) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                        else
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                if (more && f == 1.0f) atomicAdd(p + e, o[k + e]);
+                                else p[e] = o[k + e];
+                    }
+                }
+                __syncwarp();
+            }
+            if (last) kp_wait_st();
+            __syncwarp();
+            m_out = m;
+        };
         for (int j = 0; j < todo; j++) {
+            const bool fresh = TAKE ? j % L::DRAIN == 0 : j == 0;      // nothing in O that counts
+            if (TAKE && fresh && j > 0) {
+                ok = kp_wait(&sh.o_done[rt], (j - 1) & 1, abort);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                kp_fence_after();
+                drain(j > L::DRAIN, false);
+            }
             ok = kp_wait(&sh.s_full[rt][j % SB], (j / SB) & 1, abort);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
@@ -376,7 +456,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
                 const float f = mn == m ? 1.0f : kv4_exp2(m - mn);
                 m = mn;
                 l *= f;
-                if (j > 0) {
+                if (!fresh) {
                     ok = kp_wait(&sh.o_done[rt], (j - 1) & 1, abort);    // the products into O so far
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
@@ -437,6 +517,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
             ok = kp_wait(&sh.o_last[rt], 0, abort);
             ok = __all_sync(0xffffffffu, ok);
             kp_fence_after();
+            if (TAKE && ok && todo > L::DRAIN) drain(true, true);
         }
         const bool live = rr < rows;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -494,7 +575,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
 #pragma unroll
                             for (int k = 0; k < 4; k++)
                                 kp_mma_ts(o, p + h * 64 + q * 32 + k * 8, v + ((h * L::V_PANEL + k * 32) >> 4), idesc_o,
-                                          j > 0 || h < H - 1 || q + k > 0);
+                                          (sizeof(T) == 4 ? j % L::DRAIN : j) > 0 || h < H - 1 || q + k > 0);
                         if (h == 0) {
                             kp_commit(&sh.o_done[rt]);
                             kp_commit(&sh.v_empty[j % BUF]);

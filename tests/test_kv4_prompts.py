@@ -32,3 +32,28 @@ def test_half_precision_outputs_are_rounded_once(heads, kvh, hd, seqs):
     once = want.half()
     assert (got != once).double().mean().item() < 0.03
     assert relative(got, want) < 1.01 * relative(once, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv,ql,heads,kvh,hd,window,sinks", [
+    ([1200, 700], [1200, 700], 16, 8, 128, 0, 0),
+    ([20000], [300], 16, 8, 128, 0, 0), ([41000], [270], 16, 8, 128, 0, 0),
+    ([3001], [3001], 12, 12, 64, 0, 0), ([9000, 520], [1300, 513], 9, 3, 64, 0, 0), ([6000] * 3, [400] * 3, 8, 1, 32, 0, 0),
+    ([9000], [300], 16, 8, 128, 5000, 700)])
+def test_single_precision_sums_at_any_length(kv, ql, heads, kvh, hd, window, sinks):
+    """The tensor cores cut a running sum at 24 bits, twice for 16 positions: 64 times
+    before it leaves them, half of 2^-23 of a sum that is on the average 2/3 of the
+    segment's: 2.5e-6. The scores' own cuts (16 of sums of a few units, of both
+    signs), 22 bits of queries and weights and the exponentials add less than 1.5e-6.
+    (Sums that stay are off by 4.8e-5 at 20,000 positions.)"""
+    p = Paged(kv, ql, 64, kvh, hd, seed=hd)
+    p.store_all()
+    q = queries(sum(ql), heads, hd)
+    got, want = p.attend(q, window, sinks), p.want(q, window, sinks)
+    assert relative(got, want) < 4e-6
+    # the partial sums lie in the outputs' rows: strides, offsets and what is beside them
+    n = sum(ql)
+    wide = torch.full((heads + 1, n, hd + 3), 5.0, device="cuda")
+    out = wide[1:, :, 3:].transpose(0, 1)
+    p.attend(q, window, sinks, out=out)
+    assert torch.equal(out, got) and (wide[0] == 5).all() and (wide[:, :, :3] == 5).all()
