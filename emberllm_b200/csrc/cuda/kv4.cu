@@ -7,6 +7,7 @@
 
 #include "kv4.cuh"
 #include "kv4_prompt.cuh"
+#include "kv4_rule.h"
 #include "runtime_internal.cuh"
 
 namespace emb {
@@ -252,19 +253,14 @@ __global__ void __launch_bounds__(KV4_IO_THREADS) kv4_io_kernel(Kv4View c, Kv4Ro
     }
 }
 
-// Few rows are taken eight at a time, the cache cut into pieces and read once for each
-// eight: 0.055 ns for eight rows and a position. Many are taken 128 at a time by CTAs that
-// go through the cache alone: 28 ns a position, as long as there are no more than 128 of
-// them. The smaller estimate decides. Measured, eight at a time / 128 at a time, in us,
-// 16 / 8 heads of 128, fp32: 1 sequence of 20,000 positions, 8 rows 16 / 544, 128 rows 125 / 548;
-// 8 sequences of 1000, 64 rows 34 / 38, 128 rows 65 / 40; 64 sequences of 1000, 16 rows 67 / 148,
-// 64 rows 231 / 164.
 template <typename T>
 static int kv4_attention_launch(const Kv4AttnArgs &a, int hd, cudaStream_t st) {
-    const long long rows = (long long)a.max_q * a.group, heads = (long long)a.b.n_seqs * a.c.n_kv;
-    const long long eights = (rows + 7) / 8 * heads, tiles = (rows + KP_ROWS - 1) / KP_ROWS * heads;
-    if (eights > 512 * (tiles > 128 ? tiles : 128) / 128) return kv4_prompt_hd<T>(a, hd, st);
-    return rows <= 4 ? kv4_decode_hd<T, 1>(a, hd, st) : kv4_decode_hd<T, 2>(a, hd, st);
+    switch (kv4_kernel(sizeof(T), a.max_q, a.group, a.c.n_kv, a.b.n_seqs)) {
+    case KV4_FEW_4: return kv4_decode_hd<T, 1>(a, hd, st);
+    case KV4_FEW_8: return kv4_decode_hd<T, 2>(a, hd, st);
+    case KV4_MANY_1: return kv4_prompt_hd<T, 1>(a, hd, st);
+    default: return kv4_prompt_hd<T, 2>(a, hd, st);
+    }
 }
 
 // ------------------------------------------------------------ host checks ----

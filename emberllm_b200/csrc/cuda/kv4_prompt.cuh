@@ -35,10 +35,11 @@
 #pragma once
 
 #include "kv4_attn.cuh"
+#include "kv4_rule.h"
 
 namespace emb {
 
-constexpr int KP_ROWS = 128;
+constexpr int KP_ROWS = KV4_TILE_ROWS;
 constexpr int KP_DRAIN = 512;             // positions whose sums stay in tensor memory (fp32)
 constexpr unsigned long long KP_WAIT_NS = 1000000000ull;
 
@@ -804,22 +805,12 @@ static int kv4_prompt_launch(const Kv4AttnArgs &a, cudaStream_t st) {
 }
 
 template <typename T, int RT>
-static int kv4_prompt_rt(const Kv4AttnArgs &a, int hd, cudaStream_t st) {
+static int kv4_prompt_hd(const Kv4AttnArgs &a, int hd, cudaStream_t st) {
     switch (hd) {
     case 32: return kv4_prompt_launch<T, 32, RT>(a, st);
     case 64: return kv4_prompt_launch<T, 64, RT>(a, st);
     default: return kv4_prompt_launch<T, 128, RT>(a, st);
     }
-}
-
-template <typename T>
-static int kv4_prompt_hd(const Kv4AttnArgs &a, int hd, cudaStream_t st) {
-    // Two row tiles a CTA once there are enough of them. Us, one / two (16 / 8 heads of 128):
-    //   32 pairs (512 rows of 2000)      fp32 67 / 80     fp16 61 / 52
-    //   128 pairs (4 x 512 of 1200)      fp32 65 / 59     fp16 54 / 40
-    //   250 pairs (4000 of 8000)         fp32 605 / 403   fp16 494 / 252
-    const long long pairs = ((long long)a.max_q * a.group + 2 * KP_ROWS - 1) / (2 * KP_ROWS) * a.c.n_kv * a.b.n_seqs;
-    return pairs >= (sizeof(T) == 4 ? 96 : 32) ? kv4_prompt_rt<T, 2>(a, hd, st) : kv4_prompt_rt<T, 1>(a, hd, st);
 }
 
 }  // namespace emb
