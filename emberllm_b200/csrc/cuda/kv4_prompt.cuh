@@ -403,6 +403,12 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
             m_out = m;
         };
         for (int j = 0; j < todo; j++) {
+            ok = kp_wait(&sh.s_full[rt][j % SB], (j / SB) & 1, abort);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            kp_fence_after();
+            // (only now: these scores followed the products of tile j - 2, so that o_done's phase
+            // is told from the one before)
             const bool fresh = TAKE ? j % L::DRAIN == 0 : j == 0;      // nothing in O that counts
             if (TAKE && fresh && j > 0) {
                 ok = kp_wait(&sh.o_done[rt], (j - 1) & 1, abort);
@@ -411,10 +417,6 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
                 kp_fence_after();
                 drain(j > L::DRAIN, false);
             }
-            ok = kp_wait(&sh.s_full[rt][j % SB], (j / SB) & 1, abort);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            kp_fence_after();
             const uint32_t at = mine + rt * 128 + (j % SB) * NP;
             float v[64];
             // a half's scores, the hidden ones -inf

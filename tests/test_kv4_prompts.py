@@ -57,3 +57,18 @@ def test_single_precision_sums_at_any_length(kv, ql, heads, kvh, hd, window, sin
     out = wide[1:, :, 3:].transpose(0, 1)
     p.attend(q, window, sinks, out=out)
     assert torch.equal(out, got) and (wide[0] == 5).all() and (wide[:, :, :3] == 5).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("kv,ql,heads,kvh,hd", [([6000] * 3, [400] * 3, 8, 1, 32), ([9000], [1300], 9, 3, 64), ([20000], [300], 16, 8, 128),
+                                                ([3001], [3001], 12, 12, 64), ([4000, 2500], [900, 2500], 16, 8, 128)])
+def test_long_ranges_again_and_again(dtype, kv, ql, heads, kvh, hd):
+    """many runs give the first one's bits where sums leave tensor memory many times"""
+    p = Paged(kv, ql, 64, kvh, hd, seed=hd)
+    p.store_all()
+    q = queries(sum(ql), heads, hd, dtype=dtype)
+    first = p.attend(q)
+    assert relative(first, p.want(q)) < (4e-6 if dtype == torch.float32 else 2.5e-4)
+    for _ in range(60):
+        assert torch.equal(p.attend(q), first)
