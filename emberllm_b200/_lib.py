@@ -81,7 +81,7 @@ CUDA_SYMBOLS = [
 
 KV4_SYMBOLS = [
     "ember_cuda_kv4_bytes", "ember_cuda_kv4_store", "ember_cuda_kv4_read", "ember_cuda_kv4_attention_workspace",
-    "ember_cuda_kv4_attention", "ember_cuda_sample_rows",
+    "ember_cuda_kv4_attention", "ember_cuda_kv4_status", "ember_cuda_sample_rows",
     "ember_cuda_batch_new_kv4", "ember_cuda_batch_release", "ember_cuda_batch_sample", "ember_batch_new_kv4",
     "ember_batch_release", "ember_batch_sample",
 ]
@@ -173,6 +173,7 @@ def load(path=None):
         getattr(lib, "ember_cuda_kv4_" + name).argtypes = [_P, _P, _P, _P]
     lib.ember_cuda_kv4_attention_workspace.restype = ctypes.c_size_t
     lib.ember_cuda_kv4_attention_workspace.argtypes = [_P] + [ctypes.c_int32] * 4
+    lib.ember_cuda_kv4_status.argtypes = [_P, _P]
     lib.ember_cuda_sample_rows.argtypes = [_P, _P]
     lib.ember_batch_new_kv4.restype = _P
     lib.ember_batch_new_kv4.argtypes = [_P] + [ctypes.c_int] * 6

@@ -403,17 +403,18 @@ EMB_DEV void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-EMB_DEV bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
+EMB_DEV bool mbar_try_wait_at(uint32_t bar, uint32_t parity) {   // bar: its shared-memory address
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
+        : "r"(bar), "r"(parity)
         : "memory");
     return ok != 0;
 }
+EMB_DEV bool mbar_try_wait(uint64_t *bar, uint32_t parity) { return mbar_try_wait_at(smem_u32(bar), parity); }
 
 // Bounded wait: each try_wait blocks for a hardware-chosen slice; after
 // MBAR_TRIES slices (seconds in total) the wait gives up, records `code` in the
@@ -466,7 +467,7 @@ EMB_DEV void kv_round(float v, __half *out) { *out = __float2half_rn(v); }
 enum { CTL_POS = 0, CTL_TOK = 1, CTL_NOUT = 2, CTL_BASE = 3, CTL_ERR = 4, CTL_WORDS = 8 };
 
 // device error codes (written to the state's error word, read by the host)
-enum { ERR_NONE = 0, ERR_GEMV_WAIT = 1, ERR_ATTN_WAIT = 2, ERR_PF_WAIT = 3 };
+enum { ERR_NONE = 0, ERR_GEMV_WAIT = 1, ERR_ATTN_WAIT = 2, ERR_PF_WAIT = 3, ERR_KV4_WAIT = 4 };
 
 // The device expf: the host C library's expf, reproduced from the recipe and
 // exception table described in expf_core.h.

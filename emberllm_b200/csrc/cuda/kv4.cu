@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <math.h>
+#include <stdlib.h>
 
 #include "kv4.cuh"
 #include "kv4_prompt.cuh"
@@ -412,8 +413,8 @@ extern "C" size_t ember_cuda_kv4_attention_workspace(const EmberKv4Cache *cache,
     return kv4_attention_workspace(cache->head_dim, max_kv);
 }
 
-extern "C" int ember_cuda_kv4_attention(const EmberKv4Cache *cache, const EmberKv4Batch *batch,
-                                        const EmberKv4Attention *att, void *stream) {
+int emb::kv4_attention(const EmberKv4Cache *cache, const EmberKv4Batch *batch, const EmberKv4Attention *att, int *err,
+                       cudaStream_t st) {
     const char *who = "kv4 attention";
     Kv4View c;
     Kv4Rows b;
@@ -454,6 +455,34 @@ extern "C" int ember_cuda_kv4_attention(const EmberKv4Cache *cache, const EmberK
     a.n_heads = att->n_heads; a.group = att->n_heads / c.n_kv;
     a.scale = att->scale; a.max_kv = max_kv; a.max_q = max_q; a.window = att->window; a.sinks = att->sinks;
     a.ws = (float *)att->workspace;
-    return att->dtype == EMBER_DT_F32 ? kv4_attention_launch<float>(a, hd, (cudaStream_t)stream)
-                                      : kv4_attention_launch<__half>(a, hd, (cudaStream_t)stream);
+    a.err = err;
+    // tests: keys that never arrive, and so many us until the waits for them run out
+    const char *us = getenv("EMBER_KV4_LOST_KEYS_US");
+    a.lost = us != nullptr;
+    a.wait_ns = us ? strtoull(us, nullptr, 10) * 1000ull : KP_WAIT_NS;
+    return att->dtype == EMBER_DT_F32 ? kv4_attention_launch<float>(a, hd, st)
+                                      : kv4_attention_launch<__half>(a, hd, st);
+}
+
+extern "C" int ember_cuda_kv4_attention(const EmberKv4Cache *cache, const EmberKv4Batch *batch,
+                                        const EmberKv4Attention *att, void *stream) {
+    return kv4_attention(cache, batch, att, nullptr, (cudaStream_t)stream);
+}
+
+extern "C" int ember_cuda_kv4_status(const EmberKv4Cache *cache, void *stream) {
+    const char *who = "kv4 status";
+    if (!cache) return set_err("%s: null cache", who);
+    const int dev = kv4_device_of(cache->data);
+    if (dev < 0) return set_err("%s: cache data is not device memory", who);
+    DeviceScope scope(dev);
+    if (!scope.ok) return set_err("%s: cannot select device %d", who, dev);
+    const cudaStream_t st = (cudaStream_t)stream;
+    int code = 0;
+    CK(cudaMemcpyFromSymbolAsync(&code, kv4_wait_error, sizeof(code), 0, cudaMemcpyDeviceToHost, st));
+    CK(cudaStreamSynchronize(st));
+    if (!code) return 0;
+    const int none = 0;
+    CK(cudaMemcpyToSymbolAsync(kv4_wait_error, &none, sizeof(none), 0, cudaMemcpyHostToDevice, st));
+    CK(cudaStreamSynchronize(st));
+    return set_err("kv4 attention: device wait timed out (code %d)", code);
 }

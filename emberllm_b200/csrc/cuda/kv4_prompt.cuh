@@ -22,16 +22,16 @@
 // product cuts the sum it adds to toward zero at 24 bits, two for 16 positions: sums
 // are off by 2.5e-9 of themselves a position. So those of fp32 outputs leave tensor memory
 // every 512 positions and are added up by rounding additions: 1.6e-6 of the outputs at any length.
-// Us and error, staying / every 2048 / 1024 / 512 / 256 positions: two prompts of 4k 276, 9.9e-6 /
-// 287, 5.2e-6 / 304, 2.8e-6 / 321, 1.6e-6 / 356, 1.0e-6; 512 rows of 40,000 1170, 9.4e-5 / 1184,
-// 5.2e-6 / 1210, 2.8e-6 / 1262, 1.6e-6 / 1369, 1.1e-6; six ragged prompts 54, 1.3e-6 / 54 / 60 / 63,
-// 9e-7 / 68, 6.5e-7 (in plain fp32 operations 4.5e-7). Those of fp16 outputs stay: 9.4e-5 of an
-// output at 40,000 positions, half a step is 2.4e-4 and more.
+// Us and error, staying / every 2048 / 1024 / 512 positions: two fp32 prompts of 4k 282, 9.9e-6 / 295,
+// 5.2e-6 / 311, 2.8e-6 / 341, 1.6e-6; 512 rows of 40,000 1152, 9.4e-5 / 1188, 5.2e-6 / 1213, 2.8e-6 /
+// 1262, 1.6e-6; six ragged prompts of up to 1200 55, 1.3e-6 / 55 / 63 / 66, 9e-7 (plain fp32 operations:
+// 4.5e-7). Those of fp16 outputs stay: 9.4e-5 of an output at 40,000 positions, half a step is
+// 2.4e-4 and more.
 //
 // Bound by the chain scores - maximum - exponentials - weights - outputs of a row tile: tensor
 // pipe, exponentials and conversions are each busy a third of the time. Two prompts of 3.9-4.1k,
-// 16 / 8 heads of 128, fp16: 246 us, 552 TFLOP/s; six of up to 512 rows on up to 1200
-// positions, fp32: 63 us.
+// 16 / 8 heads of 128, fp16: 241 us, 563 TFLOP/s; six of up to 512 rows on up to 1200
+// positions, fp32: 66 us.
 #pragma once
 
 #include "kv4_attn.cuh"
@@ -42,6 +42,9 @@ namespace emb {
 constexpr int KP_ROWS = KV4_TILE_ROWS;
 constexpr int KP_DRAIN = 512;             // positions whose sums stay in tensor memory (fp32)
 constexpr unsigned long long KP_WAIT_NS = 1000000000ull;
+
+// calls of ember_cuda_kv4_attention leave ERR_KV4_WAIT here, ember_cuda_kv4_status takes it
+static __device__ int kv4_wait_error;
 
 template <typename T, int HD, int RT>
 struct KpLayout {
@@ -75,21 +78,28 @@ struct KpShared {
     float rscale[RT * KP_ROWS];
 };
 
-// Wait for a phase; gives up after KP_WAIT_NS or as soon as another role has given up,
-// so that a product that never completes ends the CTA (its rows become NaN).
-EMB_DEV bool kp_wait(uint64_t *bar, uint32_t parity, volatile int *abort) {
-    if (mbar_try_wait(bar, parity)) return true;
+// Wait for a phase; gives up after `ns` of waiting or as soon as another role has given up, so
+// that a product that never completes ends the CTA (its rows become NaN, the error word says
+// so). A poll counts as a millisecond at most: a process that the GPU was taken from for a while has not
+// waited. (The polling is a function of its own: inlined in all places it cost two prompts of 4k in fp16 250 us instead of 241.)
+static __device__ __noinline__ bool kp_poll(uint32_t bar, uint32_t parity, volatile int *abort, unsigned long long ns) {
     unsigned long long t0, t1;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
-    while (!mbar_try_wait(bar, parity)) {
+    while (!mbar_try_wait_at(bar, parity)) {
         if (*abort) return false;
         asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t1));
-        if (t1 - t0 > KP_WAIT_NS) {
+        const unsigned long long took = min(t1 - t0, 1000000ull);
+        if (took >= ns) {
             *abort = 1;
             return false;
         }
+        ns -= took;
+        t0 = t1;
     }
     return true;
+}
+EMB_DEV bool kp_wait_ns(uint64_t *bar, uint32_t parity, volatile int *abort, unsigned long long ns) {
+    return mbar_try_wait(bar, parity) || kp_poll(smem_u32(bar), parity, abort, ns);
 }
 
 EMB_DEV void kp_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -203,7 +213,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
 
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(&sh.k_full[i], 32 * L::KEY_WARPS);
+            mbar_init(&sh.k_full[i], 32 * L::KEY_WARPS + a.lost);
             mbar_init(&sh.k_empty[i], tiles);
             mbar_init(&sh.v_full[i], 64);
             mbar_init(&sh.v_empty[i], tiles);
@@ -225,6 +235,9 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
     kp_fence_after();
     const uint32_t tmem = sh.tmem;
     volatile int *abort = &sh.abort;
+    auto kp_wait = [&](uint64_t *bar, uint32_t parity, volatile int *flag) {
+        return kp_wait_ns(bar, parity, flag, a.wait_ns);
+    };
 
     if (warp < L::SOFT) {
         // ---------------------------------------------------------- softmax ----
@@ -624,7 +637,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
             int never = 0;
             if (kp_elect()) kp_commit(&sh.drain);
             __syncwarp();
-            kp_wait(&sh.drain, 0, &never);
+            kp_wait_ns(&sh.drain, 0, &never, KP_WAIT_NS);
         }
     } else if (warp < L::KEYS + L::KEY_WARPS) {
         // ------------------------------------------------- keys and values ----
@@ -782,6 +795,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
     __syncwarp();
     __syncthreads();
     kp_fence_after();
+    if (tid == 0 && *abort) atomicExch(a.err ? a.err : &kv4_wait_error, ERR_KV4_WAIT);
     if (warp == L::ISSUE)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)L::COLS) : "memory");
 }

@@ -582,7 +582,7 @@ static int pf_layers(EmberCudaModel *m, PfState *ps, const PfSeq &q, const int *
             c.data = (char *)c.data + (size_t)l * q.kv4_layer;
             const EmberKv4Rows rows = { q.kr, q.vr, EMBER_DT_F32, (int64_t)m->n_kv * hd, hd, (int64_t)m->n_kv * hd, hd };
             if (ember_cuda_kv4_store(&c, &q.kv4_rows, &rows, st) ||
-                ember_cuda_kv4_attention(&c, &q.kv4_rows, &q.kv4_att, st))
+                kv4_attention(&c, &q.kv4_rows, &q.kv4_att, err, st))
                 return 1;
             ta.x = q.ao; ta.ld_x = m->n_heads * hd; ta.cols = m->n_heads * hd; ta.k_pad = ps->k_pad[PF_K_QD];
             pf_quant_kernel<<<nc, 256, (size_t)ta.cols * 4, st>>>(ta);

@@ -9,6 +9,7 @@
 #include <vector>
 
 #include "ember_cuda.h"
+#include "ember_kv4.h"
 #include "common.cuh"
 
 namespace emb {
@@ -130,6 +131,14 @@ void persist_release(EmberCudaState *s);
 // enqueue n_steps token steps from ctl's token and position on s->stream;
 // greedy: pick between steps and write the picks to s->out_tokens
 int persist_run(EmberCudaState *s, int n_steps, int greedy);
+}  // namespace emb
+
+// ---- attention over the paged 4-bit cache (kv4.cu) ----
+namespace emb {
+// ember_cuda_kv4_attention whose device waits report to *err (device memory; NULL: to
+// ember_cuda_kv4_status)
+int kv4_attention(const EmberKv4Cache *cache, const EmberKv4Batch *batch, const EmberKv4Attention *att, int *err,
+                  cudaStream_t st);
 }  // namespace emb
 
 // ---- device sampling (sample.cu) ----

@@ -140,6 +140,12 @@ class Kv4Cache:
                           self.head_dim ** -0.5 if scale is None else scale, max_kv, window, sinks, ws, nws), stream):
             _fail()
 
+    def check(self, stream=0):
+        """Wait for the stream's work; RuntimeError when a device wait of an attention
+        call has run out since the last check (its rows are NaN)."""
+        if self.lib.ember_cuda_kv4_status(self._p, stream):
+            _fail()
+
 
 def sample_rows(logits, out, u, temperature=None, top_k=None, top_p=None, min_p=None, stream=0):
     """Draw one token per row of ``logits`` [rows][vocab] into ``out`` (int32), with

@@ -124,6 +124,11 @@ size_t ember_cuda_kv4_attention_workspace(const EmberKv4Cache *cache, int32_t n_
 int ember_cuda_kv4_attention(const EmberKv4Cache *cache, const EmberKv4Batch *batch, const EmberKv4Attention *att,
                              void *stream);
 
+/* Waits for the stream's work and returns 1 when a wait inside an attention call on the
+ * cache's device has run out since this was last asked (a second of waiting, which no working
+ * GPU needs): the rows it concerned are NaN. Not while the stream is captured. */
+int ember_cuda_kv4_status(const EmberKv4Cache *cache, void *stream);
+
 /* ---- one draw per row ----
  * out[r] = a token drawn from row r of logits [n_rows][vocab] (dtype F32 or F16, row
  * stride in elements, a row's elements consecutive), with that row's settings and
