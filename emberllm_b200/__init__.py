@@ -140,7 +140,9 @@ class EmberBatch:
         return [[out[k * self.n + i] for i in range(self.n)] for k in range(n_steps)]
 
     def release(self, stream):
-        """give a stream's pages back (kv4 batches); its next prompt starts anew"""
+        """Give a stream's pages back (kv4 batches). It is idle until its next prompt,
+        which starts anew: greedy and sample go on without it (its token and position
+        may be anything, its tokens are -1)."""
         self.lib.ember_batch_release(self.b, int(stream))
 
     def close(self):

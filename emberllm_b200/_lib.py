@@ -82,7 +82,7 @@ CUDA_SYMBOLS = [
 KV4_SYMBOLS = [
     "ember_cuda_kv4_bytes", "ember_cuda_kv4_store", "ember_cuda_kv4_read", "ember_cuda_kv4_attention_workspace",
     "ember_cuda_kv4_attention", "ember_cuda_kv4_status", "ember_cuda_sample_rows",
-    "ember_cuda_batch_new_kv4", "ember_cuda_batch_release", "ember_cuda_batch_sample", "ember_batch_new_kv4",
+    "ember_cuda_batch_new_kv4", "ember_cuda_batch_release", "ember_cuda_batch_idle", "ember_cuda_batch_sample", "ember_batch_new_kv4",
     "ember_batch_release", "ember_batch_sample",
 ]
 
@@ -177,6 +177,7 @@ def load(path=None):
     lib.ember_cuda_sample_rows.argtypes = [_P, _P]
     lib.ember_batch_new_kv4.restype = _P
     lib.ember_batch_new_kv4.argtypes = [_P] + [ctypes.c_int] * 6
+    lib.ember_cuda_batch_idle.argtypes = [_P, ctypes.c_int]
     lib.ember_batch_release.argtypes = [_P, ctypes.c_int]
     lib.ember_batch_sample.argtypes = [_P, _IP, _IP, ctypes.c_int, ctypes.POINTER(EmberSampleParams), _FP, _IP, _FP]
     lib.ember_cuda_batch_sample.argtypes = lib.ember_batch_sample.argtypes

@@ -811,10 +811,11 @@ __global__ void batch_take_kernel(const int *drawn, int *tok, int *pos, int *out
     pos[s] += 1;
     out[(size_t)(*nout) * S + s] = drawn[s];
 }
-// a step's cache lengths: the token at pos is the last position
-__global__ void batch_len_kernel(const int *pos, int *len, int S) {
+// a step's cache lengths: the token at pos is the last position; a stream that is idle
+// has none, so that nothing of it is stored or looked at
+__global__ void batch_len_kernel(const int *pos, const int *idle, int *len, int S) {
     const int s = blockIdx.x * blockDim.x + threadIdx.x;
-    if (s < S) len[s] = pos[s] + 1;
+    if (s < S) len[s] = idle[s] ? 0 : pos[s] + 1;
 }
 
 // The caches of a batch over pages: one pool of pages per layer, shared by the
@@ -829,12 +830,13 @@ struct Kv4Streams {
     size_t layer = 0;                 // bytes per layer
     int width = 0;                    // pages of a stream, at most
     int32_t *table = nullptr, *len = nullptr, *one = nullptr;   // [S][width]; [S]; a prompt's {0, rows, length}
+    int *idle = nullptr;              // [S]: 1 from a stream's release to its next prompt
     float *kr = nullptr, *vr = nullptr, *ao = nullptr;
     void *ws = nullptr;
     size_t ws_bytes = 0;
     int window = 0, sinks = 0;
     std::vector<int32_t> h_table, free;
-    std::vector<int> held;
+    std::vector<int> held, h_idle;
 };
 
 }  // namespace emb
@@ -946,6 +948,7 @@ static int kv4_prefill(EmberCudaBatch *b, int stream, const int *ids, int n, flo
     EmberCudaModel *m = b->m;
     Kv4Streams *k = b->kv4;
     if (kv4_reserve(b, stream, n)) return 1;
+    k->h_idle[stream] = 0;
     CK(cudaMemsetAsync(k->ctl + CTL_ERR, 0, 4, k->st));
     int nc = 0;
     for (int c0 = 0; c0 < n; c0 += nc) {
@@ -996,6 +999,7 @@ extern "C" int ember_cuda_batch_new_kv4(EmberCudaModel *m, int n_streams, int ct
     k->width = width; k->window = window; k->sinks = sinks; k->layer = layer;
     k->h_table.assign((size_t)n_streams * width, -1);
     k->held.assign(n_streams, 0);
+    k->h_idle.assign(n_streams, 0);
     for (int i = n_pages - 1; i >= 0; i--) k->free.push_back(i);
     const int hd = m->head_dim, rows = PF_CHUNK;
     const size_t n_rope = (size_t)ctx * (hd / 2) * sizeof(float2);
@@ -1010,7 +1014,7 @@ extern "C" int ember_cuda_batch_new_kv4(EmberCudaModel *m, int n_streams, int ct
         auto get = [&](void **p, size_t n) { return pf_alloc(b->allocs, p, n); };
         rc = get(&k->cache.data, layer * m->n_layers) || get((void **)&k->rope, n_rope) ||
              get((void **)&k->ctl, CTL_WORDS * 4) || get((void **)&k->ids, (size_t)rows * 4) ||
-             get((void **)&k->table, k->h_table.size() * 4) || get((void **)&k->len, (size_t)n_streams * 4) ||
+             get((void **)&k->table, k->h_table.size() * 4) || get((void **)&k->len, (size_t)n_streams * 4) || get((void **)&k->idle, (size_t)n_streams * 4) ||
              get((void **)&k->one, 16) || get((void **)&k->kr, (size_t)rows * m->n_kv * hd * 4) ||
              get((void **)&k->vr, (size_t)rows * m->n_kv * hd * 4) || get((void **)&k->ao, (size_t)rows * m->n_heads * hd * 4) ||
              get(&k->ws, k->ws_bytes ? k->ws_bytes : 16) || get((void **)&b->tok, (size_t)n_streams * 4) ||
@@ -1037,7 +1041,12 @@ extern "C" int ember_cuda_batch_release(EmberCudaBatch *b, int stream) {
     const int32_t *row = k->h_table.data() + (size_t)stream * k->width;
     for (int i = k->held[stream] - 1; i >= 0; i--) k->free.push_back(row[i]);
     k->held[stream] = 0;
+    k->h_idle[stream] = 1;
     return 0;
+}
+
+extern "C" int ember_cuda_batch_idle(const EmberCudaBatch *b, int stream) {
+    return b->kv4 && stream >= 0 && stream < b->S && b->kv4->h_idle[stream];
 }
 
 extern "C" int ember_cuda_batch_new(EmberCudaModel *m, int n_streams, int ctx, int kv_fp16, const float *rope_cs,
@@ -1152,7 +1161,7 @@ static int batch_record(EmberCudaBatch *b, bool draw) {
     q.n = b->S; q.start = 0; q.pos = b->pos;
     if (b->kv4) {
         Kv4Streams *k = b->kv4;
-        batch_len_kernel<<<(b->S + 255) / 256, 256, 0, st>>>(b->pos, k->len, b->S);
+        batch_len_kernel<<<(b->S + 255) / 256, 256, 0, st>>>(b->pos, k->idle, k->len, b->S);
         CK(cudaGetLastError());
         kv4_seq_args(b, q);
         q.kv4_rows.kv_len = k->len;
@@ -1214,9 +1223,18 @@ static int batch_run(EmberCudaBatch *b, bool draw, const int *toks, const int *p
                      float *host_logits) {
     cudaStream_t st = batch_stream(b);
     int *ctl = batch_ctl(b);
-    if (b->kv4)
+    std::vector<int> tok0, pos0;          // an idle stream goes along as token 0 at position 0
+    if (b->kv4) {
+        const std::vector<int> &idle = b->kv4->h_idle;
+        tok0.assign(toks, toks + b->S);
+        pos0.assign(pos, pos + b->S);
         for (int i = 0; i < b->S; i++)
-            if (kv4_reserve(b, i, pos[i] + n_steps)) return 1;
+            if (idle[i]) tok0[i] = pos0[i] = 0;
+            else if (kv4_reserve(b, i, pos[i] + n_steps)) return 1;
+        toks = tok0.data();
+        pos = pos0.data();
+        CK(cudaMemcpyAsync(b->kv4->idle, idle.data(), (size_t)b->S * 4, cudaMemcpyHostToDevice, st));
+    }
     cudaGraphExec_t &exec = draw ? b->g_draw : b->g_step;
     if (!exec) {
         cudaGraph_t g = nullptr;
@@ -1246,12 +1264,19 @@ static int batch_run(EmberCudaBatch *b, bool draw, const int *toks, const int *p
     CK(cudaMemcpyAsync(&herr, ctl + CTL_ERR, 4, cudaMemcpyDeviceToHost, st));
     CK(cudaStreamSynchronize(st));
     if (herr) return set_err("batch: device wait timed out (code %d)", herr);
+    for (int i = 0; i < b->S; i++)
+        if (ember_cuda_batch_idle(b, i)) {
+            for (int s = 0; host_tokens && s < n_steps; s++) host_tokens[(size_t)s * b->S + i] = -1;
+            if (host_logits) memset(host_logits + (size_t)i * b->m->vocab, 0, (size_t)b->m->vocab * 4);
+        }
     return 0;
 }
 
 static int batch_check_steps(EmberCudaBatch *b, const int *toks, const int *pos, int n_steps) {
     if (n_steps < 1 || n_steps > b->max_steps) return set_err("batch: n_steps must be in [1, %d]", b->max_steps);
+    if (n_steps > b->ctx) return set_err("batch: %d steps do not fit the context", n_steps);
     for (int i = 0; i < b->S; i++) {
+        if (ember_cuda_batch_idle(b, i)) continue;
         if (toks[i] < 0 || toks[i] >= b->m->vocab) return set_err("batch: token id %d out of range", toks[i]);
         if (pos[i] < 0 || pos[i] > b->ctx - n_steps) return set_err("batch: stream %d does not fit the context", i);
     }
@@ -1299,6 +1324,7 @@ extern "C" int ember_cuda_batch_sample(EmberCudaBatch *b, const int *toks, const
     std::vector<int> top_k(b->S);
     for (int i = 0; i < b->S; i++) {
         const EmberSampleParams &p = params[i];
+        if (ember_cuda_batch_idle(b, i)) continue;        // temperature 0
         if (p.repeat_penalty != 1.0f || p.presence_penalty != 0.0f || p.frequency_penalty != 0.0f)
             return set_err("batch: stream %d: penalties are not supported by drawn steps", i);
         if (p.temperature != p.temperature) return set_err("batch: stream %d: temperature is NaN", i);

@@ -308,8 +308,9 @@ float *ember_batch_prefill(EmberBatch *b, int stream, const int *ids, int n) {
 void ember_batch_greedy(EmberBatch *b, const int *toks, const int *pos, int n_steps, int *out_tokens,
                         float *out_logits) {
     for (int i = 0; i < b->n_streams; i++) {
+        if (ember_cuda_batch_idle(b->dev, i)) continue;
         if (toks[i] < 0 || toks[i] >= b->vocab) ember_die("token id %d out of range [0,%d)", toks[i], b->vocab);
-        if (pos[i] < 0 || pos[i] + n_steps > b->ctx)
+        if (pos[i] < 0 || (long long)pos[i] + n_steps > b->ctx)
             ember_die("stream %d: %d steps from position %d do not fit the context of %d", i, n_steps, pos[i],
                       b->ctx);
     }

@@ -165,11 +165,15 @@ int ember_cuda_sample_rows(const EmberSampleRows *args, void *stream);
  * ember_cuda_kv4_attention's, with `window` and `sinks`. Any n_streams in [1, 512];
  * head_dim 32, 64 or 128. prefill, greedy, sample and free take such a batch as any
  * other. A call that finds no free page fails and leaves the streams as they were
- * (pages handed out before it found out stay with their streams). release gives a
- * stream's pages back: its next prompt starts anew. */
+ * (pages handed out before it found out stay with their streams). Pages behind the
+ * window stay, too.
+ * release gives a stream's pages back and leaves it idle until its next prompt, which
+ * starts anew: greedy and sample go on without it. Its toks, pos, params and u are not looked at
+ * then, it takes no page, its tokens are -1 and its logits 0. */
 int ember_cuda_batch_new_kv4(EmberCudaModel *m, int n_streams, int ctx, int n_pages, int window, int sinks,
                              const float *rope_cs, int max_steps, EmberCudaBatch **out);
 int ember_cuda_batch_release(EmberCudaBatch *b, int stream);
+int ember_cuda_batch_idle(const EmberCudaBatch *b, int stream);     /* 1 or 0 */
 /* As ember_cuda_batch_greedy, but every step's tokens are drawn by
  * ember_cuda_sample_rows: stream i with params[i] (no penalties) and, at step t, the
  * random number u[t * n_streams + i]. Not for a batch that holds one state per stream
