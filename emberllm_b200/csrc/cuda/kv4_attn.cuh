@@ -62,6 +62,12 @@ EMB_DEV bool kv4_visible(int pos, int p, int window, int sinks) {
     return p <= pos && (window == 0 || pos - p < window || p < sinks);
 }
 
+// [sinks, this] are the positions in front of every row's window when the first row is
+// at `first`; hidden from all rows, they may never have been written
+EMB_DEV int kv4_before(int first, int window) {
+    return window > 0 ? (int)max(-1ll, (long long)first - window) : -1;
+}
+
 EMB_DEV float kv4_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -310,6 +316,7 @@ __global__ void __launch_bounds__(KD_THREADS, KdLayout<HD, NT>::CTAS) kv4_decode
     // positions that every row sees: up to the first row's, from the last row's window on
     const int all_to = min(len, pos0 + chunk_row / a.group + 1);
     const long long all_from = a.window > 0 ? (long long)pos0 + (chunk_row + min(rows, R) - 1) / a.group - a.window + 1 : 0;
+    const int before = kv4_before(pos0 + chunk_row / a.group, a.window);
 
     for (; i < u1; i += KD_WARPS) {
         if (i + KD_WARPS < u1) copy(pg, pn, stage ^ 1);
@@ -401,7 +408,7 @@ __global__ void __launch_bounds__(KD_THREADS, KdLayout<HD, NT>::CTAS) kv4_decode
         }
 
         // outputs
-        const bool cut = p0 + KD_UNIT > len || !ok0 || !ok1;
+        const bool cut = p0 + KD_UNIT > len || !ok0 || !ok1 || (p0 <= before && p0 + KD_UNIT > a.sinks);
         const __half2 bias_lo = bits_h2(0x64086408u);                                     // 1032
         const __half2 sixteenth = bits_h2(0x2C002C00u), bias_hi = bits_h2(0xD480D480u);   // 1/16, -72
 #pragma unroll
@@ -413,11 +420,16 @@ __global__ void __launch_bounds__(KD_THREADS, KdLayout<HD, NT>::CTAS) kv4_decode
             lds_words<NB>(vs[0], sp);
             lds_words<NB>(vs[1], sp + 4 * (4 * NB));
             if (cut) {
-                // positions behind the length may hold any bytes: their scales count as 0
+                // positions that no row sees may hold any bytes: their scales count as 0
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    const int left = (h ? ok1 : ok0) ? len - (p0 + 16 * h + 2 * t + 8 * j) : 0;
-                    const uint32_t keep = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0x0000FFFFu : 0u;
+                    const int p = p0 + 16 * h + 2 * t + 8 * j;
+                    const int left = (h ? ok1 : ok0) ? len - p : 0;
+                    uint32_t keep = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0x0000FFFFu : 0u;
+                    if (p <= before) {
+                        if (p >= a.sinks) keep &= 0xFFFF0000u;
+                        if (p + 1 >= a.sinks && p < before) keep &= 0x0000FFFFu;
+                    }
 #pragma unroll
                     for (int b = 0; b < NB; b++) vs[j][b] &= keep;
                 }

@@ -730,6 +730,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
             struct Packed { uint32_t w[4][NB], d[4][NB]; };
             int pg;
             auto page = [&](int i) { pg = page_at(i / H, (i % H) * 64 + 8 * c); };
+            const int before = kv4_before(pos0 + row_first / a.group, a.window);
             auto load = [&](Packed &u, int i) {
                 if (i >= n * H) return;
                 const int p0 = range.pos(i / H) + (i % H) * 64;
@@ -741,12 +742,13 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
                     lds_words<NB>(u.w[e], gr + 8 * HD + pair * HD + g * (4 * NB));
                     lds_words<NB>(u.d[e], gr + 16 * HD + 32 * NB + pair * (4 * NB));
                 }
-                // positions behind the length may hold any bytes: their scales count as 0
-                if (!is || p0 + 64 > len) {
+                // positions that no row sees may hold any bytes: their scales count as 0
+                if (!is || p0 + 64 > len || (p0 <= before && p0 + 64 > a.sinks)) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const int left = is ? len - (p0 + 8 * c + 2 * e) : 0;
-                        const uint32_t keep = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0x0000FFFFu : 0u;
+                        const int p = p0 + 8 * c + 2 * e;
+                        auto seen = [&](int q) { return is && q < len && (q < a.sinks || q > before); };
+                        const uint32_t keep = (seen(p) ? 0xFFFFu : 0u) | (seen(p + 1) ? 0xFFFF0000u : 0u);
 #pragma unroll
                         for (int b = 0; b < NB; b++) u.d[e][b] &= keep;
                     }

@@ -39,7 +39,8 @@ extern "C" {
  *
  * The order of the bytes inside a page is the kernels' own: only the functions
  * below read or write it. Bytes never written may have any content: positions
- * behind a sequence's length are not looked at. */
+ * that no row of a call sees (behind a sequence's length, in front of its rows' window)
+ * have no part in the result. */
 typedef struct {
     void   *data;         /* device memory of this layer's cache, 16-byte aligned     */
     int32_t n_pages;      /* n_pages * page_size at most 2^31 - 1                     */

@@ -1,5 +1,6 @@
 """A row's attention over the paged 4-bit cache does not depend on its neighbours: the
-other rows' and heads' queries may be anything, its bits stay."""
+other rows' and heads' queries may be anything, its bits stay; so may the bytes of
+positions that no row sees."""
 import pytest
 
 from .test_kv4 import Paged
@@ -54,3 +55,29 @@ def test_other_rows_queries_change_nothing(dtype, kv, ql, heads, kvh, hd):
     # 2 * 340 * (hd + 8) * 2^-24 <= 5.6e-3, values below 8)
     want = p.want(rise.cuda())
     assert torch.isfinite(both).all() and (both.double() - want).abs().amax() < 0.1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("window,sinks", [(100, 4), (33, 0), (250, 19), (1, 1), (700, 33), (64, 64)])
+@pytest.mark.parametrize("kv,ql,heads,kvh,hd", [([1500, 811], [1, 1], 16, 8, 128), ([1500, 811], [3, 2], 14, 2, 64),
+                                                ([1500, 811], [300, 130], 16, 8, 128), ([1000] * 6, [430] * 6, 9, 3, 32)])
+def test_positions_that_nobody_sees_need_not_be_written(dtype, window, sinks, kv, ql, heads, kvh, hd):
+    """a program that keeps the first tokens and a window writes nothing else: the
+    other bytes are NaN scales here, in the same pages and groups"""
+    p = Paged(kv, ql, 64, kvh, hd, seed=window)
+    p.store_all()
+    q = (torch.randn(sum(ql), heads, hd, generator=torch.Generator().manual_seed(3)) * 1.2).to(dtype).cuda()
+    want = p.attend(q, window, sinks)
+    assert torch.isfinite(want).all()
+    p.buf.fill_(0xFF)
+    at = 0
+    for i, (n, m) in enumerate(zip(kv, ql)):
+        for end, rows in ((min(sinks, n), min(sinks, n)), (n, min(n, window + m - 1))):
+            if rows:
+                start = torch.tensor([0, rows], dtype=torch.int32).cuda()
+                lens = torch.tensor([end], dtype=torch.int32).cuda()
+                src = slice(at + end - rows, at + end)
+                p.cache.store(p.k[src], p.v[src], start, lens, p.table[i:i + 1], rows)
+        at += n
+    assert torch.equal(p.attend(q, window, sinks), want)
