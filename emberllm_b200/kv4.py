@@ -38,6 +38,13 @@ def _fail():
     raise RuntimeError(_libmod.load().ember_cuda_error().decode())
 
 
+def _pack(form, *values):
+    try:
+        return form.pack(*values)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"a number does not fit its field: {e}") from None
+
+
 def _dtype(t, name):
     d = _DT[t.dtype]
     if d is None or d < 0:
@@ -69,29 +76,33 @@ class Kv4Cache:
     @staticmethod
     def nbytes(n_pages, page_size, n_kv_heads, head_dim):
         """bytes of the buffer such a cache needs"""
-        n = _libmod.load().ember_cuda_kv4_bytes(int(n_pages), int(page_size), int(n_kv_heads), int(head_dim))
+        sizes = (int(n_pages), int(page_size), int(n_kv_heads), int(head_dim))
+        n = max(sizes) < 2 ** 31 and min(sizes) > 0 and _libmod.load().ember_cuda_kv4_bytes(*sizes)
         if not n:
             raise ValueError(f"a cache of {n_pages} pages of {page_size} positions, {n_kv_heads} kv heads of {head_dim} "
                              "is not supported")
         return n
 
     def __init__(self, buffer, n_pages, page_size, n_kv_heads, head_dim):
+        n_pages, page_size, n_kv_heads, head_dim = int(n_pages), int(page_size), int(n_kv_heads), int(head_dim)
         need = Kv4Cache.nbytes(n_pages, page_size, n_kv_heads, head_dim)
         if not buffer.is_contiguous() or buffer.numel() * buffer.element_size() < need:
             raise ValueError(f"the cache needs a contiguous buffer of {need} bytes")
         self.lib = _libmod.load()
         self.buffer = buffer            # kept alive
-        self.page_size, self.n_kv_heads, self.head_dim = int(page_size), int(n_kv_heads), int(head_dim)
-        self._p = _CACHE.pack(buffer.data_ptr(), n_pages, page_size, n_kv_heads, head_dim)
+        self.page_size, self.n_kv_heads, self.head_dim = page_size, n_kv_heads, head_dim
+        self._p = _pack(_CACHE, buffer.data_ptr(), n_pages, page_size, n_kv_heads, head_dim)
 
     def _batch(self, tokens, q_start, kv_len, block_table, max_q):
+        if len(kv_len.shape) != 1:
+            raise ValueError(f"kv_len must have one dimension, not {len(kv_len.shape)}")
         n = kv_len.shape[0]
         ts = block_table.shape
         if len(ts) != 2 or ts[0] != n or _DT[block_table.dtype] != _I32:
             raise ValueError(f"block_table must be an int32 [{n}][pages] array")
         if not block_table.is_contiguous():
             raise ValueError("block_table must be contiguous")
-        return _BATCH.pack(0 if q_start is None else _array(q_start, "q_start", _I32, n + 1),
+        return _pack(_BATCH, 0 if q_start is None else _array(q_start, "q_start", _I32, n + 1),
                            _array(kv_len, "kv_len", _I32, n), block_table.data_ptr(), n, ts[1], tokens, max_q)
 
     def _io(self, fn, k, v, q_start, kv_len, block_table, max_q, stream):
@@ -100,7 +111,7 @@ class Kv4Cache:
         if k.shape[0] != v.shape[0] or k.dtype != v.dtype:
             raise ValueError("k and v must have the same rows and type")
         if fn(self._p, self._batch(k.shape[0], q_start, kv_len, block_table, max_q),
-              _ROWS.pack(k.data_ptr(), v.data_ptr(), _dtype(k, "k"), k_tok, k_head, v_tok, v_head), stream):
+              _pack(_ROWS, k.data_ptr(), v.data_ptr(), _dtype(k, "k"), k_tok, k_head, v_tok, v_head), stream):
             _fail()
 
     def store(self, k, v, q_start, kv_len, block_table, max_q=1, stream=0):
@@ -125,6 +136,8 @@ class Kv4Cache:
         cache into ``out``; ``window`` > 0 limits it to the last ``window`` positions
         and the first ``sinks``. ``max_kv`` bounds kv_len (default: all the block table
         can hold), ``scale`` defaults to head_dim ** -0.5."""
+        if len(q.shape) != 3:
+            raise ValueError(f"q must be [rows][heads][{self.head_dim}], not {list(q.shape)}")
         heads = q.shape[1]
         q_tok, q_head = _rows(q, "q", heads, self.head_dim)
         out_tok, out_head = _rows(out, "out", heads, self.head_dim)
@@ -133,10 +146,14 @@ class Kv4Cache:
         b = self._batch(q.shape[0], q_start, kv_len, block_table, max_q)
         if max_kv is None:
             max_kv = min(block_table.shape[1] * self.page_size, 2 ** 31 - 1)
-        ws, nws = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
+        ws, nws = 0, 0
+        if workspace is not None:
+            if not workspace.is_contiguous():      # (its bytes need not be there)
+                raise ValueError("workspace must be contiguous")
+            ws, nws = workspace.data_ptr(), workspace.numel() * workspace.element_size()
         if self.lib.ember_cuda_kv4_attention(
                 self._p, b,
-                _ATT.pack(q.data_ptr(), out.data_ptr(), _dtype(q, "q"), heads, q_tok, q_head, out_tok, out_head,
+                _pack(_ATT, q.data_ptr(), out.data_ptr(), _dtype(q, "q"), heads, q_tok, q_head, out_tok, out_head,
                           self.head_dim ** -0.5 if scale is None else scale, max_kv, window, sinks, ws, nws), stream):
             _fail()
 
@@ -160,7 +177,7 @@ def sample_rows(logits, out, u, temperature=None, top_k=None, top_p=None, min_p=
     def opt(t, name, dtype=_F32):
         return 0 if t is None else _array(t, name, dtype, n)
     if lib.ember_cuda_sample_rows(
-            _SAMPLE.pack(logits.data_ptr(), _dtype(logits, "logits"), n, logits.shape[1], logits.stride(0),
+            _pack(_SAMPLE, logits.data_ptr(), _dtype(logits, "logits"), n, logits.shape[1], logits.stride(0),
                          opt(temperature, "temperature"), opt(top_p, "top_p"), opt(min_p, "min_p"),
                          _array(u, "u", _F32, n), opt(top_k, "top_k", _I32), _array(out, "out", _I32, n)), stream):
         _fail()
