@@ -6,10 +6,13 @@ Arrays are CUDA tensors as torch makes them (anything with ``data_ptr``,
 ``shape``, ``stride()``, ``dtype`` and ``device`` works; this module does not
 import torch). The caller owns every buffer; a call allocates nothing and enqueues
 its work on ``stream`` (a cudaStream_t as an integer; 0 is the default stream).
+None, the default, is the stream that torch's own operations on these tensors would take
+now (torch.cuda.current_stream), or 0 for arrays of others.
 Arguments that do not fit raise ValueError; what the library refuses raises
 RuntimeError with its message.
 """
 import struct
+import sys
 
 from . import _lib as _libmod
 
@@ -32,6 +35,24 @@ class _Dtypes(dict):
 
 _DT = _Dtypes()
 _F32, _I32 = 0, -32
+
+
+_torch = None          # (its Tensor, its current stream of a device), once it is there
+
+
+def _on(stream, t):
+    """the stream a call on array t goes to"""
+    global _torch
+    if stream is not None:
+        return stream
+    if _torch is None:
+        m = sys.modules.get("torch")
+        if m is None:
+            return 0
+        # (the public call makes an object of the stream: a microsecond more)
+        _torch = m.Tensor, getattr(m._C, "_cuda_getCurrentRawStream",
+                                   lambda i: m.cuda.current_stream(i).cuda_stream)
+    return _torch[1](t.device.index) if isinstance(t, _torch[0]) and t.is_cuda else 0
 
 
 def _fail():
@@ -111,17 +132,17 @@ class Kv4Cache:
         if k.shape[0] != v.shape[0] or k.dtype != v.dtype:
             raise ValueError("k and v must have the same rows and type")
         if fn(self._p, self._batch(k.shape[0], q_start, kv_len, block_table, max_q),
-              _pack(_ROWS, k.data_ptr(), v.data_ptr(), _dtype(k, "k"), k_tok, k_head, v_tok, v_head), stream):
+              _pack(_ROWS, k.data_ptr(), v.data_ptr(), _dtype(k, "k"), k_tok, k_head, v_tok, v_head), _on(stream, k)):
             _fail()
 
-    def store(self, k, v, q_start, kv_len, block_table, max_q=1, stream=0):
+    def store(self, k, v, q_start, kv_len, block_table, max_q=1, stream=None):
         """Quantize the rows' keys and values ([rows][kv heads][head_dim]) into the
         cache: rows q_start[i]..q_start[i+1]-1 are the last positions of sequence i's
         kv_len[i]. ``q_start`` None: one row per sequence. ``max_q``: the most rows
         any sequence has."""
         self._io(self.lib.ember_cuda_kv4_store, k, v, q_start, kv_len, block_table, max_q, stream)
 
-    def read(self, k, v, q_start, kv_len, block_table, max_q=1, stream=0):
+    def read(self, k, v, q_start, kv_len, block_table, max_q=1, stream=None):
         """The inverse of ``store``: the cached values of the rows' positions into k
         and v."""
         self._io(self.lib.ember_cuda_kv4_read, k, v, q_start, kv_len, block_table, max_q, stream)
@@ -131,7 +152,7 @@ class Kv4Cache:
         return self.lib.ember_cuda_kv4_attention_workspace(self._p, n_heads, n_seqs, max_q, max_kv)
 
     def attention(self, q, out, q_start, kv_len, block_table, max_q=1, max_kv=None, scale=None, window=0, sinks=0,
-                  workspace=None, stream=0):
+                  workspace=None, stream=None):
         """Causal attention of the rows' queries ([rows][heads][head_dim]) over the
         cache into ``out``; ``window`` > 0 limits it to the last ``window`` positions
         and the first ``sinks``. ``max_kv`` bounds kv_len (default: all the block table
@@ -154,17 +175,17 @@ class Kv4Cache:
         if self.lib.ember_cuda_kv4_attention(
                 self._p, b,
                 _pack(_ATT, q.data_ptr(), out.data_ptr(), _dtype(q, "q"), heads, q_tok, q_head, out_tok, out_head,
-                          self.head_dim ** -0.5 if scale is None else scale, max_kv, window, sinks, ws, nws), stream):
+                          self.head_dim ** -0.5 if scale is None else scale, max_kv, window, sinks, ws, nws), _on(stream, q)):
             _fail()
 
-    def check(self, stream=0):
+    def check(self, stream=None):
         """Wait for the stream's work; RuntimeError when a device wait of an attention
         call has run out since the last check (its rows are NaN)."""
-        if self.lib.ember_cuda_kv4_status(self._p, stream):
+        if self.lib.ember_cuda_kv4_status(self._p, _on(stream, self.buffer)):
             _fail()
 
 
-def sample_rows(logits, out, u, temperature=None, top_k=None, top_p=None, min_p=None, stream=0):
+def sample_rows(logits, out, u, temperature=None, top_k=None, top_p=None, min_p=None, stream=None):
     """Draw one token per row of ``logits`` [rows][vocab] into ``out`` (int32), with
     each row's own random number ``u`` in [0, 1) and settings (float32 arrays,
     ``top_k`` int32; None: temperature 1, no truncation). See
@@ -179,5 +200,5 @@ def sample_rows(logits, out, u, temperature=None, top_k=None, top_p=None, min_p=
     if lib.ember_cuda_sample_rows(
             _pack(_SAMPLE, logits.data_ptr(), _dtype(logits, "logits"), n, logits.shape[1], logits.stride(0),
                          opt(temperature, "temperature"), opt(top_p, "top_p"), opt(min_p, "min_p"),
-                         _array(u, "u", _F32, n), opt(top_k, "top_k", _I32), _array(out, "out", _I32, n)), stream):
+                         _array(u, "u", _F32, n), opt(top_k, "top_k", _I32), _array(out, "out", _I32, n)), _on(stream, logits)):
         _fail()
