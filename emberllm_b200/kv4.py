@@ -59,11 +59,8 @@ def _fail():
     raise RuntimeError(_libmod.load().ember_cuda_error().decode())
 
 
-def _pack(form, *values):
-    try:
-        return form.pack(*values)
-    except (struct.error, OverflowError) as e:
-        raise ValueError(f"a number does not fit its field: {e}") from None
+def _too_large(e):
+    return ValueError(f"a number does not fit its field: {e}")
 
 
 def _dtype(t, name):
@@ -112,7 +109,7 @@ class Kv4Cache:
         self.lib = _libmod.load()
         self.buffer = buffer            # kept alive
         self.page_size, self.n_kv_heads, self.head_dim = page_size, n_kv_heads, head_dim
-        self._p = _pack(_CACHE, buffer.data_ptr(), n_pages, page_size, n_kv_heads, head_dim)
+        self._p = _CACHE.pack(buffer.data_ptr(), n_pages, page_size, n_kv_heads, head_dim)
 
     def _batch(self, tokens, q_start, kv_len, block_table, max_q):
         if len(kv_len.shape) != 1:
@@ -123,7 +120,7 @@ class Kv4Cache:
             raise ValueError(f"block_table must be an int32 [{n}][pages] array")
         if not block_table.is_contiguous():
             raise ValueError("block_table must be contiguous")
-        return _pack(_BATCH, 0 if q_start is None else _array(q_start, "q_start", _I32, n + 1),
+        return _BATCH.pack(0 if q_start is None else _array(q_start, "q_start", _I32, n + 1),
                            _array(kv_len, "kv_len", _I32, n), block_table.data_ptr(), n, ts[1], tokens, max_q)
 
     def _io(self, fn, k, v, q_start, kv_len, block_table, max_q, stream):
@@ -131,8 +128,12 @@ class Kv4Cache:
         v_tok, v_head = _rows(v, "v", self.n_kv_heads, self.head_dim)
         if k.shape[0] != v.shape[0] or k.dtype != v.dtype:
             raise ValueError("k and v must have the same rows and type")
-        if fn(self._p, self._batch(k.shape[0], q_start, kv_len, block_table, max_q),
-              _pack(_ROWS, k.data_ptr(), v.data_ptr(), _dtype(k, "k"), k_tok, k_head, v_tok, v_head), _on(stream, k)):
+        try:
+            batch = self._batch(k.shape[0], q_start, kv_len, block_table, max_q)
+            rows = _ROWS.pack(k.data_ptr(), v.data_ptr(), _dtype(k, "k"), k_tok, k_head, v_tok, v_head)
+        except struct.error as e:
+            raise _too_large(e) from None
+        if fn(self._p, batch, rows, _on(stream, k)):
             _fail()
 
     def store(self, k, v, q_start, kv_len, block_table, max_q=1, stream=None):
@@ -164,18 +165,20 @@ class Kv4Cache:
         out_tok, out_head = _rows(out, "out", heads, self.head_dim)
         if q.shape[0] != out.shape[0] or q.dtype != out.dtype:
             raise ValueError("q and out must have the same rows and type")
-        b = self._batch(q.shape[0], q_start, kv_len, block_table, max_q)
         if max_kv is None:
             max_kv = min(block_table.shape[1] * self.page_size, 2 ** 31 - 1)
         ws, nws = 0, 0
         if workspace is not None:
             if not workspace.is_contiguous():      # (its bytes need not be there)
                 raise ValueError("workspace must be contiguous")
-            ws, nws = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        if self.lib.ember_cuda_kv4_attention(
-                self._p, b,
-                _pack(_ATT, q.data_ptr(), out.data_ptr(), _dtype(q, "q"), heads, q_tok, q_head, out_tok, out_head,
-                          self.head_dim ** -0.5 if scale is None else scale, max_kv, window, sinks, ws, nws), _on(stream, q)):
+            ws, nws = workspace.data_ptr(), workspace.nbytes
+        try:
+            batch = self._batch(q.shape[0], q_start, kv_len, block_table, max_q)
+            att = _ATT.pack(q.data_ptr(), out.data_ptr(), _dtype(q, "q"), heads, q_tok, q_head, out_tok, out_head,
+                            self.head_dim ** -0.5 if scale is None else scale, max_kv, window, sinks, ws, nws)
+        except struct.error as e:
+            raise _too_large(e) from None
+        if self.lib.ember_cuda_kv4_attention(self._p, batch, att, _on(stream, q)):
             _fail()
 
     def check(self, stream=None):
@@ -198,7 +201,7 @@ def sample_rows(logits, out, u, temperature=None, top_k=None, top_p=None, min_p=
     def opt(t, name, dtype=_F32):
         return 0 if t is None else _array(t, name, dtype, n)
     if lib.ember_cuda_sample_rows(
-            _pack(_SAMPLE, logits.data_ptr(), _dtype(logits, "logits"), n, logits.shape[1], logits.stride(0),
+            _SAMPLE.pack(logits.data_ptr(), _dtype(logits, "logits"), n, logits.shape[1], logits.stride(0),
                          opt(temperature, "temperature"), opt(top_p, "top_p"), opt(min_p, "min_p"),
                          _array(u, "u", _F32, n), opt(top_k, "top_k", _I32), _array(out, "out", _I32, n)), _on(stream, logits)):
         _fail()
