@@ -59,13 +59,4 @@ EMB_DEV Kv4Seq kv4_seq(const Kv4Rows &b, int i) {
     return s;
 }
 
-// the page of position pos (0 <= pos < cap), or -1
-EMB_DEV int kv4_page(const Kv4View &c, const Kv4Rows &b, int i, int pos) {
-    const int p = b.table[(size_t)i * b.table_stride + (pos >> c.page_shift)];
-    return (unsigned)p < (unsigned)c.n_pages ? p : -1;
-}
-EMB_DEV uint8_t *kv4_chunk_ptr(const Kv4View &c, int page, int head) {
-    return c.data + ((size_t)page * c.n_kv + head) * c.chunk;
-}
-
 }  // namespace emb

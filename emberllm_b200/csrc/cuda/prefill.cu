@@ -24,6 +24,7 @@
 #include <string.h>
 
 #include <mutex>
+#include <new>
 #include <vector>
 
 #include "ember_kv4.h"
@@ -988,19 +989,36 @@ extern "C" int ember_cuda_batch_new_kv4(EmberCudaModel *m, int n_streams, int ct
     if (max_steps < 1) return set_err("batch: max_steps must be positive");
     if (window < 0 || sinks < 0) return set_err("batch: window and sinks must not be negative");
     if (!pf_supported(m)) return set_err("batch: the model's layer weights are not all Q8_0 / Q4_0");
+    if (ctx < 1 || ctx > 0x7FFFFFFF - KV4_BATCH_PAGE) return set_err("batch: a context of %d is not supported", ctx);
     const int width = (ctx + KV4_BATCH_PAGE - 1) / KV4_BATCH_PAGE;
-    if (n_pages == 0) n_pages = (long long)width * n_streams > 0x7FFFFFFF ? -1 : width * n_streams;
+    if ((long long)width * n_streams > 1 << 28)
+        return set_err("batch: %d streams of %d positions are too many for a table of pages", n_streams, ctx);
+    if (n_pages == 0) n_pages = width * n_streams;
     const size_t layer = ember_cuda_kv4_bytes(n_pages, KV4_BATCH_PAGE, m->n_kv, m->head_dim);
     if (!layer)
         return set_err("batch: a 4-bit cache of %d pages, %d kv heads of %d is not supported", n_pages, m->n_kv, m->head_dim);
-    EmberCudaBatch *b = new EmberCudaBatch();
-    Kv4Streams *k = b->kv4 = new Kv4Streams();
+    EmberCudaBatch *b = new (std::nothrow) EmberCudaBatch();
+    Kv4Streams *k = new (std::nothrow) Kv4Streams();
+    bool room = b && k;
+    try {
+        if (room) {
+            k->h_table.assign((size_t)n_streams * width, -1);
+            k->held.assign(n_streams, 0);
+            k->h_idle.assign(n_streams, 0);
+            k->free.reserve(n_pages);
+            for (int i = n_pages - 1; i >= 0; i--) k->free.push_back(i);
+        }
+    } catch (const std::bad_alloc &) {
+        room = false;
+    }
+    if (!room) {
+        delete k;
+        delete b;
+        return set_err("batch: out of host memory");
+    }
+    b->kv4 = k;
     b->m = m; b->S = n_streams; b->ctx = ctx; b->max_steps = max_steps;
     k->width = width; k->window = window; k->sinks = sinks; k->layer = layer;
-    k->h_table.assign((size_t)n_streams * width, -1);
-    k->held.assign(n_streams, 0);
-    k->h_idle.assign(n_streams, 0);
-    for (int i = n_pages - 1; i >= 0; i--) k->free.push_back(i);
     const int hd = m->head_dim, rows = PF_CHUNK;
     const size_t n_rope = (size_t)ctx * (hd / 2) * sizeof(float2);
     int rc = pf_prepare_model(m) || pf_init(m->device) || pf_prepare_head(m) || pf_state_new(m, rows, &b->ps);
@@ -1014,7 +1032,8 @@ extern "C" int ember_cuda_batch_new_kv4(EmberCudaModel *m, int n_streams, int ct
         auto get = [&](void **p, size_t n) { return pf_alloc(b->allocs, p, n); };
         rc = get(&k->cache.data, layer * m->n_layers) || get((void **)&k->rope, n_rope) ||
              get((void **)&k->ctl, CTL_WORDS * 4) || get((void **)&k->ids, (size_t)rows * 4) ||
-             get((void **)&k->table, k->h_table.size() * 4) || get((void **)&k->len, (size_t)n_streams * 4) || get((void **)&k->idle, (size_t)n_streams * 4) ||
+             get((void **)&k->table, k->h_table.size() * 4) || get((void **)&k->len, (size_t)n_streams * 4) ||
+             get((void **)&k->idle, (size_t)n_streams * 4) ||
              get((void **)&k->one, 16) || get((void **)&k->kr, (size_t)rows * m->n_kv * hd * 4) ||
              get((void **)&k->vr, (size_t)rows * m->n_kv * hd * 4) || get((void **)&k->ao, (size_t)rows * m->n_heads * hd * 4) ||
              get(&k->ws, k->ws_bytes ? k->ws_bytes : 16) || get((void **)&b->tok, (size_t)n_streams * 4) ||

@@ -66,3 +66,21 @@ def test_drawn_steps_and_refusals(ember):
     for i, p in enumerate(ps):
         assert b.prefill(i, p) == firsts[i]
     b.close()
+
+
+def test_contexts_that_no_table_can_hold_are_refused(ember):
+    """at the C entry: a status, never an exception or an overflow"""
+    b = EmberBatch(ember, 1, ctx=64, max_steps=1, kv4=True)
+    lib = b.lib
+    model = ctypes.cast(ctypes.c_void_p(lib.ember_batch_cuda(b.b)), ctypes.POINTER(ctypes.c_void_p))[0]   # its first member
+    new, out = lib.ember_cuda_batch_new_kv4, ctypes.c_void_p(1)
+    new.argtypes = [ctypes.c_void_p] + [ctypes.c_int] * 5 + [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
+    rope = (ctypes.c_float * (64 * 64 * 2))()
+    for streams, ctx, pages in ((1, 0, 10), (2, -5, 10), (1, 2 ** 31 - 1, 10), (512, 2 ** 31 - 100, 10), (3, 2 ** 30, 0),
+                                (0, 64, 0), (513, 64, 0), (1, 64, -1), (1, 64, 2 ** 26)):
+        assert new(model, streams, ctx, pages, 0, 0, rope, 1, ctypes.byref(out)) == 1
+        assert out.value is None and b"batch" in lib.ember_cuda_error()
+    assert new(model, 2, 64, 0, 0, 0, rope, 1, ctypes.byref(out)) == 0 and out.value
+    lib.ember_cuda_batch_free.argtypes = [ctypes.c_void_p]
+    lib.ember_cuda_batch_free(out)
+    b.close()
