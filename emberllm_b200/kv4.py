@@ -112,10 +112,8 @@ class Kv4Cache:
         self._p = _CACHE.pack(buffer.data_ptr(), n_pages, page_size, n_kv_heads, head_dim)
 
     def _batch(self, tokens, q_start, kv_len, block_table, max_q):
-        if len(kv_len.shape) != 1:
-            raise ValueError(f"kv_len must have one dimension, not {len(kv_len.shape)}")
-        n = kv_len.shape[0]
-        ts = block_table.shape
+        n, ts = kv_len.shape, block_table.shape
+        n = n[0] if n else -1
         if len(ts) != 2 or ts[0] != n or _DT[block_table.dtype] != _I32:
             raise ValueError(f"block_table must be an int32 [{n}][pages] array")
         if not block_table.is_contiguous():

@@ -24,6 +24,7 @@ def test_a_workspace_with_holes(workspace):
 
 @pytest.mark.parametrize("change", [
     dict(q=torch.zeros(192)), dict(q=torch.zeros(3, 256)), dict(q=torch.zeros(1, 3, 4, 64)), dict(lens=torch.zeros(3, 1, dtype=I32)),
+    dict(lens=torch.tensor(3, dtype=I32)),
     dict(max_q=1 << 40), dict(max_kv=1 << 31), dict(window=1 << 31), dict(sinks=-1 << 40), dict(max_q=1.5)])
 def test_shapes_and_numbers_that_do_not_fit(change):
     with pytest.raises(ValueError):
