@@ -77,7 +77,7 @@ struct SrShared {
 
 EMB_DEV float sr_logit(float v) { return v != v ? -INFINITY : v; }
 
-// 2^(y/64) for -2000 < y <= 0: 2^(k/64) from the table, k the nearest integer, times
+// 2^(y/64) for -3000 < y <= 0 (the weights' limit is 31.25 / ln 2 * 64 = 2885): 2^(k/64) from the table, k the nearest integer, times
 // exp(f * ln2/64), |f| <= 1/2, by its Taylor polynomial of degree 4 (the next term is
 // below 4e-14, a weight's rounding 2.8e-14). 11 double-precision operations; the
 // library's exp takes some 30.
@@ -663,12 +663,19 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(EmberSampleR
     }
 }
 
+// logits of a CTA that shares an SM (228 KB, 1 KB of them the system's per CTA) with another
+constexpr int SR_SLICE_OF_TWO = (int)((228 * 1024 / 2 - 1024 - (sizeof(SrShared) + 15) / 16 * 16) / 4 / 8 * 8);
+static_assert(SR_SLICE_OF_TWO == 20040, "the rule's comment names it");
+
 template <typename T>
 static int sample_rows_launch(const EmberSampleRows &a, int n_sm, cudaStream_t st) {
     constexpr int W = 16 / sizeof(T);
-    // as few CTAs a row as hold it with two of them on an SM, more while SMs are idle
+    // As few CTAs a row as hold it with two of them on an SM, more while SMs are idle. Us for 512 /
+    // 148 rows, one CTA an SM and two: 20,480 tokens 68 / 23 and 66 / 23, 40,960 138 / 44 and 133 / 48,
+    // 81,920 315 / 96 and 294 / 92. Above 8 x 20,040 tokens there is no choice: 430 at 160,000, 691 at
+    // 163,840.
     int nc = 1;
-    while (nc < SR_MAX_CLUSTER && (a.vocab + nc - 1) / nc > 20480) nc *= 2;
+    while (nc < SR_MAX_CLUSTER && (a.vocab + nc - 1) / nc > SR_SLICE_OF_TWO) nc *= 2;
     while (nc < SR_MAX_CLUSTER && (long long)a.n_rows * nc * 2 <= n_sm && a.vocab / (nc * 2) >= 2048) nc *= 2;
     const int slice = (a.vocab + nc * W - 1) / (nc * W) * W;
     const size_t smem = (sizeof(SrShared) + 15) / 16 * 16 + (size_t)slice * 4;
