@@ -825,7 +825,7 @@ static int kv4_prompt_launch(const Kv4AttnArgs &a, cudaStream_t st) {
 template <typename T, int RT>
 static int kv4_prompt_hd(const Kv4AttnArgs &a, int hd, cudaStream_t st) {
     switch (hd) {
-    case 32: return kv4_prompt_launch<T, 32, RT>(a, st);
+    case 32: return kv4_prompt_launch<T, 32, sizeof(T) == 2 ? 1 : RT>(a, st);    // (fp16: one row tile always)
     case 64: return kv4_prompt_launch<T, 64, RT>(a, st);
     default: return kv4_prompt_launch<T, 128, RT>(a, st);
     }

@@ -4,6 +4,7 @@ positions that no row sees."""
 import pytest
 
 from .test_kv4 import Paged
+from .test_kv4_many_rows import MANY_1, kernel
 
 torch = pytest.importorskip("torch")
 
@@ -32,8 +33,9 @@ def ramp(p):
 @pytest.mark.parametrize("kv,ql,heads,kvh,hd", [
     ([700, 150], [1, 1], 16, 8, 128), ([600, 90], [3, 2], 14, 2, 64),                      # few rows
     ([700, 520], [700, 520], 16, 8, 128), ([900], [900], 9, 3, 64), ([640] * 3, [400] * 3, 8, 1, 32),   # many
-    ([500], [300], 16, 8, 128)])
+    ([500], [330], 16, 8, 128)])
 def test_other_rows_queries_change_nothing(dtype, kv, ql, heads, kvh, hd):
+    assert (kernel(dtype, max(ql), heads, kvh, hd, len(kv)) >= MANY_1) == (max(ql) > 3)
     p = Paged(kv, ql, 32, kvh, hd, seed=1)
     ramp(p)
     n = sum(ql)
@@ -65,6 +67,7 @@ def test_other_rows_queries_change_nothing(dtype, kv, ql, heads, kvh, hd):
 def test_positions_that_nobody_sees_need_not_be_written(dtype, window, sinks, kv, ql, heads, kvh, hd):
     """a program that keeps the first tokens and a window writes nothing else: the
     other bytes are NaN scales here, in the same pages and groups"""
+    assert (kernel(dtype, max(ql), heads, kvh, hd, len(kv)) >= MANY_1) == (max(ql) > 3)
     p = Paged(kv, ql, 64, kvh, hd, seed=window)
     p.store_all()
     q = (torch.randn(sum(ql), heads, hd, generator=torch.Generator().manual_seed(3)) * 1.2).to(dtype).cuda()

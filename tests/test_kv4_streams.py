@@ -14,7 +14,7 @@ def test_arrays_that_torch_has_on_the_host_or_does_not_know():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("ql", [1, 300])
+@pytest.mark.parametrize("ql", [1, 330])
 def test_calls_wait_for_the_current_stream(ql):
     p = Paged([400], [ql], 64, 8, 128, seed=1)
     g = torch.Generator().manual_seed(2)

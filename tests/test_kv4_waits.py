@@ -41,7 +41,7 @@ def test_a_wait_that_runs_out_is_reported(monkeypatch, shape, dtype):
 
 @pytest.mark.gpu
 def test_a_prompt_whose_wait_runs_out_fails(monkeypatch):
-    assert kernel(torch.float32, 512, 16, 8, 1) == MANY_1
+    assert kernel(torch.float32, 512, 16, 8, 64, 1) == MANY_1
     monkeypatch.setitem(synth.CONFIGS, "tiny-heads", dict(
         dim=256, hidden_dim=512, n_layers=2, n_heads=16, n_kv_heads=8, head_dim=64, vocab_size=512, max_seq_len=2048,
         rope_theta=1e6, norm_eps=1e-6, rope_style=synth.ROPE_NEOX, tied=True, qk_norm=True, bias=False, quant="q8_0"))
