@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(KV4_IO_THREADS) kv4_io_kernel(Kv4View c, Kv4Ro
 
 template <typename T>
 static int kv4_attention_launch(const Kv4AttnArgs &a, int hd, cudaStream_t st) {
-    switch (kv4_kernel(sizeof(T), hd, a.max_q, a.group, a.c.n_kv, a.b.n_seqs)) {
+    switch (kv4_kernel(sizeof(T), hd, a.b.n_tokens, a.max_q, a.group, a.c.n_kv, a.b.n_seqs)) {
     case KV4_FEW_4: return kv4_decode_hd<T, 1>(a, hd, st);
     case KV4_FEW_8: return kv4_decode_hd<T, 2>(a, hd, st);
     case KV4_MANY_1: return kv4_prompt_hd<T, 1>(a, hd, st);

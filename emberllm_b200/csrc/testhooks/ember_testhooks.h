@@ -35,7 +35,8 @@ int ember_testhook_wait_timeout(int mode, unsigned tries, int *ok_out, int *err_
 
 /* The kernel that an attention call over the paged 4-bit cache takes (kv4_rule.h):
  * 1, 2 few rows (4, 8 at a time), 3, 4 many rows (one, two row tiles a CTA). */
-int ember_testhook_kv4_kernel(int elem_bytes, int head_dim, int max_q, int group, int n_kv, int n_seqs);
+int ember_testhook_kv4_kernel(int elem_bytes, int head_dim, int n_tokens, int max_q, int group, int n_kv,
+                              int n_seqs);
 
 #ifdef __cplusplus
 }

@@ -102,7 +102,7 @@ int ember_cuda_kv4_read(const EmberKv4Cache *cache, const EmberKv4Batch *batch, 
  * They keep partial sums in `out` while they run.
  * The same call gives the same bits. A row's result does not depend on its
  * neighbours in the batch; in the last bits it depends on how the cache is cut into
- * pieces, which follows from n_seqs, max_q, max_kv, window and sinks.
+ * pieces, which follows from n_tokens, n_seqs, max_q, max_kv, window and sinks.
  *
  * max_kv bounds kv_len (positions behind it are not looked at). workspace: device
  * memory of at least ember_cuda_kv4_attention_workspace() bytes, 16-byte aligned,

@@ -19,16 +19,17 @@ FEW_4, FEW_8, MANY_1, MANY_2 = 1, 2, 3, 4
 F32, F16 = torch.float32, torch.float16
 
 
-def kernel(dtype, max_q, heads, kvh, hd, seqs):
+def kernel(dtype, max_q, heads, kvh, hd, seqs, tokens=None):
     hooks = H.testhooks()
-    return hooks.ember_testhook_kv4_kernel(4 if dtype == F32 else 2, hd, max_q, heads // kvh, kvh, seqs)
+    return hooks.ember_testhook_kv4_kernel(4 if dtype == F32 else 2, hd, tokens or seqs * max_q, max_q, heads // kvh, kvh,
+                                           seqs)
 
 
 # heads, kv heads, head_dim, rows a sequence at most, sequences; the kernel they take (fp16 heads of 32: one
 # row tile always)
 SHAPES = {
-    "128-1": (16, 8, 128, 108, 3, MANY_1), "64-1": (14, 2, 64, 123, 3, MANY_1), "32-1": (9, 3, 32, 192, 3, MANY_1),
-    "128-2": (16, 8, 128, 400, 3, MANY_2), "64-2": (14, 2, 64, 550, 6, MANY_2), "32-2": (16, 8, 32, 520, 6, MANY_2),
+    "128-1": (16, 8, 128, 108, 3, MANY_1), "64-1": (14, 2, 64, 126, 3, MANY_1), "32-1": (9, 3, 32, 192, 3, MANY_1),
+    "128-2": (16, 8, 128, 400, 3, MANY_2), "64-2": (14, 2, 64, 580, 6, MANY_2), "32-2": (16, 8, 32, 520, 6, MANY_2),
 }
 ALL = [pytest.param(s, d, id=f"{s}-{'f32' if d == F32 else 'f16'}") for s in SHAPES for d in (F32, F16)]
 
@@ -36,8 +37,8 @@ ALL = [pytest.param(s, d, id=f"{s}-{'f32' if d == F32 else 'f16'}") for s in SHA
 def make(shape, dtype, fill=0xAB, page=32, more=(3, 250, 0, 1000, 64, 17), short=(0, 7, 1, 0, 33, 2)):
     """ragged sequences of that shape: some rows and positions fewer or more each"""
     heads, kvh, hd, ql, seqs, want = SHAPES[shape]
-    assert kernel(dtype, ql, heads, kvh, hd, seqs) == (MANY_1 if hd == 32 and dtype == F16 else want)
     q = [ql - short[i] for i in range(seqs)]
+    assert kernel(dtype, ql, heads, kvh, hd, seqs, sum(q)) == (MANY_1 if hd == 32 and dtype == F16 else want)
     p = Paged([n + more[i] for i, n in enumerate(q)], q, page, kvh, hd, seed=hd + ql, fill=fill)
     p.store_all()
     assert max(p.ql) == ql
@@ -63,6 +64,8 @@ def test_which_kernel():
     assert k(32, 16, 8, 128, 8) == FEW_8 and k(64, 16, 8, 128, 8) == MANY_1 and k(32, 16, 8, 128, 64) == MANY_1
     assert k(512, 16, 8, 128, 1) == MANY_1 and k(512, 16, 8, 128, 4) == MANY_2 and k(4000, 16, 8, 128, 1) == MANY_2
     assert kernel(F16, 512, 16, 8, 128, 1) == MANY_2 and kernel(F16, 512, 14, 2, 64, 2) == MANY_1
+    # a prompt among single tokens, ragged prompts
+    assert k(256, 16, 8, 128, 64, 319) == FEW_8 and k(512, 16, 8, 128, 6, 1500) == MANY_2
     assert kernel(F16, 2000, 8, 1, 32, 8) == MANY_1 and k(2000, 8, 1, 32, 8) == MANY_2
 
 
@@ -276,6 +279,20 @@ def test_few_rows_are_as_exact(kv, ql, heads, kvh, hd, seqs):
     q = (torch.randn(ql * seqs, heads, hd, generator=torch.Generator().manual_seed(2)) * 1.2).cuda()
     got, want = p.attend(q), p.want(q)
     assert (got.double() - want).norm() / want.norm() < 1.5e-6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("heads,kvh,hd", [(16, 8, 128), (9, 3, 64)])
+def test_prompts_among_single_tokens(dtype, heads, kvh, hd):
+    """a step of many streams in which some start: both kernels take such batches"""
+    for ql, want in (([1] * 20 + [256] + [1] * 20 + [0, 3], (FEW_8,)), ([1] * 5 + [600, 700, 1, 800], (MANY_1, MANY_2))):
+        kv = [n + (97 * i) % 1500 for i, n in enumerate(ql)]
+        p = Paged(kv, ql, 64, kvh, hd, seed=3)
+        p.store_all()
+        q = (torch.randn(sum(ql), heads, hd, generator=torch.Generator().manual_seed(2)) * 1.2).to(dtype).cuda()
+        assert kernel(dtype, max(ql), heads, kvh, hd, len(ql), sum(ql)) in want
+        near(p.attend(q), p.want(q))
 
 
 # ---- the framework's own prompts in it ----

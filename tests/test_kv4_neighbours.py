@@ -35,7 +35,7 @@ def ramp(p):
     ([700, 520], [700, 520], 16, 8, 128), ([900], [900], 9, 3, 64), ([640] * 3, [400] * 3, 8, 1, 32),   # many
     ([500], [330], 16, 8, 128)])
 def test_other_rows_queries_change_nothing(dtype, kv, ql, heads, kvh, hd):
-    assert (kernel(dtype, max(ql), heads, kvh, hd, len(kv)) >= MANY_1) == (max(ql) > 3)
+    assert (kernel(dtype, max(ql), heads, kvh, hd, len(kv), sum(ql)) >= MANY_1) == (max(ql) > 3)
     p = Paged(kv, ql, 32, kvh, hd, seed=1)
     ramp(p)
     n = sum(ql)
@@ -67,7 +67,7 @@ def test_other_rows_queries_change_nothing(dtype, kv, ql, heads, kvh, hd):
 def test_positions_that_nobody_sees_need_not_be_written(dtype, window, sinks, kv, ql, heads, kvh, hd):
     """a program that keeps the first tokens and a window writes nothing else: the
     other bytes are NaN scales here, in the same pages and groups"""
-    assert (kernel(dtype, max(ql), heads, kvh, hd, len(kv)) >= MANY_1) == (max(ql) > 3)
+    assert (kernel(dtype, max(ql), heads, kvh, hd, len(kv), sum(ql)) >= MANY_1) == (max(ql) > 3)
     p = Paged(kv, ql, 64, kvh, hd, seed=window)
     p.store_all()
     q = (torch.randn(sum(ql), heads, hd, generator=torch.Generator().manual_seed(3)) * 1.2).to(dtype).cuda()

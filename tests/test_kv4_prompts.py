@@ -48,7 +48,7 @@ def test_single_precision_sums_at_any_length(kv, ql, heads, kvh, hd, window, sin
     segment's: 2.5e-6. The scores' own cuts (16 of sums of a few units, of both
     signs), 22 bits of queries and weights and the exponentials add less than 1.5e-6.
     (Sums that stay are off by 4.8e-5 at 20,000 positions.)"""
-    assert kernel(torch.float32, max(ql), heads, kvh, hd, len(kv)) >= MANY_1
+    assert kernel(torch.float32, max(ql), heads, kvh, hd, len(kv), sum(ql)) >= MANY_1
     p = Paged(kv, ql, 64, kvh, hd, seed=hd)
     p.store_all()
     q = queries(sum(ql), heads, hd)
@@ -68,7 +68,7 @@ def test_single_precision_sums_at_any_length(kv, ql, heads, kvh, hd, window, sin
                                                 ([3001], [3001], 12, 12, 64), ([4000, 2500], [900, 2500], 16, 8, 128)])
 def test_long_ranges_again_and_again(dtype, kv, ql, heads, kvh, hd):
     """many runs give the first one's bits where sums leave tensor memory many times"""
-    assert kernel(dtype, max(ql), heads, kvh, hd, len(kv)) >= MANY_1
+    assert kernel(dtype, max(ql), heads, kvh, hd, len(kv), sum(ql)) >= MANY_1
     p = Paged(kv, ql, 64, kvh, hd, seed=hd)
     p.store_all()
     q = queries(sum(ql), heads, hd, dtype=dtype)
