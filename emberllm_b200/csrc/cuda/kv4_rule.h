@@ -28,8 +28,11 @@ enum { KV4_TILE_ROWS = 128 };
 //                  fp16  64 pairs 26 / 35, 250 89 / 91, 504 94 / 100, 576 108 / 115: never
 //
 // The host knows the longest sequence's rows and the batch's: groups of rows are no more than either
-// allows (64 sequences of 2000 positions, one with 256 rows and the others with one: 301 us in the kernel
-// for many, which the longest alone would choose, 146 in the one for few).
+// allows. 64 sequences of 2000 positions, one with 256 rows and the others with one: 147 us in the
+// kernel for few, 248 in the one for many, which the longest alone would choose; 512 of 1000, one
+// with 512: 908 / 1108. The kernel for few has a CTA for every eight rows that any sequence could have: too
+// many that are empty cost more (201 sequences of 2000, one with 2000 rows, 134 times the groups: 1510 /
+// 963), and a grid has its limits.
 static inline long long kv4_groups(int size, int n_tokens, int max_q, int group, int n_kv, int n_seqs) {
     const long long each = ((long long)max_q * group + size - 1) / size * n_seqs;
     const long long all = (long long)n_tokens * group / size + n_seqs;
@@ -40,7 +43,10 @@ static inline int kv4_kernel(int elem_bytes, int head_dim, int n_tokens, int max
     const long long rows = (long long)max_q * group;
     const long long eights = kv4_groups(8, n_tokens, max_q, group, n_kv, n_seqs);
     const long long tiles = kv4_groups(KV4_TILE_ROWS, n_tokens, max_q, group, n_kv, n_seqs);
-    if (eights <= (f32 ? 640 : 560) * (tiles > 128 ? tiles : 128) / 128) return rows <= 4 ? KV4_FEW_4 : KV4_FEW_8;
+    const long long chunks = (rows + 7) / 8 * n_kv, ctas = chunks * n_seqs;
+    if (eights <= (f32 ? 640 : 560) * (tiles > 128 ? tiles : 128) / 128 && ctas <= 100 * eights && chunks <= 65535 &&
+        ctas <= 0x7FFFFFFF)
+        return rows <= 4 ? KV4_FEW_4 : KV4_FEW_8;
     const long long pairs = kv4_groups(2 * KV4_TILE_ROWS, n_tokens, max_q, group, n_kv, n_seqs);
     if (rows <= KV4_TILE_ROWS || (head_dim == 32 && !f32)) return KV4_MANY_1;
     return pairs >= (head_dim == 128 ? (f32 ? 96 : 32) : head_dim == 64 ? (f32 ? 160 : 192) : 200) ? KV4_MANY_2 : KV4_MANY_1;

@@ -64,7 +64,9 @@ def test_which_kernel():
     assert k(32, 16, 8, 128, 8) == FEW_8 and k(64, 16, 8, 128, 8) == MANY_1 and k(32, 16, 8, 128, 64) == MANY_1
     assert k(512, 16, 8, 128, 1) == MANY_1 and k(512, 16, 8, 128, 4) == MANY_2 and k(4000, 16, 8, 128, 1) == MANY_2
     assert kernel(F16, 512, 16, 8, 128, 1) == MANY_2 and kernel(F16, 512, 14, 2, 64, 2) == MANY_1
-    # a prompt among single tokens, ragged prompts
+    # a prompt among single tokens, ragged prompts, grids that would be empty or too large
+    assert k(2000, 16, 8, 128, 201, 2200) >= MANY_1 and k(200000, 8, 8, 128, 4096, 237000) >= MANY_1
+    assert k(4000, 16, 8, 128, 65535, 70000) >= MANY_1 and k(1, 16, 8, 128, 65535) == FEW_4
     assert k(256, 16, 8, 128, 64, 319) == FEW_8 and k(512, 16, 8, 128, 6, 1500) == MANY_2
     assert kernel(F16, 2000, 8, 1, 32, 8) == MANY_1 and k(2000, 8, 1, 32, 8) == MANY_2
 
