@@ -4,7 +4,6 @@
 #include <cuda_runtime.h>
 
 #include <math.h>
-#include <stdlib.h>
 
 #include "kv4.cuh"
 #include "kv4_prompt.cuh"
@@ -255,12 +254,12 @@ __global__ void __launch_bounds__(KV4_IO_THREADS) kv4_io_kernel(Kv4View c, Kv4Ro
 }
 
 template <typename T>
-static int kv4_attention_launch(const Kv4AttnArgs &a, int hd, cudaStream_t st) {
+static int kv4_attention_launch(const Kv4AttnArgs &a, int hd, int *err, cudaStream_t st) {
     switch (kv4_kernel(sizeof(T), hd, a.b.n_tokens, a.max_q, a.group, a.c.n_kv, a.b.n_seqs)) {
     case KV4_FEW_4: return kv4_decode_hd<T, 1>(a, hd, st);
     case KV4_FEW_8: return kv4_decode_hd<T, 2>(a, hd, st);
-    case KV4_MANY_1: return kv4_prompt_hd<T, 1>(a, hd, st);
-    default: return kv4_prompt_hd<T, 2>(a, hd, st);
+    case KV4_MANY_1: return kv4_prompt_hd<T, 1>(a, hd, err, st);
+    default: return kv4_prompt_hd<T, 2>(a, hd, err, st);
     }
 }
 
@@ -455,13 +454,8 @@ int emb::kv4_attention(const EmberKv4Cache *cache, const EmberKv4Batch *batch, c
     a.n_heads = att->n_heads; a.group = att->n_heads / c.n_kv;
     a.scale = att->scale; a.max_kv = max_kv; a.max_q = max_q; a.window = att->window; a.sinks = att->sinks;
     a.ws = (float *)att->workspace;
-    a.err = err;
-    // tests: keys that never arrive, and so many us until the waits for them run out
-    const char *us = getenv("EMBER_KV4_LOST_KEYS_US");
-    a.lost = us != nullptr;
-    a.wait_ns = us ? strtoull(us, nullptr, 10) * 1000ull : KP_WAIT_NS;
-    return att->dtype == EMBER_DT_F32 ? kv4_attention_launch<float>(a, hd, st)
-                                      : kv4_attention_launch<__half>(a, hd, st);
+    return att->dtype == EMBER_DT_F32 ? kv4_attention_launch<float>(a, hd, err, st)
+                                      : kv4_attention_launch<__half>(a, hd, err, st);
 }
 
 extern "C" int ember_cuda_kv4_attention(const EmberKv4Cache *cache, const EmberKv4Batch *batch,

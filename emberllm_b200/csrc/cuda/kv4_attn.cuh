@@ -48,9 +48,6 @@ struct Kv4AttnArgs {
     int chunks;                   // row chunks per kv head
     int span, parts;              // units of a CTA; CTAs of the longest sequence
     float *ws;
-    int *err;                     // error word for waits that run out (NULL: the device's own)
-    unsigned long long wait_ns;
-    int lost;                     // 1: the keys' arrivals never suffice (tests of the waits)
 };
 
 constexpr int KD_WARPS = 4;

@@ -34,6 +34,8 @@
 // positions, fp32: 66 us.
 #pragma once
 
+#include <stdlib.h>
+
 #include "kv4_attn.cuh"
 #include "kv4_rule.h"
 
@@ -67,6 +69,15 @@ struct KpLayout {
     static constexpr int KN = NP / 8 / KEY_WARPS;           // positions a key thread unpacks
     static_assert(SB * NP == 128, "scores take 128 columns");
     static_assert(SMEM <= (RT == 2 ? 227 : 113) * 1024, "shared memory");
+};
+
+// what the many-row kernel takes besides (apart: 24 bytes more cost the other kernel's launch 0.6 us of
+// the host)
+struct KpArgs {
+    Kv4AttnArgs att;
+    int *err;                     // error word for waits that run out (NULL: the device's own)
+    unsigned long long wait_ns;
+    int lost;                     // 1: the keys' arrivals never suffice (tests of the waits)
 };
 
 template <int RT>
@@ -190,7 +201,8 @@ EMB_DEV KpRange<NP> kp_range(int first_pos, int last_pos, int len, int window, i
 }
 
 template <typename T, int HD, int RT>
-__global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_prompt_kernel(const Kv4AttnArgs a) {
+__global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_prompt_kernel(const KpArgs args) {
+    const Kv4AttnArgs &a = args.att;
     using L = KpLayout<T, HD, RT>;
     constexpr int NB = HD / 32, GB = kv4_group(HD), PARTS = L::PARTS, BUF = L::BUF, NP = L::NP, H = L::H, SB = L::SB;
     extern __shared__ uint8_t kp_raw[];
@@ -213,7 +225,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
 
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(&sh.k_full[i], 32 * L::KEY_WARPS + a.lost);
+            mbar_init(&sh.k_full[i], 32 * L::KEY_WARPS + args.lost);
             mbar_init(&sh.k_empty[i], tiles);
             mbar_init(&sh.v_full[i], 64);
             mbar_init(&sh.v_empty[i], tiles);
@@ -236,7 +248,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
     const uint32_t tmem = sh.tmem;
     volatile int *abort = &sh.abort;
     auto kp_wait = [&](uint64_t *bar, uint32_t parity, volatile int *flag) {
-        return kp_wait_ns(bar, parity, flag, a.wait_ns);
+        return kp_wait_ns(bar, parity, flag, args.wait_ns);
     };
 
     if (warp < L::SOFT) {
@@ -797,7 +809,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
     __syncwarp();
     __syncthreads();
     kp_fence_after();
-    if (tid == 0 && *abort) atomicExch(a.err ? a.err : &kv4_wait_error, ERR_KV4_WAIT);
+    if (tid == 0 && *abort) atomicExch(args.err ? args.err : &kv4_wait_error, ERR_KV4_WAIT);
     if (warp == L::ISSUE)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)L::COLS) : "memory");
 }
@@ -805,7 +817,10 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
 // ------------------------------------------------------------------- host ----
 
 template <typename T, int HD, int RT>
-static int kv4_prompt_launch(const Kv4AttnArgs &a, cudaStream_t st) {
+static int kv4_prompt_launch(const Kv4AttnArgs &a, int *err, cudaStream_t st) {
+    // tests: keys that never arrive, and so many us until the waits for them run out
+    const char *us = getenv("EMBER_KV4_LOST_KEYS_US");
+    const KpArgs args = { a, err, us ? strtoull(us, nullptr, 10) * 1000ull : KP_WAIT_NS, us != nullptr };
     using L = KpLayout<T, HD, RT>;
     static std::atomic<unsigned long long> ready{0};      // devices whose limit is raised
     int dev = 0;
@@ -817,17 +832,17 @@ static int kv4_prompt_launch(const Kv4AttnArgs &a, cudaStream_t st) {
     const long long tiles = ((long long)a.max_q * a.group + RT * KP_ROWS - 1) / (RT * KP_ROWS);
     if (tiles > 65535) return set_err("kv4 attention: max_q %d is too large", a.max_q);
     const dim3 grid((unsigned)a.c.n_kv, (unsigned)a.b.n_seqs, (unsigned)tiles);
-    kv4_prompt_kernel<T, HD, RT><<<grid, 32 * L::WARPS, L::SMEM, st>>>(a);
+    kv4_prompt_kernel<T, HD, RT><<<grid, 32 * L::WARPS, L::SMEM, st>>>(args);
     CK(cudaGetLastError());
     return 0;
 }
 
 template <typename T, int RT>
-static int kv4_prompt_hd(const Kv4AttnArgs &a, int hd, cudaStream_t st) {
+static int kv4_prompt_hd(const Kv4AttnArgs &a, int hd, int *err, cudaStream_t st) {
     switch (hd) {
-    case 32: return kv4_prompt_launch<T, 32, sizeof(T) == 2 ? 1 : RT>(a, st);    // (fp16: one row tile always)
-    case 64: return kv4_prompt_launch<T, 64, RT>(a, st);
-    default: return kv4_prompt_launch<T, 128, RT>(a, st);
+    case 32: return kv4_prompt_launch<T, 32, sizeof(T) == 2 ? 1 : RT>(a, err, st);    // (fp16: one row tile always)
+    case 64: return kv4_prompt_launch<T, 64, RT>(a, err, st);
+    default: return kv4_prompt_launch<T, 128, RT>(a, err, st);
     }
 }
 

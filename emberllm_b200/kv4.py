@@ -52,7 +52,8 @@ def _on(stream, t):
         # (the public call makes an object of the stream: a microsecond more)
         _torch = m.Tensor, getattr(m._C, "_cuda_getCurrentRawStream",
                                    lambda i: m.cuda.current_stream(i).cuda_stream)
-    return _torch[1](t.device.index) if isinstance(t, _torch[0]) and t.is_cuda else 0
+    device = t.get_device() if isinstance(t, _torch[0]) else -1
+    return _torch[1](device) if device >= 0 else 0
 
 
 def _fail():
@@ -156,12 +157,11 @@ class Kv4Cache:
         cache into ``out``; ``window`` > 0 limits it to the last ``window`` positions
         and the first ``sinks``. ``max_kv`` bounds kv_len (default: all the block table
         can hold), ``scale`` defaults to head_dim ** -0.5."""
-        if len(q.shape) != 3:
-            raise ValueError(f"q must be [rows][heads][{self.head_dim}], not {list(q.shape)}")
-        heads = q.shape[1]
+        shape = q.shape
+        heads = shape[1] if len(shape) > 1 else 0
         q_tok, q_head = _rows(q, "q", heads, self.head_dim)
         out_tok, out_head = _rows(out, "out", heads, self.head_dim)
-        if q.shape[0] != out.shape[0] or q.dtype != out.dtype:
+        if shape[0] != out.shape[0] or q.dtype != out.dtype:
             raise ValueError("q and out must have the same rows and type")
         if max_kv is None:
             max_kv = min(block_table.shape[1] * self.page_size, 2 ** 31 - 1)
@@ -171,7 +171,7 @@ class Kv4Cache:
                 raise ValueError("workspace must be contiguous")
             ws, nws = workspace.data_ptr(), workspace.nbytes
         try:
-            batch = self._batch(q.shape[0], q_start, kv_len, block_table, max_q)
+            batch = self._batch(shape[0], q_start, kv_len, block_table, max_q)
             att = _ATT.pack(q.data_ptr(), out.data_ptr(), _dtype(q, "q"), heads, q_tok, q_head, out_tok, out_head,
                             self.head_dim ** -0.5 if scale is None else scale, max_kv, window, sinks, ws, nws)
         except struct.error as e:
