@@ -11,7 +11,7 @@
 //   1 per row tile   issues its products: S = Q K^T and O += P V with P from tensor
 //        memory. One warp for both row tiles kept either waiting on the other's softmax,
 //        a warp that unpacks as well was waited for by all (6,900 and more cycles a tile for
-//        what now takes some 4,400)
+//        what then took 4,400; 5,300 with weights in two parts)
 //   2 values, 4 (1) keys   packed codes from global memory, asked for a tile ahead, to
 //        exact fp16 numbers (code - 8) * d in shared memory, swizzled as the products read
 //        them; the values are transposed on the way, so both operands are K-major
@@ -29,9 +29,9 @@
 // 2.4e-4 and more.
 //
 // Bound by the chain scores - maximum - exponentials - weights - outputs of a row tile: tensor
-// pipe, exponentials and conversions are each busy a third of the time. Two prompts of 3.9-4.1k,
-// 16 / 8 heads of 128, fp16: 241 us, 563 TFLOP/s; six of up to 512 rows on up to 1200
-// positions, fp32: 66 us.
+// pipe 44 %, alu 40 %, exponentials 30 %, issue 50 % busy. Two prompts of 3.9-4.1k, 16 / 8 heads of
+// 128, fp16: 244 us, 556 TFLOP/s; six of up to 512 rows on up to 1200 positions, fp32: 66 us. One
+// row tile spills up to 48 bytes stored and 96 loaded a thread, two up to 8 and 20.
 #pragma once
 
 #include <stdlib.h>
@@ -92,7 +92,8 @@ struct KpShared {
 // Wait for a phase; gives up after `ns` of waiting or as soon as another role has given up, so
 // that a product that never completes ends the CTA (its rows become NaN, the error word says
 // so). A poll counts as a millisecond at most: a process that the GPU was taken from for a while has not
-// waited. (The polling is a function of its own: inlined in all places it cost two prompts of 4k in fp16 250 us instead of 241.)
+// waited. (The polling is a function of its own: inlined in all places, two prompts of 4k in fp16 took
+// 250 us instead of 241.)
 static __device__ __noinline__ bool kp_poll(uint32_t bar, uint32_t parity, volatile int *abort, unsigned long long ns) {
     unsigned long long t0, t1;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));

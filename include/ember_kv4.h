@@ -165,12 +165,15 @@ int ember_cuda_sample_rows(const EmberSampleRows *args, void *stream);
  * quantized, so tokens may differ from those over an fp32 or fp16 cache; attention is
  * ember_cuda_kv4_attention's, with `window` and `sinks`. Any n_streams in [1, 512];
  * head_dim 32, 64 or 128. prefill, greedy, sample and free take such a batch as any
- * other. A call that finds no free page fails and leaves the streams as they were
+ * other. What other streams hold or do has no part in a stream's results; past 512
+ * positions the last bits of its attention depend on n_streams, which decides how a cache
+ * is cut into pieces.
+ * A call that finds no free page fails and leaves the streams as they were
  * (pages handed out before it found out stay with their streams). Pages behind the
  * window stay, too.
  * release gives a stream's pages back and leaves it idle until its next prompt, which
- * starts anew: greedy and sample go on without it. Its toks, pos, params and u are not looked at
- * then, it takes no page, its tokens are -1 and its logits 0. */
+ * starts anew: greedy and sample go on without it. Its toks, pos, params and u are not
+ * looked at then, it takes no page, its tokens are -1 and its logits 0. */
 int ember_cuda_batch_new_kv4(EmberCudaModel *m, int n_streams, int ctx, int n_pages, int window, int sinks,
                              const float *rope_cs, int max_steps, EmberCudaBatch **out);
 int ember_cuda_batch_release(EmberCudaBatch *b, int stream);
