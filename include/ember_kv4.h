@@ -99,7 +99,7 @@ int ember_cuda_kv4_read(const EmberKv4Cache *cache, const EmberKv4Batch *batch, 
  * and outputs accumulate in fp32. Many-row calls (prompts) add on the tensor cores,
  * which cut toward zero: 2.5e-9 of an output a position, for fp32 over 512 positions
  * at most (1.6e-6 of an output at any length), for fp16 over all (1e-4 at 40,000).
- * They keep partial sums in `out` while they run.
+ * They keep partial sums in `out` while they run. out may be q itself.
  * The same call gives the same bits. A row's result does not depend on its
  * neighbours in the batch; in the last bits it depends on how the cache is cut into
  * pieces, which follows from n_tokens, n_seqs, max_q, max_kv, window and sinks.

@@ -76,3 +76,38 @@ def test_long_ranges_again_and_again(dtype, kv, ql, heads, kvh, hd):
     assert relative(first, p.want(q)) < (4e-6 if dtype == torch.float32 else 2.5e-4)
     for _ in range(60):
         assert torch.equal(p.attend(q), first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv,ql,heads,kvh,hd", [([6000] * 3, [400] * 3, 8, 1, 32), ([9000], [1301], 9, 3, 64), ([5000], [350], 16, 8, 128),
+                                                ([3001], [3001], 12, 12, 64), ([4000, 2500], [900, 2500], 16, 8, 128)])
+def test_sums_under_a_maximum_that_rises(kv, ql, heads, kvh, hd):
+    """Scores from -25 to 25 along the sequence: the running maximum is raised some nine
+    times, between the times at which the sums leave tensor memory and at them. A score's
+    sum is cut 16 times and has 22 bits of its query: off by 25 * 20 * 2^-24 = 3e-5 at
+    most, numerator and denominator twice that."""
+    assert kernel(torch.float32, max(ql), heads, kvh, hd, len(kv), sum(ql)) >= MANY_1
+    p = Paged(kv, ql, 64, kvh, hd, seed=hd)
+    at = 0
+    for n in kv:
+        p.k[at:at + n, :, :32] = torch.linspace(-1, 1, n, device="cuda")[:, None, None]
+        at += n
+    p.store_all()
+    q = queries(sum(ql), heads, hd, scale=0.5)
+    q[..., :32] = 25 / 32 * hd ** 0.5
+    got = p.attend(q)
+    assert relative(got, p.want(q)) < 6e-5
+    assert torch.equal(p.attend(q), got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("kv,ql,heads,kvh,hd", [([2000, 700], [330, 600], 16, 8, 128), ([9000], [1301], 9, 3, 64), ([3000] * 4, [1] * 4, 16, 8, 128),
+                                                ([20000], [5], 14, 2, 64)])
+def test_outputs_in_place_of_the_queries(dtype, kv, ql, heads, kvh, hd):
+    p = Paged(kv, ql, 64, kvh, hd, seed=hd)
+    p.store_all()
+    q = queries(sum(ql), heads, hd, dtype=dtype)
+    want = p.attend(q)
+    p.attend(q, out=q)
+    assert torch.equal(q, want)
