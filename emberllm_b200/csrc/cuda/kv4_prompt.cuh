@@ -395,6 +395,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
                         for (int e = 0; e < 4; e++) w[k + e] = __ldcg(at[k / 4] + e);
                     }
                 }
+                __syncwarp();         // (the loads were some lanes', the next is the warp's)
                 kp_ld32<0>(o, col_o + c);
 #pragma unroll
                 for (int k = 0; k < 32; k++) o[k] = fmaf(w[k], f, o[k]);
