@@ -22,16 +22,15 @@
 // product cuts the sum it adds to toward zero at 24 bits, two for 16 positions: sums
 // are off by 2.5e-9 of themselves a position. So those of fp32 outputs leave tensor memory
 // every 512 positions and are added up by rounding additions: 1.6e-6 of the outputs at any length.
-// Us and error, staying / every 2048 / 1024 / 512 positions: two fp32 prompts of 4k 282, 9.9e-6 / 295,
-// 5.2e-6 / 311, 2.8e-6 / 341, 1.6e-6; 512 rows of 40,000 1152, 9.4e-5 / 1188, 5.2e-6 / 1213, 2.8e-6 /
-// 1262, 1.6e-6; six ragged prompts of up to 1200 55, 1.3e-6 / 55 / 63 / 66, 9e-7 (plain fp32 operations:
-// 4.5e-7). Those of fp16 outputs stay: 9.4e-5 of an output at 40,000 positions, half a step is
-// 2.4e-4 and more.
+// Us and error, staying / every 2048 / 1024 / 512 positions: two fp32 prompts of 4k 281, 9.9e-6 / 295,
+// 5.2e-6 / 310, 2.8e-6 / 341, 1.6e-6; six ragged prompts of up to 1200 56, 1.3e-6 / 56 / 63 / 67, 9e-7
+// (plain fp32 operations: 4.5e-7); 512 rows of 40,000 9.4e-5 / 5.2e-6 / 2.8e-6 / 1240 us, 1.6e-6. Those of
+// fp16 outputs stay: 9.4e-5 of an output at 40,000 positions, half a step is 2.4e-4 and more.
 //
 // Bound by the chain scores - maximum - exponentials - weights - outputs of a row tile: tensor
 // pipe 44 %, alu 40 %, exponentials 30 %, issue 50 % busy. Two prompts of 3.9-4.1k, 16 / 8 heads of
-// 128, fp16: 244 us, 556 TFLOP/s; six of up to 512 rows on up to 1200 positions, fp32: 66 us. One
-// row tile spills up to 48 bytes stored and 96 loaded a thread, two up to 8 and 20.
+// 128, fp16: 243 us, 559 TFLOP/s; six of up to 512 rows on up to 1200 positions, fp32: 67 us. Up
+// to 44 bytes are spilled and 72 loaded again a thread (fp32, heads of 32), mostly none.
 #pragma once
 
 #include <stdlib.h>
@@ -92,9 +91,8 @@ struct KpShared {
 // Wait for a phase; gives up after `ns` of waiting or as soon as another role has given up, so
 // that a product that never completes ends the CTA (its rows become NaN, the error word says
 // so). A poll counts as a millisecond at most: a process that the GPU was taken from for a while has not
-// waited. (The polling is a function of its own: inlined in all places, two prompts of 4k in fp16 took
-// 250 us instead of 241.)
-static __device__ __noinline__ bool kp_poll(uint32_t bar, uint32_t parity, volatile int *abort, unsigned long long ns) {
+// waited.
+EMB_DEV bool kp_poll(uint32_t bar, uint32_t parity, volatile int *abort, unsigned long long ns) {
     unsigned long long t0, t1;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
     while (!mbar_try_wait_at(bar, parity)) {
@@ -110,8 +108,17 @@ static __device__ __noinline__ bool kp_poll(uint32_t bar, uint32_t parity, volat
     }
     return true;
 }
+// (The polling is a function of its own where two row tiles need the registers: in line in all places,
+// two prompts of 4k in fp16 took 250 us instead of 241; with one row tile 512 fp32
+// rows of 40,000 took 1326 apart, 1240 in line.)
+static __device__ __noinline__ bool kp_poll_apart(uint32_t bar, uint32_t parity, volatile int *abort,
+                                                  unsigned long long ns) {
+    return kp_poll(bar, parity, abort, ns);
+}
+template <bool APART>
 EMB_DEV bool kp_wait_ns(uint64_t *bar, uint32_t parity, volatile int *abort, unsigned long long ns) {
-    return mbar_try_wait(bar, parity) || kp_poll(smem_u32(bar), parity, abort, ns);
+    return mbar_try_wait(bar, parity) ||
+           (APART ? kp_poll_apart(smem_u32(bar), parity, abort, ns) : kp_poll(smem_u32(bar), parity, abort, ns));
 }
 
 EMB_DEV void kp_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -249,7 +256,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
     const uint32_t tmem = sh.tmem;
     volatile int *abort = &sh.abort;
     auto kp_wait = [&](uint64_t *bar, uint32_t parity, volatile int *flag) {
-        return kp_wait_ns(bar, parity, flag, args.wait_ns);
+        return kp_wait_ns<RT == 2>(bar, parity, flag, args.wait_ns);
     };
 
     if (warp < L::SOFT) {
@@ -651,7 +658,7 @@ __global__ void __launch_bounds__(32 * KpLayout<T, HD, RT>::WARPS, 3 - RT) kv4_p
             int never = 0;
             if (kp_elect()) kp_commit(&sh.drain);
             __syncwarp();
-            kp_wait_ns(&sh.drain, 0, &never, KP_WAIT_NS);
+            kp_wait_ns<RT == 2>(&sh.drain, 0, &never, KP_WAIT_NS);
         }
     } else if (warp < L::KEYS + L::KEY_WARPS) {
         // ------------------------------------------------- keys and values ----
